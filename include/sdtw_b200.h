@@ -44,7 +44,9 @@ typedef int sdtw_status;
 #define SDTW_ERR_BOUNDS 4u     /* debug build (libsdtw_b200_debug.so) only: a kernel's global access fell outside
                                   its buffer and was skipped */
 
-typedef enum { SDTW_F32 = 0, SDTW_F64 = 1 } sdtw_dtype;
+/* SDTW_F16 and SDTW_BF16 are taken by the sequence-model operators (the last three sections); the Soft-DTW
+ * entry points take SDTW_F32 and SDTW_F64. */
+typedef enum { SDTW_F32 = 0, SDTW_F64 = 1, SDTW_F16 = 2, SDTW_BF16 = 3 } sdtw_dtype;
 
 /* Human-readable text of a status. */
 const char* sdtw_status_string(sdtw_status status);
@@ -266,6 +268,104 @@ size_t sdtw_grad_dist_workspace_bytes(int64_t B, int64_t M, sdtw_dtype dtype);
 sdtw_status sdtw_grad_dist(sdtw_dtype dtype, int kind, const void* X, const void* Y, const void* D, const void* E,
                            const void* g, int64_t B, int64_t N, int64_t M, int64_t d, double eps, void* workspace,
                            void* grad_X, void* grad_Y, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------
+ * Operators of a sequence model that trains under the loss. They take SDTW_F32, SDTW_F16 and SDTW_BF16 (the
+ * gradient norm SDTW_F64 too); sums, softmax statistics and norms are kept in 32 bits or more, and an output
+ * is rounded to its type once.
+ *
+ * Cross attention: N queries of a sample attend to the M states of another series.
+ *   s_ij = scale q_i . k_j,  p_i = softmax of s_ij over the cells of row i,  out_i = sum_j p_ij v_j
+ * The cells of row i < nx are the columns of sdtw_band_row_range(i, nx, ny, bandwidth) (all of [0, ny) with
+ * bandwidth < 0), nx = lengths_x[b], ny = lengths_y[b]. Rows i >= nx, and every row when ny = 0, come out as
+ * zeros and have no gradient. q (B, N, Hq, d), k and v (B, M, Hkv, d) have any strides (in elements; batch,
+ * row, head) with neighbouring features; query head h reads key head h / (Hq / Hkv). 1 <= d <= 128. Rows of
+ * q, k and v past the lengths are not used and may hold anything, NaN included; a NaN or infinity inside the
+ * lengths may reach every row of its sample.
+ *   out (B, N, Hq, d), contiguous. lse (B, Hq, N) fp32: log2 of the softmax denominator of s / ln 2 (-inf in
+ *   empty rows). out_lo (optional, 16-bit types): what rounding out to its type dropped, out's type; the
+ *   backward takes p . dp from out + out_lo, which keeps gradients exact where one state holds all the weight.
+ *   A length outside [0, N] / [0, M] raises SDTW_ERR_BAD_LENGTH; that sample's rows are NaN, its gradients 0.
+ *   backward: dout (B, N, Hq, d) with any strides; dq, dk, dv contiguous, each written in full, in one fixed
+ *   order of sums (no atomics). out and lse are the forward's for the same problem.
+ * workspace: *_workspace_bytes(problem) bytes, 256-byte aligned, any content; one call at a time.
+ * ------------------------------------------------------------------------------------------------- */
+typedef struct {
+    sdtw_dtype dtype;
+    int lengths_int32;
+    const void *q, *k, *v;
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+    int64_t B, N, M, Hq, Hkv, d;
+    const void *lengths_x, *lengths_y; /* (B,) or NULL: full */
+    int64_t bandwidth;
+    double scale;
+    uint32_t* err_word;
+} sdtw_attention_problem;
+
+size_t sdtw_cross_attention_workspace_bytes(const sdtw_attention_problem* p);
+sdtw_status sdtw_cross_attention(const sdtw_attention_problem* p, void* out, void* out_lo, float* lse,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+size_t sdtw_cross_attention_backward_workspace_bytes(const sdtw_attention_problem* p);
+sdtw_status sdtw_cross_attention_backward(const sdtw_attention_problem* p, const void* out, const void* out_lo,
+                                          const float* lse, const void* dout, const int64_t* dout_stride, void* dq,
+                                          void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------
+ * RMS norm of every head and the rotation of its features by the position, in one pass over x (B, N, H, d):
+ *   u = x (mean(x^2) + eps)^(-1/2),  z = u weight,  y = R(position) z
+ * R turns pair p of the first `rotary` features by position * base^(-2p / rotary); pairs are features
+ * (p, p + rotary/2), or (2p, 2p + 1) when interleaved. 1 <= d <= 256. weight (d): x's type, or fp32 with
+ * weight_f32; NULL: ones. positions (B, N) by strides: kind 0 fp32, 1 int32, 2 int64; NULL: the row index;
+ * angles are formed in 64 bits. Rows at or past lengths[b] come out as zeros, are not read and have no
+ * gradient; a length outside [0, N] raises SDTW_ERR_BAD_LENGTH (rows NaN, gradients 0). y, dx contiguous.
+ * backward: dx (B, N, H, d), and dweight (d) in weight's type, or NULL; sums in one fixed order.
+ * ------------------------------------------------------------------------------------------------- */
+typedef struct {
+    sdtw_dtype dtype;
+    int weight_f32;
+    const void* x;
+    int64_t x_stride[3]; /* batch, row, head, in elements */
+    int64_t B, N, H, d;
+    const void* weight;
+    const void* lengths; /* (B,) or NULL */
+    int lengths_int32;
+    int position_kind;
+    const void* positions;
+    int64_t position_stride[2];
+    int64_t rotary;
+    int interleaved;
+    double base, eps;
+    uint32_t* err_word;
+} sdtw_rotate_problem;
+
+sdtw_status sdtw_norm_rotate(const sdtw_rotate_problem* p, void* y, void* stream);
+size_t sdtw_norm_rotate_backward_workspace_bytes(int64_t d);
+sdtw_status sdtw_norm_rotate_backward(const sdtw_rotate_problem* p, const void* dy, const int64_t* dy_stride, void* dx,
+                                      void* dweight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------
+ * Global norm of `count` tensors (host array of device pointers), and clipping by it:
+ *   norm = sqrt(sum of squares of all entries)  or  the largest magnitude;
+ *   dst = src * min(1, max_norm / (norm + 1e-6))
+ * dst may be src (then nothing is read or written where the factor is one); no other two ranges may overlap.
+ * norm: one fp64 (norm_f64) or fp32 number. NaN and infinities go into the norm, a NaN norm makes every dst
+ * NaN. Sums run in one fixed order. workspace: sdtw_clip_workspace_bytes(count) bytes, 8-byte aligned.
+ * ------------------------------------------------------------------------------------------------- */
+typedef struct {
+    const void* src;
+    void* dst;
+    int64_t numel;
+    int32_t dtype;
+    int32_t reserved;
+} sdtw_tensor_ref;
+
+#define SDTW_NORM_L2 0
+#define SDTW_NORM_MAX 1
+size_t sdtw_clip_workspace_bytes(int64_t count);
+sdtw_status sdtw_global_norm(const sdtw_tensor_ref* tensors, int64_t count, int norm_kind, void* norm, int norm_f64,
+                             void* workspace, size_t workspace_bytes, void* stream);
+sdtw_status sdtw_clip_grads(const sdtw_tensor_ref* tensors, int64_t count, int norm_kind, double max_norm, void* norm,
+                            int norm_f64, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

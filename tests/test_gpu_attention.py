@@ -1,0 +1,362 @@
+"""GPU: cross attention and its gradients against a plain implementation in 64 bits, elementwise within bounds
+that follow from the roundings the kernels make (sequence_plain.py), at the sizes, masks, layouts and ways of
+calling where they can go wrong."""
+
+import math
+
+import pytest
+import torch
+
+import sequence_plain as plain
+import torchsoftdtw_b200 as T
+from torchsoftdtw_b200 import _ext
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+# B, N, M, Hq, Hkv, d, bandwidth
+SHAPES = [
+    (1, 1, 1, 1, 1, 1, -1),
+    (2, 1, 37, 4, 2, 64, -1),
+    (3, 5, 7, 2, 1, 33, -1),
+    (2, 17, 1, 3, 3, 16, -1),
+    (1, 1, 5000, 8, 1, 128, -1),
+    (5, 3, 777, 6, 2, 80, -1),
+    (2, 40, 600, 4, 4, 64, -1),
+    (2, 128, 128, 2, 2, 64, -1),
+    (2, 129, 257, 4, 2, 64, -1),
+    (1, 200, 130, 2, 2, 128, 8),
+    (2, 130, 300, 4, 1, 80, 0),
+    (2, 64, 64, 2, 2, 96, 3),
+    (2, 300, 200, 2, 1, 40, 32),
+    (1, 511, 513, 1, 1, 127, -1),
+    (2, 1000, 300, 2, 2, 32, 5),
+    (1, 257, 1025, 3, 1, 72, 64),
+    (3, 100, 90, 2, 2, 8, 0),
+]
+
+
+def make(shape, dtype, seed, ragged, train=True):
+    B, N, M, Hq, Hkv, d, _ = shape
+    g = torch.Generator().manual_seed(seed)
+    t = [torch.randn(*s, generator=g, dtype=torch.float64).to(dtype).cuda() * f
+         for s, f in (((B, N, Hq, d), 1.5), ((B, M, Hkv, d), 1.0), ((B, M, Hkv, d), 1.0), ((B, N, Hq, d), 1.0))]
+    if ragged:
+        lx = torch.randint(0, N + 1, (B,), generator=g)
+        ly = torch.randint(0, M + 1, (B,), generator=g)
+        lx[0], ly[0] = N, M
+        if B > 1:
+            lx[1], ly[1] = max(1, N // 2), 1
+        if B > 2:
+            ly[2] = 0
+        for b in range(B):  # nothing past the lengths may be used
+            t[0][b, lx[b]:] = math.nan
+            t[1][b, ly[b]:] = math.nan
+            t[2][b, ly[b]:] = math.inf
+            t[3][b, lx[b]:] = math.nan
+    else:
+        lx, ly = torch.full((B,), N), torch.full((B,), M)
+    return t, lx, ly
+
+
+def run(t, lx, ly, bw, scale=None, given=True, grads=True):
+    q, k, v, dout = t
+    leaves = [x.detach().requires_grad_(grads) for x in (q, k, v)]
+    lens = (lx.cuda(), ly.cuda()) if given else (None, None)
+    out = T.cross_attention(*leaves, *lens, bandwidth=bw, scale=scale)
+    res = {"out": out.detach()}
+    if grads:
+        res.update(zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, dout)))
+    return res
+
+
+def compare(t, lx, ly, bw, res, scale=None):
+    scale = 1 / math.sqrt(t[0].shape[-1]) if scale is None else scale
+    vals, errs = plain.attention(*t[:3], lx, ly, bw, scale, t[3] if "dq" in res else None)
+    for name, got in res.items():
+        plain.check(name, got, vals[name], errs[name])
+
+
+@pytest.mark.parametrize("ragged", [False, True], ids=["full", "ragged"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_values_and_gradients(cuda, shape, dtype, ragged):
+    t, lx, ly = make(shape, dtype, 7, ragged)
+    compare(t, lx, ly, shape[-1], run(t, lx, ly, shape[-1], given=ragged))
+    T.check_errors(cuda)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", [(2, 1, 300, 4, 2, 64, -1), (2, 150, 170, 4, 2, 64, 9)], ids=str)
+def test_forward_alone_is_the_same(cuda, shape, dtype):
+    t, lx, ly = make(shape, dtype, 3, True)
+    a = run(t, lx, ly, shape[-1], grads=False)["out"]
+    b = run(t, lx, ly, shape[-1], grads=True)["out"]
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("layout", ["heads first", "fused", "expanded", "odd stride", "reversed features", "offset"])
+def test_strides(cuda, dtype, layout):
+    B, N, M, H, d, bw = 2, 140, 150, 2, 64, 20
+    g = torch.Generator(device="cuda").manual_seed(5)
+
+    def rnd(*s):
+        return torch.randn(*s, generator=g, device=cuda).to(dtype)
+
+    if layout == "heads first":
+        t = [rnd(B, H, n, d).transpose(1, 2) for n in (N, M, M, N)]
+    elif layout == "fused":
+        kv = rnd(B, M, 2, H, d)
+        t = [rnd(B, N, 3, H, d)[:, :, 1], kv[:, :, 0], kv[:, :, 1], rnd(B, N, H, 2 * d)[..., d:]]
+    elif layout == "expanded":
+        t = [rnd(B, N, H, d), rnd(1, M, H, d).expand(B, M, H, d), rnd(B, M, 1, d).expand(B, M, H, d),
+             rnd(1, 1, 1, d).expand(B, N, H, d)]
+    elif layout == "odd stride":
+        t = [rnd(B, n, H, d + 3)[..., :d] for n in (N, M, M, N)]
+    elif layout == "offset":
+        t = [rnd(B * n * H * d + 1)[1:].view(B, n, H, d) for n in (N, M, M, N)]
+    else:
+        t = [rnd(B, n, d, H).transpose(2, 3) for n in (N, M, M, N)]
+    lx, ly = torch.tensor([N, N - 37]), torch.tensor([M - 3, M])
+    compare(t, lx, ly, bw, run(t, lx, ly, bw))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_one_state_takes_all_weight(cuda, dtype):
+    """M = 1, and a band of one state a row: out is that state, to the bit in 16-bit types; dq and dk are sums of
+    terms that cancel, within the bounds."""
+    for shape in ((2, 150, 1, 2, 1, 64, -1), (2, 400, 20, 2, 2, 64, 0), (1, 1, 1, 8, 2, 128, -1)):
+        t, lx, ly = make(shape, dtype, 11, False)
+        compare(t, lx, ly, shape[-1], run(t, lx, ly, shape[-1]))
+        if shape[2] == 1 and dtype != torch.float32:
+            out = run(t, lx, ly, shape[-1])["out"]
+            assert torch.equal(out, t[2].repeat_interleave(shape[3] // shape[4], 2).expand_as(out))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("N", [1, 130])
+def test_scores_far_from_zero(cuda, dtype, N):
+    """Weights that underflow, and scores of the whole range of a softmax, stay finite and within the bounds."""
+    shape = (1, N, 300, 2, 2, 64, -1)
+    t, lx, ly = make(shape, dtype, 13, False)
+    t[0] *= 20
+    compare(t, lx, ly, -1, run(t, lx, ly, -1))
+    t[1][:, 17] = 0
+    compare(t, lx, ly, -1, run(t, lx, ly, -1, scale=-0.25), scale=-0.25)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", [(3, 1, 70, 4, 2, 64, -1), (3, 200, 70, 4, 2, 64, 4)], ids=str)
+def test_bad_lengths_are_reported(cuda, shape, dtype):
+    T.check_errors(cuda)
+    t, lx, ly = make(shape, dtype, 17, False)
+    for a, b in ((shape[1] + 1, 5), (1, -1)):
+        lx2, ly2 = lx.clone(), ly.clone()
+        lx2[1], ly2[1] = a, b
+        res = run(t, lx2, ly2, shape[-1])
+        assert res["out"][1].isnan().all() and not res["out"][0].isnan().any() and not res["out"][2].isnan().any()
+        for name in ("dq", "dk", "dv"):
+            assert (res[name][1] == 0).all() and res[name].isfinite().all()
+        with pytest.raises(RuntimeError, match="length"):
+            T.check_errors(cuda)
+
+
+def test_int32_and_mixed_lengths(cuda):
+    t, lx, ly = make((3, 40, 50, 2, 2, 32, 6), torch.float32, 19, True)
+    want = run(t, lx, ly, 6)
+    for a, b in ((torch.int32, torch.int32), (torch.int32, torch.int64)):
+        got = run(t, lx.to(a), ly.to(b), 6)
+        assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", [(0, 4, 5, 2, 2, 16, -1), (2, 0, 5, 2, 2, 16, -1), (2, 4, 0, 2, 2, 16, -1)], ids=str)
+def test_empty_sides(cuda, shape, dtype):
+    t, lx, ly = make(shape, dtype, 23, False)
+    res = run(t, lx, ly, -1)
+    for name, like in zip(("out", "dq", "dk", "dv"), (t[0], t[0], t[1], t[2])):
+        assert res[name].shape == like.shape and (res[name] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", [(2, 1, 9000, 8, 2, 64, -1), (2, 300, 280, 4, 2, 128, 30)], ids=str)
+def test_same_bits_every_time(cuda, shape, dtype):
+    t, lx, ly = make(shape, dtype, 29, True)
+    a = run(t, lx, ly, shape[-1])
+    for _ in range(3):
+        b = run(t, lx, ly, shape[-1])
+        assert all(torch.equal(a[n], b[n]) for n in a)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_a_row_alone_is_the_row_among_others(cuda, dtype):
+    """One query a call (a decoded token) gives what the whole series gives, within the two bounds."""
+    shape = (2, 150, 333, 4, 2, 64, -1)
+    t, lx, ly = make(shape, dtype, 31, False)
+    whole = run(t, lx, ly, -1, grads=False)["out"]
+    _, errs = plain.attention(*t[:3], lx, ly, -1, 0.125)
+    for i in (0, 77, 149):
+        row = T.cross_attention(t[0][:, i:i + 1], t[1], t[2])
+        plain.check("row", row[:, 0], whole[:, i].double(), 2 * errs["out"][:, i])
+
+
+@pytest.mark.parametrize("shape", [(2, 1, 2000, 4, 2, 64, -1), (2, 200, 220, 4, 2, 64, 12)], ids=str)
+def test_streams_and_graphs(cuda, shape):
+    """Two calls at once on two streams; then two graphs, captured, replayed on new inputs in turn."""
+    sets = [make(shape, torch.bfloat16, s, True) for s in (37, 41)]
+    want = [run(*s, shape[-1]) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = []
+    for st, s in zip(streams, sets):
+        with torch.cuda.stream(st):
+            got.append([run(*s, shape[-1]) for _ in range(5)][-1])
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(g[n], w[n]) for n in w)
+    (t, lx, ly), (t2, lx2, ly2) = sets
+    graphs = []
+    for _ in range(2):
+        leaves = [x.detach().clone().requires_grad_(True) for x in t[:3]]
+        dout, dlx, dly = t[3].clone(), lx.cuda(), ly.cuda()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = T.cross_attention(*leaves, dlx, dly, bandwidth=shape[-1])
+            grads = torch.autograd.grad(out, leaves, dout)
+        graphs.append((graph, leaves, dout, dlx, dly, [out.detach(), *grads]))
+    for which in (0, 1, 0):
+        for n, (graph, leaves, dout, dlx, dly, outs) in enumerate(graphs):
+            (tt, a, b), w = sets[(which + n) % 2], want[(which + n) % 2]
+            with torch.no_grad():
+                for leaf, x in zip(leaves, tt):
+                    leaf.copy_(x)
+            dout.copy_(tt[3])
+            dlx.copy_(a)
+            dly.copy_(b)
+            graph.replay()
+        torch.cuda.synchronize()
+        for n, (*_, outs) in enumerate(graphs):
+            w = want[(which + n) % 2]
+            for got_t, name in zip(outs, ("out", "dq", "dk", "dv")):
+                assert torch.equal(got_t, w[name]), name
+
+
+def test_compile(cuda):
+    t, lx, ly = make((2, 50, 60, 4, 2, 64, 9), torch.bfloat16, 43, False)
+    w = torch.rand(64, device=cuda)
+
+    def step(q, k, v):
+        return T.cross_attention(T.norm_rotate(q, w), T.norm_rotate(k, w), v, bandwidth=9).float().square().sum()
+
+    grads = []
+    for f in (step, torch.compile(step)):
+        leaves = [x.detach().requires_grad_(True) for x in t[:3]]
+        grads.append(torch.autograd.grad(f(*leaves), leaves))
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
+
+
+def test_offsets_past_32_bits(cuda):
+    """A cache of 2^31 + elements a tensor: the last states are read from their own place."""
+    M, H, d = 1100000, 16, 128
+    k = torch.zeros(1, M, H, d, dtype=torch.bfloat16, device=cuda)
+    v = torch.zeros(1, M, H, d, dtype=torch.bfloat16, device=cuda)
+    assert k.numel() > 2**31
+    q = torch.ones(1, 1, H, d, dtype=torch.bfloat16, device=cuda)
+    k[0, M - 5] = 8.0  # a score of 8 sqrt(128): all the weight but M e^-90
+    v[0, M - 5] = torch.arange(d, device=cuda).to(torch.bfloat16)
+    out = T.cross_attention(q, k, v)
+    assert torch.equal(out, v[:, M - 5].view(1, 1, H, d))
+
+
+def test_differences(cuda):
+    """fp32 gradients against central differences of the kernel's own outputs along random directions. With step
+    h the two results are off by at most 2 e / (2 h) from the outputs' bounds e, and by (4/3) |D(h) - D(h/2)| from
+    the curvature (the error of D falls with h^2; its next term is taken up by the factor 2 instead of 4/3)."""
+    shape = (2, 9, 11, 4, 2, 16, 3)
+    t, lx, ly = make(shape, torch.float32, 47, False)
+    lx[1], ly[1] = 6, 8
+    res = run(t, lx, ly, 3)
+    _, errs = plain.attention(*t[:3], lx, ly, 3, 0.25, t[3])
+    h = 2.0**-5
+    for which, name in enumerate(("dq", "dk", "dv")):
+        direction = torch.randn_like(t[which])
+
+        def loss(step):
+            moved = [x + step * direction if n == which else x for n, x in enumerate(t[:3])]
+            out = T.cross_attention(*moved, lx.cuda(), ly.cuda(), bandwidth=3)
+            return (out.double() * t[3].double()).sum().item()
+
+        D = [(loss(s) - loss(-s)) / (2 * s) for s in (h, h / 2)]
+        noise = 1.5 * (errs["out"] * t[3].double().abs()).sum().item() / (h / 2)
+        slope = (res[name].double() * direction.double()).sum().item()
+        slack = (errs[name] * direction.double().abs()).sum().item()
+        assert abs(D[1] - slope) <= 2 * abs(D[0] - D[1]) + noise + slack, name
+
+
+def test_only_the_wanted_gradients(cuda):
+    t, lx, ly = make((1, 5, 6, 2, 2, 16, -1), torch.float32, 53, False)
+    k = t[1].detach().requires_grad_(True)
+    out = T.cross_attention(t[0], k, t[2])
+    (dk,) = torch.autograd.grad(out.sum(), k, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dk.sum(), k)  # differentiable once
+
+
+def test_a_training_step_together(cuda):
+    """Queries and keys normed and rotated along the diagonal, attention inside the band, the loss on its result,
+    all gradients and their clipping: against the same step in plain 64-bit operations."""
+    B, N, M, H, d, bw = 3, 60, 45, 2, 16, 12
+    g = torch.Generator().manual_seed(59)
+    x, y = torch.randn(B, N, H * d, generator=g).cuda(), torch.randn(B, M, H * d, generator=g).cuda()
+    lx, ly = torch.tensor([60, 41, 7]).cuda(), torch.tensor([45, 30, 45]).cuda()
+    params = [(torch.randn(H * d, H * d, generator=g) * (H * d) ** -0.5).cuda().requires_grad_(True) for _ in range(3)]
+    params += [torch.ones(d, device=cuda, requires_grad=True) for _ in range(2)]
+    pos_y = torch.arange(M, device=cuda) * ((lx - 1) / (ly - 1)).view(B, 1)
+    loss_fn = T.SoftDTW(gamma=1.0, bandwidth=bw, normalize=True)
+
+    def step(plain_step):
+        wq, wk, wv, nq, nk = params
+        q, k, v = ((s @ w).view(B, -1, H, d) for s, w in ((x, wq), (y, wk), (y, wv)))
+        if plain_step:
+            q, k, v = q.double(), k.double(), v.double()
+            ones = torch.ones(B, device=cuda)
+
+            def turned(z, n, pos):
+                z = z / (z.square().mean(-1, keepdim=True) + 1e-6).sqrt() * n.double()
+                a = pos.double().unsqueeze(-1) * 10000.0 ** (-torch.arange(0, d, 2, device=cuda).double() / d)
+                c, s = a.cos().unsqueeze(2), a.sin().unsqueeze(2)
+                f, e = z.chunk(2, -1)
+                return torch.cat((f * c - e * s, f * s + e * c), -1)
+
+            q = turned(q, nq, torch.arange(N, device=cuda) * ones.view(B, 1))
+            k = turned(k, nk, pos_y)
+            mask = plain.cell_mask(B, N, M, lx, ly, bw).cuda().view(B, 1, N, M)
+            s = (torch.einsum("bnhd,bmhd->bhnm", q, k) / math.sqrt(d)).masked_fill(~mask, -1e30)
+            p = torch.where(mask, torch.softmax(s, -1), 0.0)
+            o = torch.einsum("bhnm,bmhd->bnhd", p, v).reshape(B, N, H * d).float()
+        else:
+            q = T.norm_rotate(q, nq, lx)
+            k = T.norm_rotate(k, nk, ly, pos_y)
+            o = T.cross_attention(q, k, v, lx, ly, bandwidth=bw).reshape(B, N, H * d)
+        loss = loss_fn(o, y, lx, ly).sum()
+        return loss, torch.autograd.grad(loss, params)
+
+    loss, grads = step(False)
+    want_loss, want = step(True)
+    # The attention's inputs and outputs agree to fp32 roundings (a few 1e-6 of their size); the loss's own fp32
+    # gradient contract is 1e-5 of the largest entry, and so is each product's after it.
+    torch.testing.assert_close(loss, want_loss, rtol=2e-5, atol=0)
+    for a, b in zip(grads, want):
+        assert (a - b).abs().max() <= 1e-4 * b.abs().max()
+    for p, gr in zip(params, grads):
+        p.grad = gr.clone()
+    norm = T.clip_grad_norm_(params, 0.5)
+    exact = torch.sqrt(sum(b.double().square().sum() for b in grads))
+    assert abs(norm.item() - exact.item()) <= 2**-20 * exact.item()
+    factor = min(1.0, 0.5 / (exact.item() + 1e-6))
+    for p, gr in zip(params, grads):
+        torch.testing.assert_close(p.grad, (gr.double() * factor).float(), rtol=2**-20, atol=0)
+    T.check_errors(cuda)

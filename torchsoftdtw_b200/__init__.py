@@ -1,10 +1,13 @@
 """torchsoftdtw_b200 — a B200-native (sm_100a) Soft-DTW operator with the API of angelo-ortiz/torchsoftdtw.
 
 Public names match the reference's ``torchsoftdtw/__init__.py``; the ops are registered under the same
-``torch.ops.torchsoftdtw`` namespace. All compute runs in this package's CUDA kernels (``lib/``).
+``torch.ops.torchsoftdtw`` namespace. Beside the loss stand operators of the models that train under it
+(``cross_attention``, ``norm_rotate``, ``clip_grads`` and its kin), which the reference does not have. All compute runs in this package's CUDA kernels (``lib/``).
 """
 
 from . import _ext
+from .attention import cross_attention, norm_rotate
+from .clipping import clip_grad_norm_, clip_grads, global_norm
 from .distances import pairwise_cosine, pairwise_l1, pairwise_l2_squared
 from .softdtw import SoftDTW, SoftDTWAutograd, soft_dtw
 
@@ -12,6 +15,11 @@ __all__ = [
     "SoftDTW",
     "SoftDTWAutograd",
     "check_errors",
+    "clip_grad_norm_",
+    "clip_grads",
+    "cross_attention",
+    "global_norm",
+    "norm_rotate",
     "pairwise_cosine",
     "pairwise_l1",
     "pairwise_l2_squared",

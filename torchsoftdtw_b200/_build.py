@@ -6,7 +6,7 @@
 * ``lib/libsdtw_b200_debug.so`` — the same library built with ``-DSDTW_DEBUG_BOUNDS``: the pair-resident
   wavefront kernels check every global access against its buffer and report one outside as the error bit 4
   (``SDTW_ERR_BOUNDS``) instead of performing it. A test build, loaded only through ctypes by the tests.
-* ``_C<ext>.so`` — the PyTorch operator layer (``csrc/torch_ops.cpp``), compiled by the host C++
+* ``_C<ext>.so`` — the PyTorch operator layer (``csrc/torch_*.cpp``), compiled by the host C++
   compiler against libtorch and linked to ``lib/libsdtw_b200.so`` through ``$ORIGIN/lib``.
 
 Both are rebuilt only when a source is newer than the output. Run ``python torchsoftdtw_b200/_build.py`` (as a
@@ -96,13 +96,13 @@ def build_kernels(force: bool = False, debug_bounds: bool = False) -> str:
 
 
 def build_ops(force: bool = False) -> str:
-    """g++: csrc/torch_ops.cpp -> _C.so, linked to lib/libsdtw_b200.so."""
+    """g++: csrc/torch_*.cpp -> _C.so, linked to lib/libsdtw_b200.so."""
     import torch
     from torch.utils import cpp_extension
 
     out = ops_lib_path()
-    src = os.path.join(CSRC, "torch_ops.cpp")
-    deps = [src, os.path.join(INCLUDE, "sdtw_b200.h"), KERNEL_LIB]
+    srcs = sorted(glob.glob(os.path.join(CSRC, "torch_*.cpp")))
+    deps = [*srcs, os.path.join(CSRC, "torch_ops.h"), os.path.join(INCLUDE, "sdtw_b200.h"), KERNEL_LIB]
     if not (force or _stale(out, deps)):
         return out
     torch_dir = os.path.dirname(torch.__file__)
@@ -113,7 +113,7 @@ def build_ops(force: bool = False) -> str:
            "-DTORCH_EXTENSION_NAME=_C", "-I" + INCLUDE, "-I" + cuda_inc]
     for inc in cpp_extension.include_paths():
         cmd.append("-I" + inc)
-    cmd += [src, "-o", out, "-L" + LIBDIR, "-lsdtw_b200", "-Wl,-rpath,$ORIGIN/lib",
+    cmd += [*srcs, "-o", out, "-L" + LIBDIR, "-lsdtw_b200", "-Wl,-rpath,$ORIGIN/lib",
             "-L" + os.path.join(torch_dir, "lib"), "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
             "-Wl,-rpath," + os.path.join(torch_dir, "lib")]
     _run(cmd)

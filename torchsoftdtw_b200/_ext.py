@@ -79,7 +79,43 @@ SIGNATURES: dict[str, tuple] = {
     "sdtw_pairwise_dist": (_i, [_i, _i, _p, _p, _i64, _i64, _i64, _i64, _d, _p, _p]),
     "sdtw_grad_dist_workspace_bytes": (_sz, [_i64, _i64, _i]),
     "sdtw_grad_dist": (_i, [_i, _i, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _d, _p, _p, _p, _p]),
+    "sdtw_cross_attention_workspace_bytes": (_sz, [_p]),
+    "sdtw_cross_attention": (_i, [_p, _p, _p, _p, _p, _sz, _p]),
+    "sdtw_cross_attention_backward_workspace_bytes": (_sz, [_p]),
+    "sdtw_cross_attention_backward": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p]),
+    "sdtw_norm_rotate": (_i, [_p, _p, _p]),
+    "sdtw_norm_rotate_backward_workspace_bytes": (_sz, [_i64]),
+    "sdtw_norm_rotate_backward": (_i, [_p, _p, _p, _p, _p, _p, _sz, _p]),
+    "sdtw_clip_workspace_bytes": (_sz, [_i64]),
+    "sdtw_global_norm": (_i, [_p, _i64, _i, _p, _i, _p, _sz, _p]),
+    "sdtw_clip_grads": (_i, [_p, _i64, _i, _d, _p, _i, _p, _sz, _p]),
 }
+
+
+class AttentionProblem(ctypes.Structure):
+    """sdtw_attention_problem of include/sdtw_b200.h."""
+
+    _fields_ = [("dtype", _i), ("lengths_int32", _i), ("q", _p), ("k", _p), ("v", _p), ("q_stride", _i64 * 3),
+                ("k_stride", _i64 * 3), ("v_stride", _i64 * 3), ("B", _i64), ("N", _i64), ("M", _i64), ("Hq", _i64),
+                ("Hkv", _i64), ("d", _i64), ("lengths_x", _p), ("lengths_y", _p), ("bandwidth", _i64), ("scale", _d),
+                ("err_word", _p)]
+
+
+class RotateProblem(ctypes.Structure):
+    """sdtw_rotate_problem of include/sdtw_b200.h."""
+
+    _fields_ = [("dtype", _i), ("weight_f32", _i), ("x", _p), ("x_stride", _i64 * 3), ("B", _i64), ("N", _i64),
+                ("H", _i64), ("d", _i64), ("weight", _p), ("lengths", _p), ("lengths_int32", _i), ("position_kind", _i),
+                ("positions", _p), ("position_stride", _i64 * 2), ("rotary", _i64), ("interleaved", _i), ("base", _d),
+                ("eps", _d), ("err_word", _p)]
+
+
+class TensorRef(ctypes.Structure):
+    """sdtw_tensor_ref of include/sdtw_b200.h."""
+
+    _fields_ = [("src", _p), ("dst", _p), ("numel", _i64), ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
 # Test and tuning hooks (declared in the .cu, not part of the public header).
 DEBUG_SIGNATURES: dict[str, tuple] = {
     "sdtw_debug_inject_stall": (None, [_i]),

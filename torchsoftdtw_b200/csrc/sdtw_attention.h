@@ -1,0 +1,58 @@
+// The problem of one cross-attention call as the kernels see it.
+#pragma once
+
+#include "sdtw_sequence.cuh"
+
+namespace sdtw {
+
+struct Strides {
+    int64_t b, n, h;
+};
+
+struct AttnArgs {
+    const void *q, *k, *v;
+    Strides qs, ks, vs;
+    int64_t N, M;
+    int B, Hq, Hkv, d, group;  // group = Hq / Hkv
+    Lens lx, ly;
+    int64_t bw;
+    float scale;       // scale of the scores
+    float scale_log2;  // scale / ln 2: the softmax runs in powers of two
+    uint32_t* err;
+    void *out, *out_lo;  // (B, N, Hq, d); out_lo may be null
+    float* lse;          // (B, Hq, N)
+    // backward
+    const void *o, *o_lo;
+    const void* dout;
+    Strides gs;
+    void *dq, *dk, *dv;
+    float* delta;  // (B, Hq, N): sum_j p_ij dp_ij
+};
+
+// The lengths of sample b, and whether one of them is out of range (reported; the sample is then empty).
+__device__ __forceinline__ bool pair_lengths(const AttnArgs& a, int64_t b, int64_t& nx, int64_t& ny)
+{
+    nx = a.lx.get(b, a.N);
+    ny = a.ly.get(b, a.M);
+    if (nx >= 0 && ny >= 0) return true;
+    nx = ny = 0;
+    return false;
+}
+
+// [lo, hi): the columns of row i < nx.
+__device__ __forceinline__ void row_cells(const AttnArgs& a, int64_t i, int64_t nx, int64_t ny, int64_t& lo,
+                                          int64_t& hi)
+{
+    band_row_range(i, nx, ny, a.bw, lo, hi);
+    hi += 1;
+}
+
+// [lo, hi): the rows whose cells include column j < ny (the band is symmetric in its two axes).
+__device__ __forceinline__ void column_cells(const AttnArgs& a, int64_t j, int64_t nx, int64_t ny, int64_t& lo,
+                                             int64_t& hi)
+{
+    band_row_range(j, ny, nx, a.bw, lo, hi);
+    hi += 1;
+}
+
+}  // namespace sdtw

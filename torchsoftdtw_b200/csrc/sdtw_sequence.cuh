@@ -1,0 +1,70 @@
+// Shared device helpers of the sequence-model operators beside the loss (cross attention, head norm with
+// rotation, gradient clipping): element types, per-sample lengths, vector loads.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "sdtw_b200.h"
+#include "sdtw_common.cuh"
+
+namespace sdtw {
+
+inline size_t dtype_size(int dt) { return dt == SDTW_F64 ? 8 : (dt == SDTW_F32 ? 4 : 2); }
+
+// A lengths array (null: every sample is full). get() returns the length of sample b out of `full`, or -1
+// when it lies outside [0, full]; the kernels then treat the sample as bad and report it.
+struct Lens {
+    const void* p;
+    int is32;
+    __device__ __forceinline__ int64_t get(int64_t b, int64_t full) const
+    {
+        if (p == nullptr) return full;
+        const int64_t n =
+            is32 ? static_cast<int64_t>(static_cast<const int*>(p)[b]) : static_cast<const int64_t*>(p)[b];
+        return n < 0 || n > full ? -1 : n;
+    }
+};
+
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+template <typename T>
+__device__ __forceinline__ T from_f(float x);
+template <>
+__device__ __forceinline__ float from_f<float>(float x)
+{
+    return x;
+}
+template <>
+__device__ __forceinline__ __half from_f<__half>(float x)
+{
+    return __float2half_rn(x);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x)
+{
+    return __float2bfloat16_rn(x);
+}
+
+// V elements moved as one access of V * sizeof(T) bytes (16 at most, aligned to that size).
+template <typename T, int V>
+struct alignas(V * sizeof(T)) Vec {
+    T e[V];
+};
+
+__device__ __forceinline__ float warp_sum(float v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    return v;
+}
+__device__ __forceinline__ float warp_maxf(float v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
+    return v;
+}
+
+}  // namespace sdtw

@@ -17,6 +17,7 @@
 #include <unordered_map>
 
 #include "sdtw_b200.h"
+#include "torch_ops.h"
 
 namespace {
 
@@ -64,15 +65,19 @@ Tensor prep_lengths(const Tensor& l, const Tensor& other)
     return l.scalar_type() == other.scalar_type() ? l.contiguous() : l.to(at::kLong).contiguous();
 }
 
+}  // namespace
+
+namespace sdtw_ops {
+
 // One sticky device error word per device, owned by this library for the process lifetime. It is created
 // by the first op call on the device, which must not be under CUDA-graph capture: a word allocated there
 // would come from the graph's private memory pool (and its zero-fill would be a captured memset), and the
 // library would keep a pointer that dies with the graph. A capture that reaches a device without a word
 // raises instead; one eager call before the capture (a warm-up step) creates it.
-uint32_t* error_word(const Tensor& like)
+uint32_t* error_word(const at::Tensor& like)
 {
     static std::mutex mu;
-    static std::unordered_map<int, Tensor> words;
+    static std::unordered_map<int, at::Tensor> words;
     std::lock_guard<std::mutex> lock(mu);
     const int dev = like.get_device();
     auto it = words.find(dev);
@@ -88,7 +93,7 @@ uint32_t* error_word(const Tensor& like)
     return reinterpret_cast<uint32_t*>(it->second.data_ptr<int>());
 }
 
-bool sync_checks_enabled()
+static bool sync_checks_enabled()
 {
     static const bool on = [] {
         const char* v = std::getenv("TORCHSOFTDTW_B200_SYNC_CHECK");
@@ -103,7 +108,7 @@ void check_status(sdtw_status st, const char* what)
 }
 
 // With TORCHSOFTDTW_B200_SYNC_CHECK=1, every op synchronises and raises on a device-side error.
-void maybe_sync_check(const Tensor& like, cudaStream_t stream)
+void maybe_sync_check(const at::Tensor& like, cudaStream_t stream)
 {
     if (!sync_checks_enabled()) return;
     const uint32_t bits = sdtw_read_error_word(error_word(like), stream);
@@ -111,6 +116,14 @@ void maybe_sync_check(const Tensor& like, cudaStream_t stream)
                 (bits & SDTW_ERR_TIMEOUT) ? " (a wait on a neighbouring strip timed out)" : "",
                 (bits & SDTW_ERR_BAD_LENGTH) ? " (a length was outside [0, N] / [0, M])" : "");
 }
+
+}  // namespace sdtw_ops
+
+namespace {
+
+using sdtw_ops::check_status;
+using sdtw_ops::error_word;
+using sdtw_ops::maybe_sync_check;
 
 // band_r: R is read by this library's backward alone (the module path), which needs only part of it.
 std::tuple<Tensor, Tensor> run_forward(const Tensor& Dacc, const Tensor& lx, const Tensor& ly, double gamma,
