@@ -5,7 +5,7 @@
 // The cells of a row are one interval of columns (lengths and band), so every mask is two comparisons.
 #include <cmath>
 
-#include "sdtw_attention.h"
+#include "sdtw_attention_tc.h"
 
 namespace sdtw {
 namespace {
@@ -285,6 +285,9 @@ sdtw_status sdtw_cross_attention(const sdtw_attention_problem* p, void* out, voi
     a.out_lo = out_lo;
     a.lse = lse;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (p->dtype != SDTW_F32 && p->M > 0 && attention_tc_takes(a.q, a.qs, a.B, a.N, a.Hq, a.d) &&
+        attention_tc_takes(a.k, a.ks, a.B, a.M, a.Hkv, a.d) && attention_tc_takes(a.v, a.vs, a.B, a.M, a.Hkv, a.d))
+        return static_cast<sdtw_status>(attention_tc_forward(a, p->dtype == SDTW_BF16, s));
     if (p->dtype == SDTW_F32)
         forward_rows<float>(a, s);
     else if (p->dtype == SDTW_F16)
