@@ -5,6 +5,7 @@
 // The cells of a row are one interval of columns (lengths and band), so every mask is two comparisons.
 #include <cmath>
 
+#include "sdtw_attention_split.h"
 #include "sdtw_attention_tc.h"
 
 namespace sdtw {
@@ -12,66 +13,6 @@ namespace {
 
 constexpr int kRowThreads = 128;  // four warps, a row each
 constexpr int kDMax = 128;
-
-// One warp a query row: lane l scores states j0 + l, the running maximum and sum of the softmax are the
-// warp's, and lane l owns features l, l + 32, .. of the sum.
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(AttnArgs a)
-{
-    __shared__ float qs[kRowThreads / 32][kDMax];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (kRowThreads / 32) + warp;
-    if (row >= static_cast<int64_t>(a.B) * a.Hq * a.N) return;
-    const int64_t i = row % a.N, h = row / a.N % a.Hq, b = row / a.N / a.Hq;
-    int64_t nx, ny, lo = 0, hi = 0;
-    const bool good = pair_lengths(a, b, nx, ny);
-    if (!good && lane == 0) atomicOr(a.err, kErrBadLength);
-    if (i < nx && ny > 0) row_cells(a, i, nx, ny, lo, hi);
-    const T* qr = static_cast<const T*>(a.q) + b * a.qs.b + i * a.qs.n + h * a.qs.h;
-    const T* kb = static_cast<const T*>(a.k) + b * a.ks.b + h / a.group * a.ks.h;
-    const T* vb = static_cast<const T*>(a.v) + b * a.vs.b + h / a.group * a.vs.h;
-    if (hi > lo)
-        for (int f = lane; f < a.d; f += 32) qs[warp][f] = to_f(qr[f]) * a.scale_log2;
-    __syncwarp();
-    float m = -INFINITY, l = 0.f, o[kDMax / 32] = {0.f, 0.f, 0.f, 0.f};
-    for (int64_t j0 = lo; j0 < hi; j0 += 32) {
-        const int64_t j = j0 + lane;
-        float s = -INFINITY;
-        if (j < hi) {
-            const T* kr = kb + j * a.ks.n;
-            s = 0.f;
-            for (int f = 0; f < a.d; ++f) s = fmaf(qs[warp][f], to_f(kr[f]), s);
-        }
-        const float m2 = fmaxf(m, warp_maxf(s));
-        const float base = m2 == -INFINITY ? 0.f : m2;
-        const float p = j < hi ? exp2f(s - base) : 0.f, fix = exp2f(m - base);
-        l = l * fix + warp_sum(p);
-        m = m2;
-#pragma unroll
-        for (int e = 0; e < kDMax / 32; ++e) o[e] *= fix;
-        const int cells = static_cast<int>(hi - j0 < 32 ? hi - j0 : 32);
-        for (int t = 0; t < cells; ++t) {
-            const float pt = __shfl_sync(kFull, p, t);
-            const T* vr = vb + (j0 + t) * a.vs.n;
-#pragma unroll
-            for (int e = 0; e < kDMax / 32; ++e)
-                if (lane + 32 * e < a.d) o[e] = fmaf(pt, to_f(vr[lane + 32 * e]), o[e]);
-        }
-    }
-    const float inv = hi > lo ? 1.f / l : 0.f;
-    T* outr = static_cast<T*>(a.out) + ((b * a.N + i) * a.Hq + h) * a.d;
-    T* lor = a.out_lo ? static_cast<T*>(a.out_lo) + ((b * a.N + i) * a.Hq + h) * a.d : nullptr;
-#pragma unroll
-    for (int e = 0; e < kDMax / 32; ++e) {
-        const int f = lane + 32 * e;
-        if (f >= a.d) continue;
-        const float x = good ? o[e] * inv : __int_as_float(0x7fc00000);
-        const T y = from_f<T>(x);
-        outr[f] = y;
-        if (lor) lor[f] = from_f<T>(good ? x - to_f(y) : 0.f);
-    }
-    if (lane == 0) a.lse[(b * a.Hq + h) * a.N + i] = hi > lo ? m + log2f(l) : -INFINITY;
-}
 
 // One warp a query row: delta, then dq.
 template <typename T>
@@ -198,7 +139,7 @@ sdtw_status checked(const sdtw_attention_problem* p)
     constexpr int64_t kMost = 1 << 24;  // rows of a sample, heads and samples are counted in 32 bits
     if (p->B < 0 || p->N < 0 || p->M < 0 || p->Hq < 1 || p->Hkv < 1 || p->Hq % p->Hkv != 0) return SDTW_EINVAL;
     if (p->B > kMost || p->N > kMost || p->M > kMost || p->Hq > 65535 || p->d < 1 || p->d > kDMax) return SDTW_EINVAL;
-    if (static_cast<double>(p->B) * static_cast<double>(p->Hq) * static_cast<double>(p->N + p->M + 256) > 4e9)
+    if (static_cast<double>(p->B) * static_cast<double>(p->Hq) * static_cast<double>(p->N + p->M + 256) > 2e9)
         return SDTW_EINVAL;  // one warp a row: the rows of all heads fit a grid
     if (!std::isfinite(p->scale)) return SDTW_EINVAL;
     const bool rows = p->B > 0 && p->N > 0, states = p->B > 0 && p->M > 0;
@@ -235,13 +176,6 @@ AttnArgs args_of(const sdtw_attention_problem* p)
 unsigned row_ctas(int64_t rows) { return static_cast<unsigned>((rows + kRowThreads / 32 - 1) / (kRowThreads / 32)); }
 
 template <typename T>
-void forward_rows(const AttnArgs& a, cudaStream_t s)
-{
-    attend_rows_kernel<T><<<row_ctas(static_cast<int64_t>(a.B) * a.Hq * a.N), kRowThreads, 0, s>>>(a);
-    count_launch();
-}
-
-template <typename T>
 void backward_rows(const AttnArgs& a, cudaStream_t s)
 {
     if (a.N > 0) {
@@ -252,6 +186,20 @@ void backward_rows(const AttnArgs& a, cudaStream_t s)
         attend_dkdv_rows_kernel<T><<<row_ctas(static_cast<int64_t>(a.B) * a.Hkv * a.M), kRowThreads, 0, s>>>(a);
         count_launch();
     }
+}
+
+// The tensor-core kernels take 16-bit operands that TMA can read; below kSplitRows packed rows a key head the kernel that
+// splits the states is faster.
+constexpr int64_t kSplitRows = 64;
+
+bool takes_tc(const sdtw_attention_problem* p, const AttnArgs& a)
+{
+    return p->dtype != SDTW_F32 && p->M > 0 && attention_tc_takes(a.q, a.qs, a.B, a.N, a.Hq, a.d) &&
+           attention_tc_takes(a.k, a.ks, a.B, a.M, a.Hkv, a.d) && attention_tc_takes(a.v, a.vs, a.B, a.M, a.Hkv, a.d);
+}
+bool forward_tc(const sdtw_attention_problem* p, const AttnArgs& a)
+{
+    return a.N * a.group > kSplitRows && takes_tc(p, a);
 }
 
 sdtw_status last_error()
@@ -267,8 +215,10 @@ extern "C" {
 
 size_t sdtw_cross_attention_workspace_bytes(const sdtw_attention_problem* p)
 {
-    (void)p;
-    return 0;
+    using namespace sdtw;
+    if (checked(p) != SDTW_OK || p->B == 0 || p->N == 0) return 0;
+    const AttnArgs a = args_of(p);
+    return forward_tc(p, a) ? 0 : attention_split_workspace_bytes(a, p->dtype);
 }
 
 sdtw_status sdtw_cross_attention(const sdtw_attention_problem* p, void* out, void* out_lo, float* lse,
@@ -278,23 +228,15 @@ sdtw_status sdtw_cross_attention(const sdtw_attention_problem* p, void* out, voi
     const sdtw_status st = checked(p);
     if (st != SDTW_OK || p->B == 0 || p->N == 0) return st;
     if (out == nullptr || lse == nullptr) return SDTW_EINVAL;
-    (void)workspace;
-    (void)workspace_bytes;
+    const size_t need = sdtw_cross_attention_workspace_bytes(p);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return SDTW_EWORKSPACE;
     AttnArgs a = args_of(p);
     a.out = out;
     a.out_lo = out_lo;
     a.lse = lse;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (p->dtype != SDTW_F32 && p->M > 0 && attention_tc_takes(a.q, a.qs, a.B, a.N, a.Hq, a.d) &&
-        attention_tc_takes(a.k, a.ks, a.B, a.M, a.Hkv, a.d) && attention_tc_takes(a.v, a.vs, a.B, a.M, a.Hkv, a.d))
-        return static_cast<sdtw_status>(attention_tc_forward(a, p->dtype == SDTW_BF16, s));
-    if (p->dtype == SDTW_F32)
-        forward_rows<float>(a, s);
-    else if (p->dtype == SDTW_F16)
-        forward_rows<__half>(a, s);
-    else
-        forward_rows<__nv_bfloat16>(a, s);
-    return last_error();
+    if (forward_tc(p, a)) return static_cast<sdtw_status>(attention_tc_forward(a, p->dtype == SDTW_BF16, s));
+    return static_cast<sdtw_status>(attention_split_forward(a, p->dtype, workspace, s));
 }
 
 size_t sdtw_cross_attention_backward_workspace_bytes(const sdtw_attention_problem* p)
