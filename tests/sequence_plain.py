@@ -64,6 +64,13 @@ def attention(q, k, v, lx, ly, bandwidth, scale, dout=None):
     w = u if dtype != torch.float32 else 2**-21
     spread = P @ V.abs()
     out_err = (rel + w) * spread
+    # fp16 rounds what lies below 2^-14 by up to 2^-25 whatever its size. The forward keeps weights 2^6 larger than
+    # relative to (at most) the row's largest, which the denominator, at least one, divides: 2^-31 a cell. The backward
+    # keeps P 2^10 larger: 2^-35 a cell; and dS so much larger that the largest |do| of the head's rows is at least 8:
+    # 2^-28 of that |do| a cell.
+    half = float(dtype == torch.float16)
+    cells = mask.double()
+    out_err = out_err + half * 2.0**-31 * (cells @ V.abs())
     vals = {"out": out.transpose(1, 2)}
     errs = {"out": (out_err + u * (out.abs() + out_err)).transpose(1, 2)}
     if dout is None:
@@ -76,12 +83,14 @@ def attention(q, k, v, lx, ly, bandwidth, scale, dout=None):
     # delta comes from the stored output (in two parts: u^2 of it is lost) and carries its error and g(d).
     delta_err = (G.abs() * (out_err + (u * u + (d + 8) * F32) * (out.abs() + out_err))).sum(-1, keepdim=True)
     dS_err = (rel + w) * dS.abs() + P * (1 + rel) * ((2**-21 + (d + 8) * F32) * a + delta_err)
+    peak = G.square().sum(-1).amax(-1).sqrt().view(B, Hkv, rep).amax(-1).repeat_interleave(rep, 1).view(B, H, 1, 1)
+    dS_err = dS_err + half * 2.0**-28 * peak * cells
     long = (2**-21 + (max(N * rep, M) + 8) * F32)  # sums over rows or states
 
     def per_state(x):
         return x.view(B, Hkv, rep, M, d).sum(2).transpose(1, 2)
 
-    dv_err = ((rel + w) * P).transpose(2, 3) @ G.abs() + long * (P.transpose(2, 3) @ G.abs())
+    dv_err = ((rel + w) * P + half * 2.0**-35 * cells).transpose(2, 3) @ G.abs() + long * (P.transpose(2, 3) @ G.abs())
     dq_err = abs(scale) * ((dS_err + long * (dS.abs() + dS_err)) @ K.abs())
     dk_err = abs(scale) * ((dS_err + long * (dS.abs() + dS_err)).transpose(2, 3) @ Q.abs())
     vals.update(dq=(dS @ K * scale).transpose(1, 2), dk=per_state(dS.transpose(2, 3) @ Q * scale),

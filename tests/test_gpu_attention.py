@@ -147,6 +147,18 @@ def test_scores_far_from_zero(cuda, dtype, N):
     compare(t, lx, ly, -1, run(t, lx, ly, -1, scale=-0.25), scale=-0.25)
 
 
+@pytest.mark.parametrize("size", [2.0**-14, 2.0**11])
+def test_small_and_large_gradients_in_fp16(cuda, size):
+    """fp16 gradients of the output far below and above one: dS stays inside the type wherever dq, dk and dv do."""
+    for shape in ((1, 200, 260, 4, 2, 64, -1), (1, 150, 300, 1, 1, 128, 20)):
+        t, lx, ly = make(shape, torch.float16, 61, False)
+        t[3] *= size
+        t[2] *= 4
+        res = run(t, lx, ly, shape[-1])
+        assert all(x.isfinite().all() for x in res.values())
+        compare(t, lx, ly, shape[-1], res)
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("shape", [(3, 1, 70, 4, 2, 64, -1), (3, 200, 70, 4, 2, 64, 4)], ids=str)
 def test_bad_lengths_are_reported(cuda, shape, dtype):

@@ -242,7 +242,8 @@ sdtw_status sdtw_cross_attention(const sdtw_attention_problem* p, void* out, voi
 size_t sdtw_cross_attention_backward_workspace_bytes(const sdtw_attention_problem* p)
 {
     if (sdtw::checked(p) != SDTW_OK) return 0;
-    return static_cast<size_t>(p->B) * p->Hq * p->N * sizeof(float);  // delta
+    // delta, and a word a key head
+    return (static_cast<size_t>(p->B) * p->Hq * p->N + static_cast<size_t>(p->B) * p->Hkv) * sizeof(float);
 }
 
 sdtw_status sdtw_cross_attention_backward(const sdtw_attention_problem* p, const void* out, const void* out_lo,
@@ -268,6 +269,10 @@ sdtw_status sdtw_cross_attention_backward(const sdtw_attention_problem* p, const
     a.dv = dv;
     a.delta = static_cast<float*>(workspace);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (p->N > 0 && takes_tc(p, a) && attention_tc_takes(a.dout, a.gs, a.B, a.N, a.Hq, a.d)) {
+        uint32_t* peak = reinterpret_cast<uint32_t*>(a.delta + static_cast<size_t>(a.B) * a.Hq * a.N);
+        return static_cast<sdtw_status>(attention_tc_backward(a, p->dtype == SDTW_BF16, peak, s));
+    }
     if (p->dtype == SDTW_F32)
         backward_rows<float>(a, s);
     else if (p->dtype == SDTW_F16)

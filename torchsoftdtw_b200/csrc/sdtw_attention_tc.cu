@@ -413,24 +413,6 @@ cudaError_t get_encode(PFN_cuTensorMapEncodeTiled_v12000& fn)
     return cudaSuccess;
 }
 
-// Tiles of 128 rows x 64 features of one head of (B, rows, H, d); what lies outside reads as zero.
-template <typename T>
-bool make_map(PFN_cuTensorMapEncodeTiled_v12000 encode, CUtensorMap* map, const void* ptr, const Strides& st, int64_t B,
-              int64_t rows, int64_t H, int64_t d)
-{
-    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(H),
-                                static_cast<cuuint64_t>(B)};
-    // The stride of a dimension of size one is never used, and may be anything in the caller's tensor.
-    const auto bytes = [](int64_t s, int64_t size) { return static_cast<cuuint64_t>(size == 1 ? 16 : s * 2); };
-    const cuuint64_t strides[3] = {bytes(st.n, rows), bytes(st.h, H), bytes(st.b, B)};
-    const cuuint32_t box[4] = {64, kTile, 1, 1};
-    const cuuint32_t ones[4] = {1, 1, 1, 1};
-    const auto type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    return encode(map, type, 4, const_cast<void*>(ptr), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <typename T, int DPAD, int NT>
 cudaError_t launch_forward(FwdArgs& f, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t s)
 {
@@ -459,12 +441,11 @@ cudaError_t launch_forward(FwdArgs& f, const CUtensorMap& mq, const CUtensorMap&
 template <typename T>
 cudaError_t forward_t(const AttnArgs& a, cudaStream_t s)
 {
-    PFN_cuTensorMapEncodeTiled_v12000 encode;
-    const cudaError_t e = get_encode(encode);
-    if (e != cudaSuccess) return e;
     CUtensorMap mq, mk, mv;
-    if (!make_map<T>(encode, &mq, a.q, a.qs, a.B, a.N, a.Hq, a.d) || !make_map<T>(encode, &mk, a.k, a.ks, a.B, a.M, a.Hkv, a.d) ||
-        !make_map<T>(encode, &mv, a.v, a.vs, a.B, a.M, a.Hkv, a.d))
+    constexpr bool half = std::is_same<T, __half>::value;
+    if (!attention_tile_map(&mq, half, a.q, a.qs, a.B, a.N, a.Hq, a.d, kTile) ||
+        !attention_tile_map(&mk, half, a.k, a.ks, a.B, a.M, a.Hkv, a.d, kTile) ||
+        !attention_tile_map(&mv, half, a.v, a.vs, a.B, a.M, a.Hkv, a.d, kTile))
         return cudaErrorInvalidValue;
     FwdArgs f{};
     f.a = a;
@@ -477,6 +458,23 @@ cudaError_t forward_t(const AttnArgs& a, cudaStream_t s)
 }
 
 }  // namespace
+
+bool attention_tile_map(CUtensorMap* map, bool half, const void* ptr, const Strides& st, int64_t B, int64_t rows, int64_t H,
+                        int64_t d, int box_rows)
+{
+    PFN_cuTensorMapEncodeTiled_v12000 encode;
+    if (get_encode(encode) != cudaSuccess) return false;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(H),
+                                static_cast<cuuint64_t>(B)};
+    // The stride of a dimension of size one is never used, and may be anything in the caller's tensor.
+    const auto bytes = [](int64_t s, int64_t size) { return static_cast<cuuint64_t>(size == 1 ? 16 : s * 2); };
+    const cuuint64_t strides[3] = {bytes(st.n, rows), bytes(st.h, H), bytes(st.b, B)};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1};
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    return encode(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr),
+                  dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 bool attention_tc_takes(const void* p, const Strides& st, int64_t B, int64_t rows, int64_t H, int64_t d)
 {

@@ -1,6 +1,8 @@
 // The tensor-core kernels of cross attention (16-bit operands).
 #pragma once
 
+#include <cuda.h>
+
 #include "sdtw_attention.h"
 
 namespace sdtw {
@@ -8,7 +10,15 @@ namespace sdtw {
 // Whether TMA can read the heads' tiles of this operand: 16-byte steps in every dimension.
 bool attention_tc_takes(const void* p, const Strides& st, int64_t B, int64_t rows, int64_t H, int64_t d);
 
+// TMA map of tiles of box_rows rows x 64 features of one head of (B, rows, H, d), 128-byte swizzle; what lies outside reads
+// as zero.
+bool attention_tile_map(CUtensorMap* map, bool half, const void* ptr, const Strides& st, int64_t B, int64_t rows, int64_t H,
+                        int64_t d, int box_rows);
+
 // out, out_lo and lse of a (M > 0), from q, k and v that attention_tc_takes.
 cudaError_t attention_tc_forward(const AttnArgs& a, bool bf16, cudaStream_t s);
+
+// dq, dk, dv and delta of a (N, M > 0), from q, k, v and dout that attention_tc_takes. peak: (B, Hkv) words, fp16 only.
+cudaError_t attention_tc_backward(const AttnArgs& a, bool bf16, uint32_t* peak, cudaStream_t s);
 
 }  // namespace sdtw

@@ -73,6 +73,18 @@ void lengths_check(const OptTensor& l, int64_t B, const Tensor& like, const char
 // t with neighbouring features, as the kernels read it: t itself, or a contiguous copy.
 Tensor feature_rows(const Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
 
+// t as the tensor-core kernels read it (16-byte steps in every dimension), copied where that is all it lacks: their
+// time is several times less than that of the kernels for any layout, even with the copy.
+Tensor tensor_core_rows(const Tensor& t)
+{
+    const Tensor r = feature_rows(t);
+    if (r.scalar_type() == at::kFloat || r.size(-1) % 8 != 0) return r;
+    bool fits = reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 == 0;
+    for (int i = 0; i < 3; ++i) fits = fits && (r.size(i) == 1 || (r.stride(i) > 0 && r.stride(i) % 8 == 0));
+    if (fits) return r;
+    return r.is_contiguous() ? r.clone(at::MemoryFormat::Contiguous) : r.contiguous();
+}
+
 Tensor workspace_of(size_t bytes, const Tensor& like)
 {
     return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
@@ -110,12 +122,13 @@ struct AttentionCall {
     Tensor q, k, v, lx, ly;  // what p points into
 };
 
+// tensor_core: the call is one that the tensor-core kernels take (a decoded token's cache, for one, is never copied).
 void fill_attention(AttentionCall& c, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& lengths_x,
-                    const OptTensor& lengths_y, int64_t bandwidth, double scale)
+                    const OptTensor& lengths_y, int64_t bandwidth, double scale, bool tensor_core)
 {
-    c.q = feature_rows(q);
-    c.k = feature_rows(k);
-    c.v = feature_rows(v);
+    c.q = tensor_core ? tensor_core_rows(q) : feature_rows(q);
+    c.k = tensor_core ? tensor_core_rows(k) : feature_rows(k);
+    c.v = tensor_core ? tensor_core_rows(v) : feature_rows(v);
     sdtw_attention_problem& p = c.p;
     p.dtype = code_of(q.scalar_type());
     // Both lengths are read with one element type.
@@ -156,7 +169,7 @@ std::tuple<Tensor, Tensor, Tensor> attention_cuda(const Tensor& q, const Tensor&
     attention_checks(q, k, v, lengths_x, lengths_y, scale);
     const c10::cuda::CUDAGuard guard(q.device());
     AttentionCall c;
-    fill_attention(c, q, k, v, lengths_x, lengths_y, bandwidth, scale);
+    fill_attention(c, q, k, v, lengths_x, lengths_y, bandwidth, scale, q.size(1) * (q.size(2) / k.size(2)) > 64);
     const Tensor out = at::empty({c.p.B, c.p.N, c.p.Hq, c.p.d}, q.options());
     const bool lo = need_grad && q.scalar_type() != at::kFloat;
     const Tensor out_lo = lo ? at::empty_like(out) : at::empty({0}, q.options());
@@ -179,7 +192,7 @@ std::tuple<Tensor, Tensor, Tensor> attention_backward_cuda(const Tensor& dout, c
     attention_checks(q, k, v, lengths_x, lengths_y, scale);
     const c10::cuda::CUDAGuard guard(q.device());
     AttentionCall c;
-    fill_attention(c, q, k, v, lengths_x, lengths_y, bandwidth, scale);
+    fill_attention(c, q, k, v, lengths_x, lengths_y, bandwidth, scale, true);
     TORCH_CHECK(dout.sizes() == q.sizes() && dout.scalar_type() == q.scalar_type() && dout.device() == q.device(),
                 "the gradient of the output must have the output's shape, dtype and device");
     TORCH_CHECK(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.device() == q.device() &&
@@ -192,7 +205,7 @@ std::tuple<Tensor, Tensor, Tensor> attention_backward_cuda(const Tensor& dout, c
     TORCH_CHECK(lse.sizes() == at::IntArrayRef({c.p.B, c.p.Hq, c.p.N}) && lse.scalar_type() == at::kFloat &&
                     lse.device() == q.device() && lse.is_contiguous(),
                 "lse is not the forward's");
-    const Tensor g = feature_rows(dout);
+    const Tensor g = tensor_core_rows(dout);
     const int64_t gs[3] = {g.stride(0), g.stride(1), g.stride(2)};
     const Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()),
                  dv = at::empty(v.sizes(), v.options());
