@@ -9,8 +9,7 @@
 // Few rows are bound by reading K and V once, so the rows of a padded mma cost nothing; the splits exist to have every SM
 // read. Up to eight splits form a cluster and join their sums through distributed shared memory, in one launch; more
 // (a single sequence of few heads) leave partial sums in the workspace for a second launch. Both join in split order.
-#include <type_traits>
-
+#include "sdtw_attention_mma.cuh"
 #include "sdtw_attention_split.h"
 
 namespace sdtw {
@@ -41,64 +40,6 @@ struct Geom {
     static constexpr int BYTES = OFF_STATS + 4 * (2 * kWarps * 16 + 2 * ROWS + kClusterMax * ROWS);
 };
 
-__device__ __forceinline__ float tf32(float x)
-{
-    uint32_t r;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-    return __uint_as_float(r);
-}
-__device__ __forceinline__ void split2(float x, uint32_t& head, uint32_t& tail)
-{
-    const float h = tf32(x);
-    head = __float_as_uint(h);
-    tail = __float_as_uint(tf32(x - h));
-}
-__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
-{
-    asm volatile(
-        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <typename T>
-__device__ __forceinline__ void mma_16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
-{
-    if constexpr (std::is_same<T, __half>::value)
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4])
-{
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
-}
-__device__ __forceinline__ void ldmatrix4t(uint32_t addr, uint32_t (&r)[4])
-{
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
-}
-__device__ __forceinline__ uint32_t pack(float lo, float hi, __half)
-{
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ uint32_t pack(float lo, float hi, __nv_bfloat16)
-{
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 __device__ __forceinline__ void cluster_sync()
 {
     asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
@@ -110,26 +51,6 @@ __device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank)
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(p)), "r"(rank));
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
     return v;
-}
-
-// One 16-byte unit of a row (features f ..) from global to shared memory, in pieces of VB bytes; features from d on are
-// not touched (they were cleared), nor read. A row that is not `on` becomes zero.
-template <typename T, int VB>
-__device__ __forceinline__ void copy_unit(T* dst, const T* src, int f, int d, bool on)
-{
-    constexpr int E = VB / static_cast<int>(sizeof(T)), UNIT = 16 / static_cast<int>(sizeof(T));
-#pragma unroll
-    for (int e = 0; e < UNIT; e += E) {
-        if (f + e >= d) break;
-        if constexpr (VB == 16)
-            cp_async_16(dst, src, on ? 16 : 0);
-        else if constexpr (VB == 8)
-            cp_async_8(dst + e, src + e, on ? 8 : 0);
-        else if constexpr (VB == 4)
-            cp_async_4(dst + e, src + e, on ? 4 : 0);
-        else
-            dst[e] = on ? src[e] : from_f<T>(0.f);
-    }
 }
 
 struct SplitArgs {
@@ -259,7 +180,6 @@ __global__ void __launch_bounds__(kThreads, 2) attend_split_kernel(const __grid_
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[x][e] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    const uint32_t q_at = smem_addr(sq + rw * 16 * G::LD);
 
     for (int t = t0; t < t1; ++t) {
         cp_async_wait<G::STAGES - 2>();
@@ -274,41 +194,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_split_kernel(const __grid_
         for (int x = 0; x < G::NK / 8; ++x)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[x][e] = 0.f;
-        if constexpr (!G::F32) {
-            const uint32_t k_at = smem_addr(kt) + 2 * (((lane & 7) + ((lane >> 4) & 1) * 8) * G::LD + ((lane >> 3) & 1) * 8);
-#pragma unroll
-            for (int k = 0; k < DPAD; k += 16) {
-                uint32_t qa[4];
-                ldmatrix4(q_at + 2 * ((lane & 15) * G::LD + (lane >> 4) * 8 + k), qa);
-#pragma unroll
-                for (int x = 0; x < G::NK / 16; ++x) {
-                    uint32_t kk[4];
-                    ldmatrix4(k_at + 2 * (16 * x * G::LD + k), kk);
-                    mma_16<T>(s[2 * x], qa, kk[0], kk[1]);
-                    mma_16<T>(s[2 * x + 1], qa, kk[2], kk[3]);
-                }
-            }
-        } else {
-            const float* qr = reinterpret_cast<const float*>(sq) + (rw * 16 + (lane >> 2)) * G::LD + (lane & 3);
-            const float* kr = reinterpret_cast<const float*>(kt) + (lane >> 2) * G::LD + (lane & 3);
-#pragma unroll 4
-            for (int k = 0; k < DPAD; k += 8) {
-                uint32_t qh[4], ql[4];
-                split2(qr[k], qh[0], ql[0]);
-                split2(qr[8 * G::LD + k], qh[1], ql[1]);
-                split2(qr[k + 4], qh[2], ql[2]);
-                split2(qr[8 * G::LD + k + 4], qh[3], ql[3]);
-#pragma unroll
-                for (int x = 0; x < G::NK / 8; ++x) {
-                    uint32_t bh[2], bl[2];
-                    split2(kr[8 * x * G::LD + k], bh[0], bl[0]);
-                    split2(kr[8 * x * G::LD + k + 4], bh[1], bl[1]);
-                    mma_tf32(s[x], ql, bh[0], bh[1]);
-                    mma_tf32(s[x], qh, bl[0], bl[1]);
-                    mma_tf32(s[x], qh, bh[0], bh[1]);
-                }
-            }
-        }
+        product_rows<T, DPAD, G::LD, G::NK / 8>(s, sq + rw * 16 * G::LD, kt, lane);
         // Scores in powers of two, masked; the row's maximum over the warp's states.
         const int64_t off0 = jw - lo[0], off1 = jw - lo[1];
         const bool inside = off0 >= 0 && off1 >= 0 && jw + G::NK <= hi[0] && jw + G::NK <= hi[1];
@@ -351,42 +237,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_split_kernel(const __grid_
                 s[x][e] = ex2f(s[x][e] - base[e >> 1] + kShift);
                 l[e >> 1] += s[x][e];
             }
-        if constexpr (!G::F32) {
-            const uint32_t v_at = smem_addr(vt) + 2 * (((lane & 7) + ((lane >> 3) & 1) * 8) * G::LD + ((lane >> 4) & 1) * 8);
-#pragma unroll
-            for (int x = 0; x < G::NK / 16; ++x) {
-                const uint32_t pa[4] = {pack(s[2 * x][0], s[2 * x][1], T()), pack(s[2 * x][2], s[2 * x][3], T()),
-                                        pack(s[2 * x + 1][0], s[2 * x + 1][1], T()),
-                                        pack(s[2 * x + 1][2], s[2 * x + 1][3], T())};
-#pragma unroll
-                for (int y = 0; y < DPAD / 16; ++y) {
-                    uint32_t vv[4];
-                    ldmatrix4t(v_at + 2 * (16 * x * G::LD + 16 * y), vv);
-                    mma_16<T>(o[2 * y], pa, vv[0], vv[1]);
-                    mma_16<T>(o[2 * y + 1], pa, vv[2], vv[3]);
-                }
-            }
-        } else {
-            // The accumulator's columns 2t, 2t + 1 serve as the operand's K = t, t + 4; V's rows are taken in that order.
-            const float* vr = reinterpret_cast<const float*>(vt) + 2 * (lane & 3) * G::LD + (lane >> 2);
-#pragma unroll
-            for (int x = 0; x < G::NK / 8; ++x) {
-                uint32_t ph[4], pl[4];
-                split2(s[x][0], ph[0], pl[0]);
-                split2(s[x][2], ph[1], pl[1]);
-                split2(s[x][1], ph[2], pl[2]);
-                split2(s[x][3], ph[3], pl[3]);
-#pragma unroll
-                for (int y = 0; y < DPAD / 8; ++y) {
-                    uint32_t bh[2], bl[2];
-                    split2(vr[8 * x * G::LD + 8 * y], bh[0], bl[0]);
-                    split2(vr[(8 * x + 1) * G::LD + 8 * y], bh[1], bl[1]);
-                    mma_tf32(o[y], pl, bh[0], bh[1]);
-                    mma_tf32(o[y], ph, bl[0], bl[1]);
-                    mma_tf32(o[y], ph, bh[0], bh[1]);
-                }
-            }
-        }
+        product_columns<T, DPAD, G::LD, G::NK / 8>(o, s, vt, lane);
     }
     cp_async_wait<0>();
     constexpr float kUnshift = std::is_same<T, __half>::value ? 0x1p-10f : 1.f;
@@ -611,12 +462,7 @@ template <typename T>
 cudaError_t forward_t(SplitArgs& f, const Plan& p, cudaStream_t s)
 {
     const AttnArgs& a = f.a;
-    // The largest piece that every row starts on a multiple of.
-    const int64_t es = sizeof(T);
-    uintptr_t bits = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
-                     static_cast<uintptr_t>(a.d * es);
-    for (const Strides* st : {&a.qs, &a.ks, &a.vs}) bits |= static_cast<uintptr_t>((st->b | st->n | st->h) * es);
-    const int vb = bits % 16 == 0 ? 16 : (bits % 4 == 0 ? 4 : 2);
+    const int vb = copy_bytes(step_bits<T>(a.q, a.qs) | step_bits<T>(a.k, a.ks) | step_bits<T>(a.v, a.vs) | a.d * sizeof(T));
     return p.row_warps == 1 ? launch_d<T, 1>(f, vb, s) : launch_d<T, 4>(f, vb, s);
 }
 

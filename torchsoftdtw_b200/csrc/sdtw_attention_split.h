@@ -1,4 +1,4 @@
-// Cross attention with the states split over CTAs: few query rows, and float32 (any strides, any alignment).
+// Cross attention on warp-level mma: few query rows (states split over CTAs), float32, and any strides and alignment.
 #pragma once
 
 #include "sdtw_attention.h"
@@ -9,5 +9,8 @@ size_t attention_split_workspace_bytes(const AttnArgs& a, int dtype);
 
 // out, out_lo and lse of a (B, N > 0).
 cudaError_t attention_split_forward(const AttnArgs& a, int dtype, void* workspace, cudaStream_t s);
+
+// dq, dk, dv and delta of a (B > 0). peak: (B, Hkv) words, fp16 only.
+cudaError_t attention_mma_backward(const AttnArgs& a, int dtype, uint32_t* peak, cudaStream_t s);
 
 }  // namespace sdtw
