@@ -282,7 +282,7 @@ sdtw_status sdtw_grad_dist(sdtw_dtype dtype, int kind, const void* X, const void
  * row, head) with neighbouring features; query head h reads key head h / (Hq / Hkv). 1 <= d <= 128. Rows of
  * q, k and v past the lengths are not used and may hold anything, NaN included; a NaN or infinity inside the
  * lengths may reach every row of its sample.
- *   out (B, N, Hq, d), contiguous. lse (B, Hq, N) fp32: log2 of the softmax denominator of s / ln 2 (-inf in
+ *   out (B, N, Hq, d), contiguous. lse (B, Hq, N) fp32 (optional, the backward needs it): log2 of the softmax denominator of s / ln 2 (-inf in
  *   empty rows). out_lo (optional, 16-bit types): what rounding out to its type dropped, out's type; the
  *   backward takes p . dp from out + out_lo, which keeps gradients exact where one state holds all the weight.
  *   A length outside [0, N] / [0, M] raises SDTW_ERR_BAD_LENGTH; that sample's rows are NaN, its gradients 0.

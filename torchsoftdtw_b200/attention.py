@@ -2,14 +2,12 @@
 
 The operators of a model that trains under the loss. They take the loss's own pair contract: per-sample
 ``lengths_x`` / ``lengths_y`` and the Sakoe-Chiba ``bandwidth``, with features split into heads. All compute runs
-in this library's CUDA kernels (``torchsoftdtw_b200::attention``, ``norm_rotate`` and their backward ops).
+in this library's CUDA kernels (``torchsoftdtw_b200::cross_attention``, ``norm_rotate`` and their backward ops, autograd included).
 """
 
 import math
 
 import torch
-from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _ext
 
@@ -19,11 +17,16 @@ _ext.load()
 # ---- FakeTensor kernels for torch.compile ----
 
 
+@torch.library.register_fake("torchsoftdtw_b200::cross_attention")
+def _cross_attention_fake(q, k, v, lengths_x, lengths_y, bandwidth, scale):
+    return q.new_empty(q.shape)
+
+
 @torch.library.register_fake("torchsoftdtw_b200::attention")
-def _attention_fake(q, k, v, lengths_x, lengths_y, bandwidth, scale, need_grad):
+def _attention_fake(q, k, v, lengths_x, lengths_y, bandwidth, scale):
     B, N, H, _ = q.shape
-    lo = need_grad and q.dtype != torch.float32
-    return (q.new_empty(q.shape), q.new_empty(q.shape if lo else (0,)), q.new_empty((B, H, N), dtype=torch.float32))
+    lo = q.new_empty((0,) if q.dtype == torch.float32 else q.shape)
+    return q.new_empty(q.shape), lo, q.new_empty((B, H, N), dtype=torch.float32)
 
 
 @torch.library.register_fake("torchsoftdtw_b200::attention_backward")
@@ -40,50 +43,6 @@ def _norm_rotate_fake(x, weight, lengths, positions, rotary_dim, base, interleav
 def _norm_rotate_backward_fake(dy, x, weight, lengths, positions, rotary_dim, base, interleaved, eps, need_weight):
     dw = weight.new_empty(weight.shape) if need_weight and weight is not None else x.new_empty((0,))
     return x.new_empty(x.shape), dw
-
-
-class _CrossAttention(Function):
-    @staticmethod
-    @torch.amp.custom_fwd(device_type="cuda")
-    def forward(ctx, q, k, v, lengths_x, lengths_y, bandwidth, scale):
-        out, out_lo, lse = torch.ops.torchsoftdtw_b200.attention(q, k, v, lengths_x, lengths_y, bandwidth, scale, True)
-        ctx.save_for_backward(q, k, v, out, out_lo, lse, lengths_x, lengths_y)
-        ctx.bandwidth, ctx.scale = bandwidth, scale
-        return out
-
-    @staticmethod
-    @once_differentiable
-    @torch.amp.custom_bwd(device_type="cuda")
-    def backward(ctx, dout):
-        q, k, v, out, out_lo, lse, lengths_x, lengths_y = ctx.saved_tensors
-        dq, dk, dv = torch.ops.torchsoftdtw_b200.attention_backward(
-            dout, q, k, v, out, out_lo, lse, lengths_x, lengths_y, ctx.bandwidth, ctx.scale)
-        need = ctx.needs_input_grad
-        return (dq if need[0] else None), (dk if need[1] else None), (dv if need[2] else None), None, None, None, None
-
-
-class _NormRotate(Function):
-    @staticmethod
-    @torch.amp.custom_fwd(device_type="cuda")
-    def forward(ctx, x, weight, lengths, positions, rotary_dim, base, interleaved, eps):
-        out = torch.ops.torchsoftdtw_b200.norm_rotate(x, weight, lengths, positions, rotary_dim, base, interleaved, eps)
-        ctx.save_for_backward(x, weight, lengths, positions)
-        ctx.options = (rotary_dim, base, interleaved, eps)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    @torch.amp.custom_bwd(device_type="cuda")
-    def backward(ctx, dy):
-        x, weight, lengths, positions = ctx.saved_tensors
-        need_x, need_w = ctx.needs_input_grad[:2]
-        dx, dw = torch.ops.torchsoftdtw_b200.norm_rotate_backward(dy, x, weight, lengths, positions, *ctx.options,
-                                                                  bool(need_w))
-        return (dx if need_x else None), (dw if need_w else None), None, None, None, None, None, None
-
-
-def _grad_wanted(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def cross_attention(
@@ -119,9 +78,7 @@ def cross_attention(
     """
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1]) if q.dim() > 0 and q.shape[-1] > 0 else 1.0
-    if _grad_wanted(q, k, v):
-        return _CrossAttention.apply(q, k, v, lengths_x, lengths_y, bandwidth, scale)
-    return torch.ops.torchsoftdtw_b200.attention(q, k, v, lengths_x, lengths_y, bandwidth, scale, False)[0]
+    return torch.ops.torchsoftdtw_b200.cross_attention(q, k, v, lengths_x, lengths_y, bandwidth, scale)
 
 
 def norm_rotate(
@@ -157,6 +114,4 @@ def norm_rotate(
     """
     if rotary_dim is None:
         rotary_dim = x.shape[-1] // 2 * 2 if x.dim() > 0 else 0
-    if _grad_wanted(x, weight):
-        return _NormRotate.apply(x, weight, lengths, positions, rotary_dim, base, interleaved, eps)
     return torch.ops.torchsoftdtw_b200.norm_rotate(x, weight, lengths, positions, rotary_dim, base, interleaved, eps)

@@ -27,7 +27,6 @@ def _clip_grads_fake(grads, out, max_norm, norm_type):
     return grads[0].new_empty((), dtype=torch.float64 if wide else torch.float32)
 
 
-@torch.no_grad()
 def global_norm(tensors: Sequence[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
     """The norm of all entries of all tensors together.
 
@@ -45,7 +44,6 @@ def global_norm(tensors: Sequence[torch.Tensor], norm_type: float = 2.0) -> torc
     return torch.ops.torchsoftdtw_b200.global_norm(tensors, float(norm_type))
 
 
-@torch.no_grad()
 def clip_grads(
     grads: Sequence[torch.Tensor],
     max_norm: float,
@@ -78,7 +76,6 @@ def clip_grads(
     return out, norm
 
 
-@torch.no_grad()
 def clip_grad_norm_(
     parameters: torch.Tensor | Iterable[torch.Tensor],
     max_norm: float,

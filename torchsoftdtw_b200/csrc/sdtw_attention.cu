@@ -88,7 +88,7 @@ sdtw_status sdtw_cross_attention(const sdtw_attention_problem* p, void* out, voi
     using namespace sdtw;
     const sdtw_status st = checked(p);
     if (st != SDTW_OK || p->B == 0 || p->N == 0) return st;
-    if (out == nullptr || lse == nullptr) return SDTW_EINVAL;
+    if (out == nullptr) return SDTW_EINVAL;
     const size_t need = sdtw_cross_attention_workspace_bytes(p);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return SDTW_EWORKSPACE;
     AttnArgs a = args_of(p);

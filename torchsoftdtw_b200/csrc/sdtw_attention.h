@@ -20,7 +20,7 @@ struct AttnArgs {
     float scale_log2;  // scale / ln 2: the softmax runs in powers of two
     uint32_t* err;
     void *out, *out_lo;  // (B, N, Hq, d); out_lo may be null
-    float* lse;          // (B, Hq, N)
+    float* lse;          // (B, Hq, N); the forward's may be null
     // backward
     const void *o, *o_lo;
     const void* dout;

@@ -76,6 +76,7 @@ __device__ __forceinline__ void store_out(const AttnArgs& a, int b, int hk, int6
 }
 __device__ __forceinline__ void store_lse(const AttnArgs& a, int b, int hk, int64_t r, float v)
 {
+    if (!a.lse) return;
     const int64_t n = r / a.group;
     const int h = hk * a.group + static_cast<int>(r % a.group);
     a.lse[(static_cast<int64_t>(b) * a.Hq + h) * a.N + n] = v;

@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(Geom<DPAD, NT>::THREADS, NT == 1 ? 2 : 1)
             }
             if (i < a.N) store_row32<T>(out, out_lo, v, c, a.d);
         }
-        if (i < a.N)
+        if (i < a.N && a.lse)
             a.lse[(static_cast<int64_t>(b) * a.Hq + h) * a.N + i] = width > 0 ? fmaf(m, sl, log2f(sum) - kShift) : -INFINITY;
         fence_before();
     }

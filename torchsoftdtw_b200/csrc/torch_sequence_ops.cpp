@@ -1,9 +1,12 @@
-// PyTorch operator layer of the sequence-model operators beside the loss: torchsoftdtw_b200::attention /
-// attention_backward, norm_rotate / norm_rotate_backward, global_norm / clip_grads. It checks arguments,
-// allocates outputs and workspaces, and forwards every call to the C ABI (include/sdtw_b200.h).
+// PyTorch operator layer of the sequence-model operators beside the loss: torchsoftdtw_b200::cross_attention (with
+// attention / attention_backward below autograd), norm_rotate / norm_rotate_backward, global_norm / clip_grads. It
+// checks arguments, allocates outputs and workspaces, and forwards every call to the C ABI (include/sdtw_b200.h).
+// Autograd is in C++: at these kernels' times, a training step through Python functions would be bound by the host
+// (about 100 us a step against 45 us of kernels at 32 x 512 x 8 x 64).
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -161,26 +164,46 @@ void fill_attention(AttentionCall& c, const Tensor& q, const Tensor& k, const Te
     p.err_word = error_word(q);
 }
 
-// Returns (out, out_lo, lse); out_lo is empty unless need_grad and the type has 16 bits.
-std::tuple<Tensor, Tensor, Tensor> attention_cuda(const Tensor& q, const Tensor& k, const Tensor& v,
-                                                  const OptTensor& lengths_x, const OptTensor& lengths_y,
-                                                  int64_t bandwidth, double scale, bool need_grad)
+// The forward; with `grad`, also what the backward needs: out_lo (16-bit types) and lse.
+Tensor attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& lengths_x,
+                         const OptTensor& lengths_y, int64_t bandwidth, double scale, bool grad, Tensor* out_lo, Tensor* lse)
 {
     attention_checks(q, k, v, lengths_x, lengths_y, scale);
     const c10::cuda::CUDAGuard guard(q.device());
     AttentionCall c;
     fill_attention(c, q, k, v, lengths_x, lengths_y, bandwidth, scale, q.size(1) * (q.size(2) / k.size(2)) > 64);
     const Tensor out = at::empty({c.p.B, c.p.N, c.p.Hq, c.p.d}, q.options());
-    const bool lo = need_grad && q.scalar_type() != at::kFloat;
-    const Tensor out_lo = lo ? at::empty_like(out) : at::empty({0}, q.options());
-    const Tensor lse = at::empty({c.p.B, c.p.Hq, c.p.N}, q.options().dtype(at::kFloat));
+    void* lo_ptr = nullptr;
+    float* lse_ptr = nullptr;
+    if (grad) {
+        *lse = at::empty({c.p.B, c.p.Hq, c.p.N}, q.options().dtype(at::kFloat));
+        lse_ptr = lse->data_ptr<float>();
+        const bool lo = q.scalar_type() != at::kFloat;
+        *out_lo = lo ? at::empty({c.p.B, c.p.N, c.p.Hq, c.p.d}, q.options()) : at::empty({0}, q.options());
+        if (lo) lo_ptr = out_lo->data_ptr();
+    }
     const size_t wsb = sdtw_cross_attention_workspace_bytes(&c.p);
     const Tensor ws = wsb > 0 ? workspace_of(wsb, q) : Tensor();
     const cudaStream_t stream = stream_of(q);
-    check_status(sdtw_cross_attention(&c.p, out.data_ptr(), lo ? out_lo.data_ptr() : nullptr, lse.data_ptr<float>(),
-                                      wsb > 0 ? ws.data_ptr() : nullptr, wsb, stream),
+    check_status(sdtw_cross_attention(&c.p, out.data_ptr(), lo_ptr, lse_ptr, wsb > 0 ? ws.data_ptr() : nullptr, wsb, stream),
                  "cross_attention");
     maybe_sync_check(q, stream);
+    return out;
+}
+
+Tensor cross_attention_cuda(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& lengths_x,
+                            const OptTensor& lengths_y, int64_t bandwidth, double scale)
+{
+    return attention_forward(q, k, v, lengths_x, lengths_y, bandwidth, scale, false, nullptr, nullptr);
+}
+
+// Returns (out, out_lo, lse); out_lo is empty for float32.
+std::tuple<Tensor, Tensor, Tensor> attention_cuda(const Tensor& q, const Tensor& k, const Tensor& v,
+                                                  const OptTensor& lengths_x, const OptTensor& lengths_y,
+                                                  int64_t bandwidth, double scale)
+{
+    Tensor out_lo, lse;
+    const Tensor out = attention_forward(q, k, v, lengths_x, lengths_y, bandwidth, scale, true, &out_lo, &lse);
     return {out, out_lo, lse};
 }
 
@@ -351,17 +374,16 @@ bool tensor_checks(at::TensorList ts)
     return wide;
 }
 
-Tensor dense(const Tensor& t) { return t.is_non_overlapping_and_dense() ? t : t.contiguous(); }
+bool is_dense(const Tensor& t) { return t.is_contiguous() || t.is_non_overlapping_and_dense(); }
 
-sdtw_tensor_ref ref_of(const Tensor& src, const Tensor& dst)
+sdtw_tensor_ref ref_of(const Tensor& src, void* dst)
 {
-    return {src.data_ptr(), dst.defined() ? dst.data_ptr() : nullptr, src.numel(),
-            static_cast<int32_t>(code_of(src.scalar_type())), 0};
+    return {src.data_ptr(), dst, src.numel(), static_cast<int32_t>(code_of(src.scalar_type())), 0};
 }
 
 Tensor norm_result(const Tensor& like, bool wide)
 {
-    return at::empty({}, like.options().dtype(wide ? at::kDouble : at::kFloat).layout(at::kStrided));
+    return at::empty({}, like.options().dtype(wide ? at::kDouble : at::kFloat));
 }
 
 Tensor global_norm_cuda(at::TensorList tensors, double norm_type)
@@ -372,9 +394,10 @@ Tensor global_norm_cuda(at::TensorList tensors, double norm_type)
     const c10::cuda::CUDAGuard guard(tensors[0].device());
     std::vector<Tensor> keep;
     std::vector<sdtw_tensor_ref> refs;
+    refs.reserve(tensors.size());
     for (const Tensor& t : tensors) {
-        keep.push_back(dense(t));
-        refs.push_back(ref_of(keep.back(), Tensor()));
+        if (!is_dense(t)) keep.push_back(t.contiguous());
+        refs.push_back(ref_of(is_dense(t) ? t : keep.back(), nullptr));
     }
     const Tensor norm = norm_result(tensors[0], wide);
     const size_t wsb = sdtw_clip_workspace_bytes(static_cast<int64_t>(refs.size()));
@@ -394,36 +417,48 @@ Tensor clip_grads_cuda(at::TensorList grads, at::TensorList out, double max_norm
     TORCH_CHECK(grads.size() == out.size(), "out must hold one tensor for each gradient, got ", num(out.size()), " for ",
                 num(grads.size()));
     const bool wide = tensor_checks(grads);
-    tensor_checks(out);
     const c10::cuda::CUDAGuard guard(grads[0].device());
     struct Range {
         uintptr_t begin, end;
-        bool written;
         size_t index;
+        bool written;
     };
     std::vector<Range> ranges;
-    std::vector<Tensor> src, dst;
+    std::vector<Tensor> keep;                          // copies of gradients that are not dense
+    std::vector<std::pair<size_t, Tensor>> later;      // results that are copied to out[i] at the end
     std::vector<sdtw_tensor_ref> refs;
+    ranges.reserve(2 * grads.size());
+    refs.reserve(grads.size());
     const auto range_of = [](const Tensor& t, bool written, size_t i) {
-        int64_t last = 0;
-        for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+        int64_t last = t.is_contiguous() ? t.numel() - 1 : 0;
+        if (!t.is_contiguous())
+            for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
         const uintptr_t p = reinterpret_cast<uintptr_t>(t.data_ptr());
-        return Range{p, p + static_cast<uintptr_t>(last + 1) * t.element_size(), written, i};
+        return Range{p, p + static_cast<uintptr_t>(last + 1) * t.element_size(), i, written};
     };
     for (size_t i = 0; i < grads.size(); ++i) {
         const Tensor &g = grads[i], &o = out[i];
-        TORCH_CHECK(o.sizes() == g.sizes() && o.scalar_type() == g.scalar_type() && o.device() == g.device(),
+        TORCH_CHECK(o.sizes() == g.sizes() && o.scalar_type() == g.scalar_type() && o.device() == g.device() &&
+                        o.layout() == at::kStrided,
                     "out[", num(i), "] must have the gradient's shape, dtype and device");
+        const bool alike = o.strides() == g.strides();
         if (g.numel() > 0) {
-            const bool same = o.data_ptr() == g.data_ptr() && o.strides() == g.strides();
             ranges.push_back(range_of(o, true, i));
-            if (!same) ranges.push_back(range_of(g, false, i));
+            if (!alike || o.data_ptr() != g.data_ptr()) ranges.push_back(range_of(g, false, i));
         }
-        src.push_back(dense(g));
         // Results that are not laid out as their gradient are scaled into a buffer that is, then copied.
-        const bool direct = o.is_non_overlapping_and_dense() && o.strides() == src.back().strides();
-        dst.push_back(direct ? o : at::empty_like(src.back()));
-        refs.push_back(ref_of(src.back(), dst.back()));
+        if (alike && is_dense(g)) {
+            refs.push_back(ref_of(g, o.data_ptr()));
+        } else {
+            if (!is_dense(g)) keep.push_back(g.contiguous());
+            const Tensor& src = is_dense(g) ? g : keep.back();
+            if (is_dense(o) && o.strides() == src.strides()) {
+                refs.push_back(ref_of(src, o.data_ptr()));
+            } else {
+                later.emplace_back(i, at::empty_like(src));
+                refs.push_back(ref_of(src, later.back().second.data_ptr()));
+            }
+        }
     }
     std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
     uintptr_t read_end = 0, write_end = 0;
@@ -438,19 +473,197 @@ Tensor clip_grads_cuda(at::TensorList grads, at::TensorList out, double max_norm
     check_status(sdtw_clip_grads(refs.data(), static_cast<int64_t>(refs.size()), kind, max_norm, norm.data_ptr(), wide,
                                  ws.data_ptr(), wsb, stream_of(grads[0])),
                  "clip_grads");
-    for (size_t i = 0; i < out.size(); ++i)
-        if (out[i].numel() > 0 && dst[i].data_ptr() != out[i].data_ptr()) out[i].copy_(dst[i]);
+    for (const auto& [i, t] : later)
+        if (t.numel() > 0) out[i].copy_(t);
+    for (const Tensor& o : out)
+        if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
     return norm;
 }
 
-// Argument errors of CPU tensors read like those of CUDA ones; then they are rejected.
-std::tuple<Tensor, Tensor, Tensor> attention_cpu(const Tensor& q, const Tensor& k, const Tensor& v,
-                                                 const OptTensor& lengths_x, const OptTensor& lengths_y,
-                                                 int64_t bandwidth, double scale, bool need_grad)
+// ---------------------------------------------------------------------------------------------------
+// Autograd
+// ---------------------------------------------------------------------------------------------------
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+template <typename F>
+auto typed_op(const char* name)
+{
+    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+const auto& attention_op()
+{
+    static const auto op = typed_op<decltype(attention_cuda)>("torchsoftdtw_b200::attention");
+    return op;
+}
+const auto& cross_attention_op()
+{
+    static const auto op = typed_op<decltype(cross_attention_cuda)>("torchsoftdtw_b200::cross_attention");
+    return op;
+}
+const auto& attention_backward_op()
+{
+    static const auto op = typed_op<decltype(attention_backward_cuda)>("torchsoftdtw_b200::attention_backward");
+    return op;
+}
+const auto& norm_rotate_op()
+{
+    static const auto op = typed_op<decltype(norm_rotate_cuda)>("torchsoftdtw_b200::norm_rotate");
+    return op;
+}
+const auto& norm_rotate_backward_op()
+{
+    static const auto op = typed_op<decltype(norm_rotate_backward_cuda)>("torchsoftdtw_b200::norm_rotate_backward");
+    return op;
+}
+
+OptTensor optional_of(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+Tensor tensor_of(const OptTensor& t) { return t ? *t : Tensor(); }
+bool wants_grad(std::initializer_list<Tensor> ts)
+{
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor& t : ts)
+        if (t.defined() && t.requires_grad()) return true;
+    return false;
+}
+
+// The gradients themselves are not differentiable: differentiating them raises.
+variable_list twice(const char* name)
+{
+    TORCH_CHECK(false, name, " is differentiable once; its gradients have no gradient");
+    return {};
+}
+
+struct AttentionBackward : torch::autograd::Function<AttentionBackward> {
+    static variable_list forward(AutogradContext*, const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v,
+                                 const Tensor& out, const Tensor& out_lo, const Tensor& lse, const OptTensor& lx,
+                                 const OptTensor& ly, int64_t bandwidth, double scale)
+    {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        auto [dq, dk, dv] = attention_backward_op().call(dout, q, k, v, out, out_lo, lse, lx, ly, bandwidth, scale);
+        return {dq, dk, dv};
+    }
+    static variable_list backward(AutogradContext*, const variable_list&) { return twice("cross_attention"); }
+};
+
+std::tuple<Tensor, Tensor, Tensor> attention_backward_autograd(const Tensor& dout, const Tensor& q, const Tensor& k,
+                                                               const Tensor& v, const Tensor& out, const Tensor& out_lo,
+                                                               const Tensor& lse, const OptTensor& lx, const OptTensor& ly,
+                                                               int64_t bandwidth, double scale)
+{
+    if (wants_grad({dout, q, k, v, out})) {
+        const variable_list g = AttentionBackward::apply(dout, q, k, v, out, out_lo, lse, lx, ly, bandwidth, scale);
+        return {g[0], g[1], g[2]};
+    }
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return attention_backward_op().call(dout, q, k, v, out, out_lo, lse, lx, ly, bandwidth, scale);
+}
+
+struct CrossAttention : torch::autograd::Function<CrossAttention> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& lx,
+                          const OptTensor& ly, int64_t bandwidth, double scale)
+    {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        auto [out, out_lo, lse] = attention_op().call(q, k, v, lx, ly, bandwidth, scale);
+        ctx->save_for_backward({q, k, v, out, out_lo, lse, tensor_of(lx), tensor_of(ly)});
+        ctx->saved_data["bandwidth"] = bandwidth;
+        ctx->saved_data["scale"] = scale;
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads)
+    {
+        const variable_list s = ctx->get_saved_variables();
+        auto [dq, dk, dv] = attention_backward_op().call(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], optional_of(s[6]),
+                                                         optional_of(s[7]), ctx->saved_data["bandwidth"].toInt(),
+                                                         ctx->saved_data["scale"].toDouble());
+        return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+Tensor cross_attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& lx, const OptTensor& ly,
+                                int64_t bandwidth, double scale)
+{
+    if (wants_grad({q, k, v})) return CrossAttention::apply(q, k, v, lx, ly, bandwidth, scale);
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return cross_attention_op().call(q, k, v, lx, ly, bandwidth, scale);
+}
+
+struct NormRotateBackward : torch::autograd::Function<NormRotateBackward> {
+    static variable_list forward(AutogradContext*, const Tensor& dy, const Tensor& x, const OptTensor& weight,
+                                 const OptTensor& lengths, const OptTensor& positions, int64_t rotary, double base,
+                                 bool interleaved, double eps, bool need_weight)
+    {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        auto [dx, dw] = norm_rotate_backward_op().call(dy, x, weight, lengths, positions, rotary, base, interleaved, eps,
+                                                       need_weight);
+        return {dx, dw};
+    }
+    static variable_list backward(AutogradContext*, const variable_list&) { return twice("norm_rotate"); }
+};
+
+std::tuple<Tensor, Tensor> norm_rotate_backward_autograd(const Tensor& dy, const Tensor& x, const OptTensor& weight,
+                                                         const OptTensor& lengths, const OptTensor& positions,
+                                                         int64_t rotary, double base, bool interleaved, double eps,
+                                                         bool need_weight)
+{
+    if (wants_grad({dy, x, tensor_of(weight)})) {
+        const variable_list g = NormRotateBackward::apply(dy, x, weight, lengths, positions, rotary, base, interleaved, eps,
+                                                          need_weight);
+        return {g[0], g[1]};
+    }
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return norm_rotate_backward_op().call(dy, x, weight, lengths, positions, rotary, base, interleaved, eps, need_weight);
+}
+
+struct NormRotate : torch::autograd::Function<NormRotate> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight, const OptTensor& lengths,
+                          const OptTensor& positions, int64_t rotary, double base, bool interleaved, double eps)
+    {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        const Tensor y = norm_rotate_op().call(x, weight, lengths, positions, rotary, base, interleaved, eps);
+        ctx->save_for_backward({x, tensor_of(weight), tensor_of(lengths), tensor_of(positions)});
+        ctx->saved_data["rotary"] = rotary;
+        ctx->saved_data["base"] = base;
+        ctx->saved_data["interleaved"] = interleaved;
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["need_weight"] = weight.has_value() && weight->requires_grad();
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads)
+    {
+        const variable_list s = ctx->get_saved_variables();
+        const bool need_weight = ctx->saved_data["need_weight"].toBool();
+        auto [dx, dw] = norm_rotate_backward_op().call(
+            grads[0], s[0], optional_of(s[1]), optional_of(s[2]), optional_of(s[3]), ctx->saved_data["rotary"].toInt(),
+            ctx->saved_data["base"].toDouble(), ctx->saved_data["interleaved"].toBool(), ctx->saved_data["eps"].toDouble(),
+            need_weight);
+        return {dx, need_weight ? dw : Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+Tensor norm_rotate_autograd(const Tensor& x, const OptTensor& weight, const OptTensor& lengths, const OptTensor& positions,
+                            int64_t rotary, double base, bool interleaved, double eps)
+{
+    if (wants_grad({x, tensor_of(weight)}))
+        return NormRotate::apply(x, weight, lengths, positions, rotary, base, interleaved, eps);
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return norm_rotate_op().call(x, weight, lengths, positions, rotary, base, interleaved, eps);
+}
+
+// CPU tensors: argument errors read like those of CUDA ones; then the device is refused.
+Tensor cross_attention_cpu(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& lengths_x,
+                           const OptTensor& lengths_y, int64_t bandwidth, double scale)
 {
     (void)bandwidth;
-    (void)need_grad;
     attention_checks(q, k, v, lengths_x, lengths_y, scale);
+    return {};
+}
+
+std::tuple<Tensor, Tensor, Tensor> attention_cpu(const Tensor& q, const Tensor& k, const Tensor& v,
+                                                 const OptTensor& lengths_x, const OptTensor& lengths_y,
+                                                 int64_t bandwidth, double scale)
+{
+    cross_attention_cpu(q, k, v, lengths_x, lengths_y, bandwidth, scale);
     return {};
 }
 
@@ -466,8 +679,10 @@ Tensor norm_rotate_cpu(const Tensor& x, const OptTensor& weight, const OptTensor
 
 TORCH_LIBRARY_FRAGMENT(torchsoftdtw_b200, m)
 {
-    m.def("attention(Tensor q, Tensor k, Tensor v, Tensor? lengths_x, Tensor? lengths_y, int bandwidth, float scale, "
-          "bool need_grad) -> (Tensor, Tensor, Tensor)");
+    m.def("cross_attention(Tensor q, Tensor k, Tensor v, Tensor? lengths_x, Tensor? lengths_y, int bandwidth, float scale) "
+          "-> Tensor");
+    m.def("attention(Tensor q, Tensor k, Tensor v, Tensor? lengths_x, Tensor? lengths_y, int bandwidth, float scale) "
+          "-> (Tensor, Tensor, Tensor)");
     m.def("attention_backward(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor out_lo, Tensor lse, "
           "Tensor? lengths_x, Tensor? lengths_y, int bandwidth, float scale) -> (Tensor, Tensor, Tensor)");
     m.def("norm_rotate(Tensor x, Tensor? weight, Tensor? lengths, Tensor? positions, int rotary_dim, float base, "
@@ -480,6 +695,7 @@ TORCH_LIBRARY_FRAGMENT(torchsoftdtw_b200, m)
 
 TORCH_LIBRARY_IMPL(torchsoftdtw_b200, CUDA, m)
 {
+    m.impl("cross_attention", &cross_attention_cuda);
     m.impl("attention", &attention_cuda);
     m.impl("attention_backward", &attention_backward_cuda);
     m.impl("norm_rotate", &norm_rotate_cuda);
@@ -490,8 +706,20 @@ TORCH_LIBRARY_IMPL(torchsoftdtw_b200, CUDA, m)
 
 TORCH_LIBRARY_IMPL(torchsoftdtw_b200, CPU, m)
 {
+    m.impl("cross_attention", &cross_attention_cpu);
     m.impl("attention", &attention_cpu);
     m.impl("norm_rotate", &norm_rotate_cpu);
     m.impl("global_norm", &global_norm_cuda);
     m.impl("clip_grads", &clip_grads_cuda);
+}
+
+TORCH_LIBRARY_IMPL(torchsoftdtw_b200, Autograd, m)
+{
+    m.impl("cross_attention", &cross_attention_autograd);
+    m.impl("attention_backward", &attention_backward_autograd);
+    m.impl("norm_rotate", &norm_rotate_autograd);
+    m.impl("norm_rotate_backward", &norm_rotate_backward_autograd);
+    // Norms and clipped gradients are results, not steps of a graph.
+    m.impl("global_norm", torch::CppFunction::makeFallthrough());
+    m.impl("clip_grads", torch::CppFunction::makeFallthrough());
 }
