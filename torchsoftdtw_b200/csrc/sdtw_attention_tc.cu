@@ -4,7 +4,7 @@
 // warps specialise and meet only at mbarriers:
 //   * four softmax warps a tile: one row a thread. S (128 x 128 fp32) is read from tensor memory, masked where
 //     the tile leaves the row's interval, and P = 2^(s scale / ln 2 - m) goes back over it as 16-bit operand;
-//   * one MMA thread: S = Q K^T (both from shared memory), O += P V (P from tensor memory, V read with its rows as
+//   * one MMA warp: S = Q K^T (both from shared memory), O += P V (P from tensor memory, V read with its rows as
 //     K), issued so that one tile's products run while the other tile's softmax does;
 //   * one TMA warp: Q once, then K and V tiles through a ring.
 // The running maximum m is only raised, and O rescaled, when a row's scores outgrow it by 2^8: P stays below 2^8
@@ -209,7 +209,8 @@ __global__ void __launch_bounds__(Geom<DPAD, NT>::THREADS, NT == 1 ? 2 : 1)
         }
     } else if (warp == G::SOFTMAX_WARPS) {
         // ---------------- MMA ----------------
-        if (lane == 0 && ja < jb) {
+        if (ja < jb) {
+            const uint32_t leader = elect_leader();
             const uint32_t idesc_s = mma_idesc<T>(kTile, false);
             const uint32_t idesc_o = mma_idesc<T>(f.dn, true);
             const int ksteps = f.dn / 16;
@@ -218,19 +219,21 @@ __global__ void __launch_bounds__(Geom<DPAD, NT>::THREADS, NT == 1 ? 2 : 1)
             const auto ring = [&](int n) { return mbar_wait(full + 8 * (n % G::SLOTS), (n / G::SLOTS) & 1, bound); };
             const auto slot_at = [&](int n) { return base + G::OFF_RING + (n % G::SLOTS) * G::TILE_BYTES; };
             const auto scores = [&](int w, int n) {
-                for (int k = 0; k < ksteps; ++k) {
+                const uint64_t qd = desc_k(base + w * G::TILE_BYTES), kd = desc_k(slot_at(n));
+#pragma unroll
+                for (int k = 0; k < DPAD / 16; ++k) {
                     const uint32_t at = (k / 4) * G::BLOCK + (k % 4) * 32;
-                    mma_ss(tmem + G::S_COL + w * kTile, desc_k(base + w * G::TILE_BYTES + at), desc_k(slot_at(n) + at),
-                           idesc_s, k > 0);
+                    if (k < ksteps)
+                        mma_ss(tmem + G::S_COL + w * kTile, desc_at(qd, at), desc_at(kd, at), idesc_s, k > 0, leader);
                 }
-                mma_commit(s_full + 8 * w);
+                mma_commit(s_full + 8 * w, leader);
             };
             if (ok && (ok = ring(0))) {
                 fence_after();
 #pragma unroll
                 for (int w = 0; w < NT; ++w)
                     if (ja >= first[w] && ja < last[w]) scores(w, 0);
-                mma_commit(empty);
+                mma_commit(empty, leader);
             }
             for (int j = ja; ok && j < jb; ++j) {
                 const int nv = 2 * (j - ja) + 1, nk = nv + 1;
@@ -243,11 +246,13 @@ __global__ void __launch_bounds__(Geom<DPAD, NT>::THREADS, NT == 1 ? 2 : 1)
                         if (ok) ok = mbar_wait(p_full + 8 * w, used[w] & 1, bound);
                         if (!ok) break;
                         fence_after();
+                        const uint64_t vd = desc_mn(slot_at(nv), G::BLOCK);
+#pragma unroll
                         for (int k = 0; k < kTile / 16; ++k)
-                            mma_ts(tmem + G::O_COL + w * DPAD, tmem + G::S_COL + w * kTile + 8 * k,
-                                   desc_mn(slot_at(nv) + 2048 * k, G::BLOCK), idesc_o, k > 0 || used[w] > 0);
+                            mma_ts(tmem + G::O_COL + w * DPAD, tmem + G::S_COL + w * kTile + 8 * k, desc_at(vd, 2048 * k),
+                                   idesc_o, k > 0 || used[w] > 0, leader);
                         ++used[w];
-                        if (j + 1 >= last[w]) mma_commit(o_full + 8 * w);
+                        if (j + 1 >= last[w]) mma_commit(o_full + 8 * w, leader);
                     }
                     if (j + 1 >= first[w] && j + 1 < last[w]) {
                         if (!have_k) have_k = ok = ring(nk);
@@ -259,14 +264,14 @@ __global__ void __launch_bounds__(Geom<DPAD, NT>::THREADS, NT == 1 ? 2 : 1)
                 if (!ok) break;
                 // The commits also cover slots that no tile read (they only bridge two tiles' ranges).
                 if (!have_v && !(ok = ring(nv))) break;
-                mma_commit(empty + 8 * (nv % G::SLOTS));
+                mma_commit(empty + 8 * (nv % G::SLOTS), leader);
                 if (j + 1 < jb) {
                     if (!have_k && !(ok = ring(nk))) break;
-                    mma_commit(empty + 8 * (nk % G::SLOTS));
+                    mma_commit(empty + 8 * (nk % G::SLOTS), leader);
                 }
             }
             // All products have completed before the tensor memory is given back.
-            mma_commit(fix);
+            mma_commit(fix, leader);
             mbar_drain(fix, (ny < a.M && jb > ja && ny - static_cast<int64_t>(jb - 1) * kTile < kTile) ? 1 : 0, f.timeout_ns);
         }
         __syncwarp();

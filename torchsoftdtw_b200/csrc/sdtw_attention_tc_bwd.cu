@@ -4,7 +4,7 @@
 //   dq = scale dS K;   dv = P^T dO,  dk = scale dS^T Q  (S^T = K Q^T and dP^T = V dO^T directly, states as rows)
 // Seven products where one launch with atomic sums of dq would take five: the price of sums in one fixed order.
 // P and dS go back over S and dP in tensor memory as the 16-bit A operand of the next product, so nothing of size
-// queries x states leaves the SM. One thread issues all products, in an order in which the products that wait for the
+// queries x states leaves the SM. One warp issues all products, in an order in which the products that wait for the
 // elementwise warps alternate with those that do not: in dk/dv  dV(i), S(i+1) | dK(i), dP(i+1), while the elementwise
 // warps form dS(i) | P(i+1).
 //
@@ -180,13 +180,17 @@ __global__ void __launch_bounds__(DqGeom<T, DPAD>::THREADS, DPAD == 64 ? 2 : 1)
         }
     } else if (warp == G::WARPS) {
         // ---------------- MMA ----------------
-        if (lane == 0 && ja < jb) {
+        if (ja < jb) {
+            const uint32_t leader = elect_leader();
             const uint32_t idesc_s = mma_idesc<T>(G::KT, false), idesc_q = mma_idesc<T>(f.dn, true);
             const int n = jb - ja, ksteps = f.dn / 16;
             const auto product = [&](uint32_t d, int rows_at, int cols_at) {
-                for (int k = 0; k < ksteps; ++k)
-                    mma_ss(tmem + d, desc_k(base + rows_at + (k / 4) * G::ROW_BLOCK + (k % 4) * 32),
-                           desc_k(base + cols_at + (k / 4) * G::COL_BLOCK + (k % 4) * 32), idesc_s, k > 0);
+                const uint64_t rd = desc_k(base + rows_at), cd = desc_k(base + cols_at);
+#pragma unroll
+                for (int k = 0; k < DPAD / 16; ++k)
+                    if (k < ksteps)
+                        mma_ss(tmem + d, desc_at(rd, (k / 4) * G::ROW_BLOCK + (k % 4) * 32),
+                               desc_at(cd, (k / 4) * G::COL_BLOCK + (k % 4) * 32), idesc_s, k > 0, leader);
             };
             const auto k_at = [&](int i) { return G::OFF_RING + 2 * (i % G::STAGES) * G::COL_BYTES; };
             const auto scores = [&](int i) {
@@ -194,7 +198,7 @@ __global__ void __launch_bounds__(DqGeom<T, DPAD>::THREADS, DPAD == 64 ? 2 : 1)
                 if (i > 0 && !mbar_wait(s_free, (i - 1) & 1, bound)) return false;
                 fence_after();
                 product(G::S_COL, 0, k_at(i));
-                mma_commit(s_full);
+                mma_commit(s_full, leader);
                 return true;
             };
             const auto dprobs = [&](int i) {
@@ -202,8 +206,8 @@ __global__ void __launch_bounds__(DqGeom<T, DPAD>::THREADS, DPAD == 64 ? 2 : 1)
                 if (i > 0 && !mbar_wait(dp_free, (i - 1) & 1, bound)) return false;
                 fence_after();
                 product(G::DP_COL, G::OFF_DO, k_at(i) + G::COL_BYTES);
-                mma_commit(dp_full);
-                mma_commit(v_empty + 8 * (i % G::STAGES));
+                mma_commit(dp_full, leader);
+                mma_commit(v_empty + 8 * (i % G::STAGES), leader);
                 return true;
             };
             bool ok = mbar_wait(row_full, 0, bound) && scores(0) && dprobs(0);
@@ -212,13 +216,14 @@ __global__ void __launch_bounds__(DqGeom<T, DPAD>::THREADS, DPAD == 64 ? 2 : 1)
                 ok = ok && mbar_wait(ds_full, i & 1, bound);
                 if (!ok) break;
                 fence_after();
+                const uint64_t kd = desc_mn(base + k_at(i), G::COL_BLOCK);
+#pragma unroll
                 for (int k = 0; k < G::KT / 16; ++k)
-                    mma_ts(tmem + G::ACC_COL, tmem + G::DS_COL + 8 * k, desc_mn(base + k_at(i) + 2048 * k, G::COL_BLOCK),
-                           idesc_q, i > 0 || k > 0);
-                mma_commit(ds_free);
-                mma_commit(k_empty + 8 * (i % G::STAGES));
+                    mma_ts(tmem + G::ACC_COL, tmem + G::DS_COL + 8 * k, desc_at(kd, 2048 * k), idesc_q, i > 0 || k > 0, leader);
+                mma_commit(ds_free, leader);
+                mma_commit(k_empty + 8 * (i % G::STAGES), leader);
             }
-            mma_commit(acc_full);
+            mma_commit(acc_full, leader);
             mbar_drain(acc_full, 0, f.timeout_ns);  // before the tensor memory is given back
         }
         __syncwarp();
@@ -507,33 +512,38 @@ __global__ void __launch_bounds__(DkvGeom<T, DPAD>::THREADS, DPAD == 64 ? 2 : 1)
         }
     } else if (warp == G::WARPS) {
         // ---------------- MMA ----------------
-        if (lane == 0 && n > 0) {
+        if (n > 0) {
+            const uint32_t leader = elect_leader();
             const uint32_t idesc_s = mma_idesc<T>(G::QT, false), idesc_o = mma_idesc<T>(f.dn, true);
             const int ksteps = f.dn / 16;
             const auto product = [&](uint32_t d, int rows_at, int cols_at) {
-                for (int k = 0; k < ksteps; ++k)
-                    mma_ss(tmem + d, desc_k(base + rows_at + (k / 4) * G::ROW_BLOCK + (k % 4) * 32),
-                           desc_k(base + cols_at + (k / 4) * G::COL_BLOCK + (k % 4) * 32), idesc_s, k > 0);
+                const uint64_t rd = desc_k(base + rows_at), cd = desc_k(base + cols_at);
+#pragma unroll
+                for (int k = 0; k < DPAD / 16; ++k)
+                    if (k < ksteps)
+                        mma_ss(tmem + d, desc_at(rd, (k / 4) * G::ROW_BLOCK + (k % 4) * 32),
+                               desc_at(cd, (k / 4) * G::COL_BLOCK + (k % 4) * 32), idesc_s, k > 0, leader);
             };
             // 64 columns of P or dS lie packed in the first 32 columns of their warpgroup's 64.
             const auto gradient = [&](uint32_t d, uint32_t src, int cols_at, bool more) {
+                const uint64_t cd = desc_mn(base + cols_at, G::COL_BLOCK);
+#pragma unroll
                 for (int k = 0; k < G::QT / 16; ++k)
-                    mma_ts(tmem + d, tmem + src + (k / 4) * 64 + (k % 4) * 8, desc_mn(base + cols_at + 2048 * k, G::COL_BLOCK),
-                           idesc_o, more || k > 0);
+                    mma_ts(tmem + d, tmem + src + (k / 4) * 64 + (k % 4) * 8, desc_at(cd, 2048 * k), idesc_o, more || k > 0, leader);
             };
             const auto q_at = [&](int i) { return G::OFF_RING + 2 * (i % G::STAGES) * G::COL_BYTES; };
             const auto scores = [&](int i) {
                 if (!mbar_wait(q_full + 8 * (i % G::STAGES), (i / G::STAGES) & 1, bound)) return false;
                 fence_after();
                 product(G::S_COL, 0, q_at(i));
-                mma_commit(s_full);
+                mma_commit(s_full, leader);
                 return true;
             };
             const auto dprobs = [&](int i) {
                 if (!mbar_wait(g_full + 8 * (i % G::STAGES), (i / G::STAGES) & 1, bound)) return false;
                 fence_after();
                 product(G::DP_COL, G::OFF_V, q_at(i) + G::COL_BYTES);
-                mma_commit(dp_full);
+                mma_commit(dp_full, leader);
                 return true;
             };
             bool ok = mbar_wait(row_full, 0, bound) && scores(0) && dprobs(0);
@@ -542,16 +552,16 @@ __global__ void __launch_bounds__(DkvGeom<T, DPAD>::THREADS, DPAD == 64 ? 2 : 1)
                 if (!ok) break;
                 fence_after();
                 gradient(G::DV_COL, G::S_COL, q_at(i) + G::COL_BYTES, i > 0);
-                mma_commit(g_empty + 8 * (i % G::STAGES));
+                mma_commit(g_empty + 8 * (i % G::STAGES), leader);
                 if (i + 1 < n && !(ok = scores(i + 1))) break;
                 ok = mbar_wait(ds_full, i & 1, bound);
                 if (!ok) break;
                 fence_after();
                 gradient(G::DK_COL, G::DP_COL, q_at(i), i > 0);
-                mma_commit(q_empty + 8 * (i % G::STAGES));
+                mma_commit(q_empty + 8 * (i % G::STAGES), leader);
                 if (i + 1 < n) ok = dprobs(i + 1);
             }
-            mma_commit(acc_full);
+            mma_commit(acc_full, leader);
             mbar_drain(acc_full, 0, f.timeout_ns);  // before the tensor memory is given back
         }
         __syncwarp();

@@ -39,14 +39,17 @@ struct Bound {
     uint32_t* err;
 };
 
-// Waits for the phase with the given parity. False when it ran out of time, or another role of the CTA did.
+// Waits for the phase with the given parity. False when it ran out of time, or another role of the CTA did. The
+// clock is first read after 256 tries (each of which the hardware suspends for a while): waits of a healthy CTA never pay for it.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const Bound& w)
 {
-    if (mbar_try_wait(bar, parity)) return true;
+#pragma unroll 1
+    for (int i = 0; i < 256; ++i)
+        if (mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = global_ns();
     while (true) {
 #pragma unroll 1
-        for (int i = 0; i < 16; ++i)
+        for (int i = 0; i < 64; ++i)
             if (mbar_try_wait(bar, parity)) return true;
         if (*w.abort) return false;
         if (global_ns() - t0 > w.timeout_ns) {
@@ -59,6 +62,9 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const B
 // The same wait for one's own operations in flight, which goes on after an abort.
 __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity, uint64_t timeout_ns)
 {
+#pragma unroll 1
+    for (int i = 0; i < 256; ++i)
+        if (mbar_try_wait(bar, parity)) return;
     const uint64_t t0 = global_ns();
     while (!mbar_try_wait(bar, parity) && global_ns() - t0 <= timeout_ns) {
     }
@@ -80,10 +86,23 @@ __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::aft
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Arrives on the barrier when every product issued by this thread so far has completed.
-__device__ __forceinline__ void mma_commit(uint32_t bar)
+// The warp that issues products runs them as one: its control flow and descriptors stay uniform, and only the
+// instructions themselves are for its leader. (Inside a branch of one lane each product cost about 110 cycles of
+// operand moves, against the 64 that the tensor core takes for it.)
+__device__ __forceinline__ uint32_t elect_leader()
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    uint32_t is;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.b32 %0, 1, 0, p; }" : "=r"(is));
+    return is;
+}
+// Arrives on the barrier when every product issued by the leader so far has completed.
+__device__ __forceinline__ void mma_commit(uint32_t bar, uint32_t leader)
+{
+    asm volatile(
+        "{ .reg .pred q; setp.ne.b32 q, %1, 0; "
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0]; }" ::"r"(bar),
+        "r"(leader)
+        : "memory");
 }
 
 // Instruction descriptor: fp32 accumulators, 16-bit operands (both bf16 or both fp16), A 128 rows, B n columns; b_mn:
@@ -104,6 +123,8 @@ __device__ __forceinline__ uint64_t desc_k(uint32_t saddr)
     return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(1) << 16) |
            (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
 }
+// A descriptor `bytes` further on (a tile lies below 256 KB, so its address field takes the sum).
+__device__ __forceinline__ uint64_t desc_at(uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); }
 // MN-major: the tile's rows are K, its 64-column blocks the operand's columns.
 __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t block)
 {
@@ -112,21 +133,21 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t block)
 }
 
 // d += a b (accumulate) or d = a b: A and B in shared memory.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate)
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate, uint32_t leader)
 {
     asm volatile(
-        "{ .reg .pred p; setp.ne.b32 p, %4, 0; "
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
+        "{ .reg .pred p, q; setp.ne.b32 p, %4, 0; setp.ne.b32 q, %5, 0; "
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)), "r"(leader)
         : "memory");
 }
 // The same with A in tensor memory: lane = row, each 32-bit column two neighbouring K.
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate)
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate, uint32_t leader)
 {
     asm volatile(
-        "{ .reg .pred p; setp.ne.b32 p, %4, 0; "
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
+        "{ .reg .pred p, q; setp.ne.b32 p, %4, 0; setp.ne.b32 q, %5, 0; "
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)), "r"(leader)
         : "memory");
 }
 
