@@ -1,15 +1,16 @@
 // Cross attention of 16-bit operands on the tensor cores (tcgen05): forward.
 //
-// A CTA takes NT tiles of 128 query rows of one head and walks the 128-state tiles that their cells touch. Its
+// A CTA takes NT tiles of 128 query rows of one head and walks the 64-state tiles that their cells touch. Its
 // warps specialise and meet only at mbarriers:
-//   * four softmax warps a tile: one row a thread. S (128 x 128 fp32) is read from tensor memory, masked where
-//     the tile leaves the row's interval, and P = 2^(s scale / ln 2 - m) goes back over it as 16-bit operand;
-//   * one MMA warp: S = Q K^T (both from shared memory), O += P V (P from tensor memory, V read with its rows as
-//     K), issued so that one tile's products run while the other tile's softmax does;
+//   * eight softmax warps a row tile: two threads a row, 32 states each. S (128 x 64 fp32) is read from tensor memory,
+//     masked where the tile leaves the row's interval, and P = 2^(s scale / ln 2 - m) goes back over it as 16-bit operand;
+//   * one MMA warp a row tile: S = Q K^T (both from shared memory), O += P V (P from tensor memory, V read with its rows
+//     as K). A row tile has two S buffers, so that the scores of the next state tile are there when a softmax ends;
 //   * one TMA warp: Q once, then K and V tiles through a ring.
 // The running maximum m is only raised, and O rescaled, when a row's scores outgrow it by 2^8: P stays below 2^8
-// until then, and the final division by the row's sum makes it exact. With two tiles (NT = 2) every K and V tile
-// is read once for 256 rows and the two tiles' products and softmaxes alternate on their units.
+// until then, and the final division by the row's sum makes it exact. So a tile's weights are formed at once with the m of
+// the tile before, beside its maximum, and formed again in the rare case that the maximum has outgrown it; the two threads
+// of a row only have to agree on that, which one barrier with an OR does.
 #include <mutex>
 #include <type_traits>
 
@@ -23,27 +24,31 @@ using namespace tc;
 
 namespace {
 
-constexpr int kTile = 128;  // query rows and states a tile
+constexpr int kTile = 128;    // query rows a tile
+constexpr int kStates = 64;   // states a tile
 constexpr float kGrow = 8.f;  // log2 of what a row's scores may outgrow its m by
 
 template <int DPAD, int NT>
 struct Geom {
-    static constexpr int TILE_BYTES = kTile * DPAD * 2;
-    static constexpr int BLOCK = kTile * 128;  // 64 features of a tile
+    static constexpr int Q_BYTES = kTile * DPAD * 2, KV_BYTES = kStates * DPAD * 2;
+    static constexpr int Q_BLOCK = kTile * 128, KV_BLOCK = kStates * 128;  // 64 features of a tile
     static constexpr int NBLOCK = DPAD / 64;
-    static constexpr int SLOTS = NT == 2 ? (DPAD == 128 ? 5 : 8) : 4;
-    static constexpr int OFF_RING = NT * TILE_BYTES;
-    static constexpr int OFF_BAR = OFF_RING + SLOTS * TILE_BYTES;
-    // barriers: q_full, fix, ring full[SLOTS], ring empty[SLOTS], s_full[NT], p_full[NT], o_full[NT]
-    static constexpr int NBAR = 2 + 2 * SLOTS + 3 * NT;
+    static constexpr int SLOTS = DPAD == 128 ? 9 : 8;
+    static constexpr int OFF_RING = NT * Q_BYTES;
+    static constexpr int OFF_ROW = OFF_RING + SLOTS * KV_BYTES;  // a number of each softmax thread's, for its partner
+    static constexpr int OFF_BAR = OFF_ROW + NT * 256 * 4;
+    // barriers: q_full, fix, ring full[SLOTS], ring empty[SLOTS], s_full[NT][2], p_full[NT][2], pv_full[NT],
+    // o_full[NT], idle[NT]
+    static constexpr int NBAR = 2 + 2 * SLOTS + 7 * NT;
     static constexpr int OFF_MISC = OFF_BAR + 8 * NBAR;  // tmem address, abort, tile ranges
     static constexpr int BYTES = OFF_MISC + 64 + 1024;   // and slack to align the base
-    static constexpr uint32_t S_COL = 0;                 // S (and P over it): 128 columns a tile
-    static constexpr uint32_t O_COL = NT * kTile;        // O: DPAD columns a tile
-    static constexpr uint32_t COLS_NEEDED = NT * (kTile + DPAD);
+    static constexpr uint32_t S_COL = 0;                 // S (and P over it): two buffers of 64 columns a row tile
+    static constexpr uint32_t O_COL = NT * 2 * kStates;  // O: DPAD columns a row tile
+    static constexpr uint32_t COLS_NEEDED = NT * (2 * kStates + DPAD);
     static constexpr uint32_t TMEM_COLS = COLS_NEEDED <= 256 ? 256 : 512;
-    static constexpr int SOFTMAX_WARPS = 4 * NT;
-    static constexpr int THREADS = 32 * (SOFTMAX_WARPS + 2);
+    static constexpr int SOFTMAX_WARPS = 8 * NT;
+    static constexpr int TMA_WARP = SOFTMAX_WARPS + NT;
+    static constexpr int THREADS = 32 * (TMA_WARP + 1);
     static_assert(BYTES <= 227 * 1024, "shared memory");
 };
 
@@ -54,37 +59,6 @@ struct FwdArgs {
     int dn;        // d rounded up to 16: columns of O
     int negative;  // scale < 0: the scores change sign
 };
-
-// 16-bit results of one row, from `v` times `f`: features c .. c + 31 that lie below d. The residual row (may be
-// null) takes what the rounding dropped.
-template <typename T>
-__device__ __forceinline__ void store_row32(T* row, T* lo, const float (&v)[32], int c, int d)
-{
-    if (d % 8 == 0) {  // rows start on 16 bytes
-#pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-            if (c + i >= d) break;
-            uint32_t w[4], r[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float x = v[i + 2 * e], y = v[i + 2 * e + 1];
-                w[e] = pack2(x, y, T());
-                const T* h = reinterpret_cast<const T*>(&w[e]);
-                r[e] = pack2(x - to_f(h[0]), y - to_f(h[1]), T());
-            }
-            *reinterpret_cast<uint4*>(row + c + i) = make_uint4(w[0], w[1], w[2], w[3]);
-            if (lo) *reinterpret_cast<uint4*>(lo + c + i) = make_uint4(r[0], r[1], r[2], r[3]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (c + i < d) {
-                const T h = from_f<T>(v[i]);
-                row[c + i] = h;
-                if (lo) lo[c + i] = from_f<T>(v[i] - to_f(h));
-            }
-    }
-}
 
 template <typename T, int DPAD, int NT>
 __global__ void __launch_bounds__(Geom<DPAD, NT>::THREADS, NT == 1 ? 2 : 1)
@@ -98,7 +72,7 @@ __global__ void __launch_bounds__(Geom<DPAD, NT>::THREADS, NT == 1 ? 2 : 1)
     const uint32_t base = smem_addr(sm);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t q_full = base + G::OFF_BAR, fix = q_full + 8, full = fix + 8, empty = full + 8 * G::SLOTS;
-    const uint32_t s_full = empty + 8 * G::SLOTS, p_full = s_full + 8 * NT, o_full = p_full + 8 * NT;
+    const uint32_t s_full = empty + 8 * G::SLOTS, p_full = s_full + 16 * NT, pv_full = p_full + 16 * NT, o_full = pv_full + 8 * NT, idle = o_full + 8 * NT;
     uint32_t* misc = reinterpret_cast<uint32_t*>(sm + G::OFF_MISC);
     volatile int* ranges = reinterpret_cast<volatile int*>(misc + 2);  // first and last + 1 state tile of each tile
     const Bound bound{f.timeout_ns, reinterpret_cast<volatile int*>(misc + 1), a.err};
@@ -116,12 +90,16 @@ __global__ void __launch_bounds__(Geom<DPAD, NT>::THREADS, NT == 1 ? 2 : 1)
         mbar_init(fix, 1);
         for (int s = 0; s < G::SLOTS; ++s) {
             mbar_init(full + 8 * s, 1);
-            mbar_init(empty + 8 * s, 1);
+            mbar_init(empty + 8 * s, NT);  // every MMA warp passes every tile
         }
         for (int w = 0; w < NT; ++w) {
-            mbar_init(s_full + 8 * w, 1);
-            mbar_init(p_full + 8 * w, 4);
+            for (int x = 0; x < 2; ++x) {
+                mbar_init(s_full + 16 * w + 8 * x, 1);
+                mbar_init(p_full + 16 * w + 8 * x, 8);
+            }
+            mbar_init(pv_full + 8 * w, 1);
             mbar_init(o_full + 8 * w, 1);
+            mbar_init(idle + 8 * w, 1);
             const int64_t r0 = row0 + w * kTile;
             int first = 0, last = 0;
             if (r0 < nx && ny > 0) {
@@ -129,8 +107,8 @@ __global__ void __launch_bounds__(Geom<DPAD, NT>::THREADS, NT == 1 ? 2 : 1)
                 int64_t lo, hi, lo1, hi1;
                 row_cells(a, r0, nx, ny, lo, hi);
                 row_cells(a, r1 - 1, nx, ny, lo1, hi1);
-                first = static_cast<int>(lo / kTile);
-                last = static_cast<int>((hi1 + kTile - 1) / kTile);
+                first = static_cast<int>(lo / kStates);
+                last = static_cast<int>((hi1 + kStates - 1) / kStates);
             }
             ranges[2 * w] = first;
             ranges[2 * w + 1] = last;
@@ -155,132 +133,150 @@ __global__ void __launch_bounds__(Geom<DPAD, NT>::THREADS, NT == 1 ? 2 : 1)
         }
     }
 
-    if (warp == G::SOFTMAX_WARPS + 1) {
+    const int count = jb > ja ? jb - ja : 0;  // state tiles
+    if (warp == G::TMA_WARP) {
         // ---------------- TMA ----------------
-        int issued = 0;
-        bool ok = true;
-        if (ja < jb) {
+        if (count > 0) {
             if (lane == 0) {
                 uint32_t bytes = 0;
                 for (int w = 0; w < NT; ++w)
-                    if (last[w] > first[w]) bytes += G::TILE_BYTES;
+                    if (last[w] > first[w]) bytes += G::Q_BYTES;
                 mbar_expect_tx(q_full, bytes);
                 for (int w = 0; w < NT; ++w)
                     if (last[w] > first[w])
                         for (int x = 0; x < G::NBLOCK; ++x)
-                            tma_load_4d(base + w * G::TILE_BYTES + x * G::BLOCK, &mq, q_full, 64 * x, row0 + w * kTile, h, b);
+                            tma_load_4d(base + w * G::Q_BYTES + x * G::Q_BLOCK, &mq, q_full, 64 * x, row0 + w * kTile, h, b);
             }
-            for (int n = 0; n < 2 * (jb - ja) && ok; ++n) {  // K and V of each state tile
-                const int j = ja + n / 2, slot = n % G::SLOTS;
-                const bool is_v = n & 1;
-                if (n >= G::SLOTS && !mbar_wait(empty + 8 * slot, (n / G::SLOTS - 1) & 1, bound)) {
-                    ok = false;
-                    break;
-                }
-                const uint32_t dst = base + G::OFF_RING + slot * G::TILE_BYTES;
+            int issued = 0;
+            const auto load = [&](int j, bool is_v) {
+                const int n = issued, slot = n % G::SLOTS;
+                if (n >= G::SLOTS && !mbar_wait(empty + 8 * slot, (n / G::SLOTS - 1) & 1, bound)) return false;
+                const int at = G::OFF_RING + slot * G::KV_BYTES;
                 // V rows past the length meet weights of zero, but may hold NaN: the tile that the length ends in
-                // is cleared behind it before it is handed on.
-                const int64_t left = ny - static_cast<int64_t>(j) * kTile;
-                const bool clear = is_v && left < kTile && ny < a.M;
+                // is cleared behind it before it is handed on (once a CTA: the last one).
+                const int64_t left = ny - static_cast<int64_t>(j) * kStates;
+                const bool clear = is_v && left < kStates && ny < a.M;
                 const uint32_t bar = clear ? fix : full + 8 * slot;
                 if (lane == 0) {
-                    mbar_expect_tx(bar, G::TILE_BYTES);
+                    mbar_expect_tx(bar, G::KV_BYTES);
                     for (int x = 0; x < G::NBLOCK; ++x)
-                        tma_load_4d(dst + x * G::BLOCK, is_v ? &mv : &mk, bar, 64 * x, j * kTile, hk, b);
+                        tma_load_4d(base + at + x * G::KV_BLOCK, is_v ? &mv : &mk, bar, 64 * x, j * kStates, hk, b);
                 }
                 __syncwarp();
-                if (clear) {  // once a CTA: only the last state tile can end inside
-                    if (!mbar_wait(fix, 0, bound)) ok = false;
-                    const int skip = static_cast<int>(left) * 8;  // 16-byte units a 64-feature block
-                    unsigned char* at = sm + G::OFF_RING + slot * G::TILE_BYTES;
+                bool ok = true;
+                if (clear) {
+                    ok = mbar_wait(fix, 0, bound);
                     for (int x = 0; x < G::NBLOCK; ++x)
-                        for (int u = skip + lane; u < kTile * 8; u += 32)
-                            *reinterpret_cast<uint4*>(at + x * G::BLOCK + 16 * u) = make_uint4(0, 0, 0, 0);
+                        for (int u = static_cast<int>(left) * 8 + lane; u < kStates * 8; u += 32)
+                            *reinterpret_cast<uint4*>(sm + at + x * G::KV_BLOCK + 16 * u) = make_uint4(0, 0, 0, 0);
                     fence_async_shared();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(full + 8 * slot);
                 }
                 issued = n + 1;
-            }
+                return ok;
+            };
+            // In the order of use: K 0, K 1, then V t and K t + 2.
+            bool ok = load(ja, false) && (count < 2 || load(ja + 1, false));
+            for (int t = 0; t < count && ok; ++t) ok = load(ja + t, true) && (t + 2 >= count || load(ja + t + 2, false));
             // Every load has landed before the CTA ends (also after an abort).
             mbar_drain(q_full, 0, f.timeout_ns);
             for (int n = issued < G::SLOTS ? 0 : issued - G::SLOTS; n < issued; ++n)
                 mbar_drain(full + 8 * (n % G::SLOTS), (n / G::SLOTS) & 1, f.timeout_ns);
         }
-    } else if (warp == G::SOFTMAX_WARPS) {
-        // ---------------- MMA ----------------
-        if (ja < jb) {
+    } else if (warp >= G::SOFTMAX_WARPS) {
+        // ---------------- MMA, one warp a row tile ----------------
+        const int w = warp - G::SOFTMAX_WARPS;
+        if (count > 0) {
             const uint32_t leader = elect_leader();
-            const uint32_t idesc_s = mma_idesc<T>(kTile, false);
+            const uint32_t idesc_s = mma_idesc<T>(kStates, false);
             const uint32_t idesc_o = mma_idesc<T>(f.dn, true);
-            const int ksteps = f.dn / 16;
-            uint32_t used[NT] = {};  // P tiles consumed
+            const int ja_w = NT == 1 || w == 0 ? first[0] : first[NT - 1];
+            const int jb_w = NT == 1 || w == 0 ? last[0] : last[NT - 1];
+            const uint64_t qd = desc_k(base + w * G::Q_BYTES);
+            const uint32_t s_col = tmem + G::S_COL + 2 * w * kStates, o_col = tmem + G::O_COL + w * DPAD;
+            int slot = 0;
+            uint32_t phase = 0;
             bool ok = mbar_wait(q_full, 0, bound);
-            const auto ring = [&](int n) { return mbar_wait(full + 8 * (n % G::SLOTS), (n / G::SLOTS) & 1, bound); };
-            const auto slot_at = [&](int n) { return base + G::OFF_RING + (n % G::SLOTS) * G::TILE_BYTES; };
-            const auto scores = [&](int w, int n) {
-                const uint64_t qd = desc_k(base + w * G::TILE_BYTES), kd = desc_k(slot_at(n));
-#pragma unroll
-                for (int k = 0; k < DPAD / 16; ++k) {
-                    const uint32_t at = (k / 4) * G::BLOCK + (k % 4) * 32;
-                    if (k < ksteps)
-                        mma_ss(tmem + G::S_COL + w * kTile, desc_at(qd, at), desc_at(kd, at), idesc_s, k > 0, leader);
+            const auto arrived = [&] { return mbar_wait(full + 8 * slot, phase, bound); };
+            const auto release = [&] {  // behind the products that read the slot
+                mma_commit(empty + 8 * slot, leader);
+                if (++slot == G::SLOTS) {
+                    slot = 0;
+                    phase ^= 1;
                 }
-                mma_commit(s_full + 8 * w, leader);
             };
-            if (ok && (ok = ring(0))) {
+            // The scores of state tile j into the buffer of its turn. Products complete in no promised order among
+            // themselves, so the PV product that read the weights there has to be awaited.
+            const auto scores = [&](int j) {
+                const int it = j - ja_w, x = it & 1;
+                if (it >= 2) ok = mbar_wait(pv_full + 8 * w, it & 1, bound) && ok;
+                ok = ok && arrived();
+                if (!ok) return;
                 fence_after();
+                const uint64_t kd = desc_k(base + G::OFF_RING + slot * G::KV_BYTES);
 #pragma unroll
-                for (int w = 0; w < NT; ++w)
-                    if (ja >= first[w] && ja < last[w]) scores(w, 0);
-                mma_commit(empty, leader);
+                for (int k = 0; k < DPAD / 16; ++k)  // features past d are zero; a branch between products costs more
+                    mma_ss(s_col + x * kStates, desc_at(qd, (k / 4) * G::Q_BLOCK + (k % 4) * 32),
+                           desc_at(kd, (k / 4) * G::KV_BLOCK + (k % 4) * 32), idesc_s, k > 0, leader);
+                mma_commit(s_full + 16 * w + 8 * x, leader);
+            };
+            // In the order of the loads: K 0, K 1, then V t and K t + 2. A tile outside this row tile's range (it only
+            // bridges the CTA's two) is passed on when it has landed.
+            for (int t = 0; ok && t < 2 && t < count; ++t) {
+                if (ja + t >= ja_w && ja + t < jb_w)
+                    scores(ja + t);
+                else
+                    ok = arrived();
+                release();
             }
-            for (int j = ja; ok && j < jb; ++j) {
-                const int nv = 2 * (j - ja) + 1, nk = nv + 1;
-                bool have_v = false, have_k = false;
+            for (int t = 0; ok && t < count; ++t) {
+                const int j = ja + t;
+                ok = arrived();
+                if (ok && j >= ja_w && j < jb_w) {
+                    const int it = j - ja_w, x = it & 1;
+                    if (!(ok = mbar_wait(p_full + 16 * w + 8 * x, (it >> 1) & 1, bound))) break;
+                    fence_after();
+                    const uint64_t vd = desc_mn(base + G::OFF_RING + slot * G::KV_BYTES, G::KV_BLOCK);
 #pragma unroll
-                for (int w = 0; w < NT; ++w) {
-                    if (!ok) break;
-                    if (j >= first[w] && j < last[w]) {
-                        if (!have_v) have_v = ok = ring(nv);
-                        if (ok) ok = mbar_wait(p_full + 8 * w, used[w] & 1, bound);
-                        if (!ok) break;
-                        fence_after();
-                        const uint64_t vd = desc_mn(slot_at(nv), G::BLOCK);
-#pragma unroll
-                        for (int k = 0; k < kTile / 16; ++k)
-                            mma_ts(tmem + G::O_COL + w * DPAD, tmem + G::S_COL + w * kTile + 8 * k, desc_at(vd, 2048 * k),
-                                   idesc_o, k > 0 || used[w] > 0, leader);
-                        ++used[w];
-                        if (j + 1 >= last[w]) mma_commit(o_full + 8 * w, leader);
-                    }
-                    if (j + 1 >= first[w] && j + 1 < last[w]) {
-                        if (!have_k) have_k = ok = ring(nk);
-                        if (!ok) break;
-                        fence_after();
-                        scores(w, nk);
-                    }
+                    for (int k = 0; k < kStates / 16; ++k)
+                        mma_ts(o_col, s_col + x * kStates + 8 * k, desc_at(vd, 2048 * k), idesc_o, k > 0 || it > 0, leader);
+                    mma_commit(pv_full + 8 * w, leader);
+                    if (j + 1 == jb_w) mma_commit(o_full + 8 * w, leader);
                 }
-                if (!ok) break;
-                // The commits also cover slots that no tile read (they only bridge two tiles' ranges).
-                if (!have_v && !(ok = ring(nv))) break;
-                mma_commit(empty + 8 * (nv % G::SLOTS), leader);
-                if (j + 1 < jb) {
-                    if (!have_k && !(ok = ring(nk))) break;
-                    mma_commit(empty + 8 * (nk % G::SLOTS), leader);
+                release();
+                if (ok && t + 2 < count) {
+                    if (j + 2 >= ja_w && j + 2 < jb_w)
+                        scores(j + 2);
+                    else
+                        ok = arrived();
+                    release();
                 }
             }
             // All products have completed before the tensor memory is given back.
-            mma_commit(fix, leader);
-            mbar_drain(fix, (ny < a.M && jb > ja && ny - static_cast<int64_t>(jb - 1) * kTile < kTile) ? 1 : 0, f.timeout_ns);
+            mma_commit(idle + 8 * w, leader);
+            mbar_drain(idle + 8 * w, 0, f.timeout_ns);
         }
         __syncwarp();
     } else {
-        // ---------------- softmax: one row a thread ----------------
-        const int w = NT == 1 ? 0 : warp >> 2;
-        const int64_t i = row0 + w * kTile + (tid & 127);
+        // ---------------- softmax: two threads a row, 32 states of a tile each ----------------
+        const int w = NT == 1 ? 0 : warp >> 3, half = (warp >> 2) & 1;
+        const int row = 32 * (warp & 3) + lane, pair = 1 + 4 * w + (warp & 3);  // the pair's named barrier
+        const int64_t i = row0 + w * kTile + row;
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-        const uint32_t ts = tmem + lanes + G::S_COL + w * kTile, to = tmem + lanes + G::O_COL + w * DPAD;
+        const uint32_t ts0 = tmem + lanes + G::S_COL + 2 * w * kStates, to = tmem + lanes + G::O_COL + w * DPAD;
+        float* mine = reinterpret_cast<float*>(sm + G::OFF_ROW) + w * 256 + half * 128 + row;
+        const float* theirs = reinterpret_cast<float*>(sm + G::OFF_ROW) + w * 256 + (1 - half) * 128 + row;
+        const auto meet = [&] { asm volatile("barrier.cta.sync %0, 64;" ::"r"(pair) : "memory"); };
+        const auto either = [&](bool x) {
+            uint32_t r;
+            asm volatile(
+                "{ .reg .pred p, q; setp.ne.b32 p, %1, 0; barrier.cta.red.or.pred q, %2, 64, p; selp.b32 %0, 1, 0, q; }"
+                : "=r"(r)
+                : "r"(static_cast<uint32_t>(x)), "r"(pair)
+                : "memory");
+            return r != 0;
+        };
         int64_t lo = 0, hi = 0;
         if (i < nx && ny > 0) row_cells(a, i, nx, ny, lo, hi);
         const int ilo = static_cast<int>(lo), width = static_cast<int>(hi - lo);
@@ -289,106 +285,141 @@ __global__ void __launch_bounds__(Geom<DPAD, NT>::THREADS, NT == 1 ? 2 : 1)
         const float sl = a.scale_log2;
         // fp16 weights are kept 2^6 larger, so that weights down to 2^-20 of a row's largest stay normal numbers.
         constexpr float kShift = std::is_same<T, __half>::value ? 6.f : 0.f;
-        float m = -INFINITY, sum = 0.f;
-        bool ok = true;
+        float m = -INFINITY, bias = 0.f, sum = 0.f;
+        bool ok = true;  // the same in both threads of a row from each meeting on
         for (int j = ja_w; j < jb_w; ++j) {
             const int it = j - ja_w;
-            if (!mbar_wait(s_full + 8 * w, it & 1, bound)) {
-                ok = false;
-                break;
-            }
+            const uint32_t ts = ts0 + (it & 1) * kStates;
+            ok = __all_sync(kFull, ok && mbar_wait(s_full + 16 * w + 8 * (it & 1), (it >> 1) & 1, bound));
             fence_after();
-            uint32_t s[kTile];
-#pragma unroll
-            for (int c = 0; c < kTile; c += 32) tmem_ld32(ts + c, s + c);
+            const int off = j * kStates + 32 * half - ilo;
+            const bool whole = __all_sync(kFull, off >= 0 && off + 32 <= width);
+            uint32_t s[32], p[16];
+            tmem_ld32(ts + 32 * half, s);
             wait_ld();
             settle(s);
             if (f.negative) {
 #pragma unroll
-                for (int c = 0; c < kTile; ++c) s[c] ^= 0x80000000u;
+                for (int c = 0; c < 32; ++c) s[c] ^= 0x80000000u;
             }
-            const int off = j * kTile - ilo;
-            if (!__all_sync(kFull, off >= 0 && off + kTile <= width)) {
+            if (!whole) {
 #pragma unroll
-                for (int c = 0; c < kTile; ++c)
+                for (int c = 0; c < 32; ++c)
                     if (static_cast<unsigned>(off + c) >= static_cast<unsigned>(width)) s[c] = 0xff800000u;
             }
-            float t0 = __uint_as_float(s[0]), t1 = __uint_as_float(s[1]);
-            float t2 = __uint_as_float(s[2]), t3 = __uint_as_float(s[3]);
+            float t0 = m, t1 = __uint_as_float(s[0]), t2 = __uint_as_float(s[1]), t3 = __uint_as_float(s[2]);
 #pragma unroll
-            for (int c = 4; c < kTile; c += 4) {
+            for (int c = 0; c < 32; c += 4) {
                 t0 = fmaxf(t0, __uint_as_float(s[c]));
                 t1 = fmaxf(t1, __uint_as_float(s[c + 1]));
                 t2 = fmaxf(t2, __uint_as_float(s[c + 2]));
                 t3 = fmaxf(t3, __uint_as_float(s[c + 3]));
             }
-            const float m2 = fmaxf(m, fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)));
-            if (it == 0) {
-                m = m2;
-            } else if (__any_sync(kFull, (m2 - m) * sl > kGrow)) {
-                // O holds the sum of the tiles before (their products completed before this tile's scores).
-                const float fix_up = m2 == -INFINITY ? 1.f : ex2f((m - m2) * sl);
-                m = m2;
-                sum *= fix_up;
-                for (int c = 0; c < f.dn; c += 16) {
-                    uint32_t o[16];
-                    tmem_ld16(to + c, o);
-                    wait_ld();
-                    settle(o);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fix_up);
-                    tmem_st16(to + c, o);
-                }
-            }
-            const float bias = m == -INFINITY ? 0.f : fmaf(-m, sl, kShift);
-            float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-            for (int c = 0; c < kTile; c += 32) {
-                uint32_t p[16];
+            float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
+            float tile = 0.f;
+            const auto weights = [&] {  // P and its sum with the present m
+                float l0 = 0.f, l1 = 0.f;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const float x = ex2f(fmaf(__uint_as_float(s[c + 2 * e]), sl, bias));
-                    const float y = ex2f(fmaf(__uint_as_float(s[c + 2 * e + 1]), sl, bias));
+                    const float x = ex2f(fmaf(__uint_as_float(s[2 * e]), sl, bias));
+                    const float y = ex2f(fmaf(__uint_as_float(s[2 * e + 1]), sl, bias));
                     l0 += x;
                     l1 += y;
                     p[e] = pack2(x, y, T());
                 }
-                tmem_st16(ts + c / 2, p);
+                tile = l0 + l1;
+            };
+            if (it > 0) weights();
+            // Both warps have read their scores when they meet here: P may overwrite them.
+            if (either(it == 0 || !ok || (top - m) * sl > kGrow)) {
+                *mine = ok ? top : __int_as_float(0x7fc00000);
+                meet();
+                const float other = *theirs;
+                meet();
+                if (!ok || __any_sync(kFull, other != other)) {  // this warp gave up, or its partner did (a maximum is no NaN)
+                    ok = false;
+                    break;
+                }
+                top = fmaxf(top, other);
+                if (it > 0) {
+                    // O holds the sum of the tiles before, once their products have completed. Its features go by 16 to
+                    // the two threads of the row.
+                    ok = __all_sync(kFull, mbar_wait(pv_full + 8 * w, (it - 1) & 1, bound));
+                    fence_after();
+                    const float fix_up = top == -INFINITY ? 1.f : ex2f((m - top) * sl);
+                    sum *= fix_up;
+                    for (int c = 16 * half; c < f.dn; c += 32) {
+                        uint32_t o[16];
+                        tmem_ld16(to + c, o);
+                        wait_ld();
+                        settle(o);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fix_up);
+                        tmem_st16(to + c, o);
+                    }
+                }
+                m = top;
+                bias = m == -INFINITY ? 0.f : fmaf(-m, sl, kShift);
+                weights();
             }
-            sum += l0 + l1;
+            tmem_st16(ts + 16 * half, p);
+            sum += tile;
             wait_st();
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_full + 8 * w);
+            if (lane == 0) mbar_arrive(p_full + 16 * w + 8 * (it & 1));
         }
+        // (Not pv_full: PV products of this tile and the one before may both have completed by now, or neither, and a
+        // parity tells a phase only from its neighbours.)
         if (ok && jb_w > ja_w) ok = mbar_wait(o_full + 8 * w, 0, bound);
         fence_after();
-        ok = __all_sync(kFull, ok);
-        // Rows without a cell are zero; a bad sample's, and all after a wait that ran out, NaN.
+        *mine = sum;
+        ok = !either(!ok);
+        sum += *theirs;
+        // Rows without a cell are zero; a bad sample's, and all after a wait that ran out, NaN. A pair of warps lays its 32
+        // rows down in shared memory (Q's place; all scores are done) in 16-byte units, turned by the row against bank
+        // conflicts, and stores them row by row.
         const float scale = width > 0 ? 1.f / sum : 0.f;
+        const bool any = jb_w > ja_w && ok;
         const bool broken = !ok || !good;
-        T* out = static_cast<T*>(a.out) + ((static_cast<int64_t>(b) * a.N + i) * a.Hq + h) * a.d;
-        T* out_lo = a.out_lo ? static_cast<T*>(a.out_lo) + ((static_cast<int64_t>(b) * a.N + i) * a.Hq + h) * a.d : nullptr;
-        for (int c = 0; c < a.d; c += 32) {
-            float v[32];
-            if (jb_w > ja_w && ok) {
-                uint32_t o[32];
-                tmem_ld32(to + c, o);
-                wait_ld();
-                settle(o);
+        constexpr int UPR = DPAD / 8;  // units a row
+        uint4* rows = reinterpret_cast<uint4*>(sm + w * G::Q_BYTES) + (warp & 3) * 32 * UPR;
+        const int64_t i0 = row0 + w * kTile + 32 * (warp & 3);
+        for (int part = 0; part < (a.out_lo ? 2 : 1); ++part) {
+            for (int c = 16 * half; c < f.dn; c += 32) {
+                uint32_t o[16];
+                if (any) {
+                    tmem_ld16(to + c, o);
+                    wait_ld();
+                    settle(o);
+                }
 #pragma unroll
-                for (int e = 0; e < 32; ++e) v[e] = width > 0 ? __uint_as_float(o[e]) * scale : 0.f;
-            } else {
+                for (int e = 0; e < 16; e += 8) {
+                    uint32_t v[4];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) v[e] = 0.f;
+                    for (int x = 0; x < 4; ++x) {
+                        float v0 = any && width > 0 ? __uint_as_float(o[e + 2 * x]) * scale : 0.f;
+                        float v1 = any && width > 0 ? __uint_as_float(o[e + 2 * x + 1]) * scale : 0.f;
+                        if (broken) v0 = v1 = __int_as_float(0x7fc00000);
+                        v[x] = pack2(v0, v1, T());
+                        if (part == 1) {
+                            const T* r = reinterpret_cast<const T*>(&v[x]);
+                            v[x] = pack2(v0 - to_f(r[0]), v1 - to_f(r[1]), T());
+                        }
+                    }
+                    rows[lane * UPR + (((c + e) / 8) ^ (lane & 7))] = make_uint4(v[0], v[1], v[2], v[3]);
+                }
             }
-            if (broken) {
-#pragma unroll
-                for (int e = 0; e < 32; ++e) v[e] = __int_as_float(0x7fc00000);
-            }
-            if (i < a.N) store_row32<T>(out, out_lo, v, c, a.d);
+            meet();
+            T* out = static_cast<T*>(part ? a.out_lo : a.out) + ((static_cast<int64_t>(b) * a.N + i0) * a.Hq + h) * a.d;
+            const int64_t pitch = static_cast<int64_t>(a.Hq) * a.d;
+#pragma unroll 4
+            for (int r = half * (32 / UPR) + lane / UPR; r < 32; r += 2 * (32 / UPR))
+                if (i0 + r < a.N && lane % UPR * 8 < a.d)
+                    *reinterpret_cast<uint4*>(out + r * pitch + lane % UPR * 8) = rows[r * UPR + ((lane % UPR) ^ (r & 7))];
+            meet();
         }
-        if (i < a.N && a.lse)
+        if (half == 0 && i < a.N && a.lse)
             a.lse[(static_cast<int64_t>(b) * a.Hq + h) * a.N + i] = width > 0 ? fmaf(m, sl, log2f(sum) - kShift) : -INFINITY;
         fence_before();
     }
@@ -449,8 +480,8 @@ cudaError_t forward_t(const AttnArgs& a, cudaStream_t s)
     CUtensorMap mq, mk, mv;
     constexpr bool half = std::is_same<T, __half>::value;
     if (!attention_tile_map(&mq, half, a.q, a.qs, a.B, a.N, a.Hq, a.d, kTile) ||
-        !attention_tile_map(&mk, half, a.k, a.ks, a.B, a.M, a.Hkv, a.d, kTile) ||
-        !attention_tile_map(&mv, half, a.v, a.vs, a.B, a.M, a.Hkv, a.d, kTile))
+        !attention_tile_map(&mk, half, a.k, a.ks, a.B, a.M, a.Hkv, a.d, kStates) ||
+        !attention_tile_map(&mv, half, a.v, a.vs, a.B, a.M, a.Hkv, a.d, kStates))
         return cudaErrorInvalidValue;
     FwdArgs f{};
     f.a = a;

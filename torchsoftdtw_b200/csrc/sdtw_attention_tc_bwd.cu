@@ -183,14 +183,13 @@ __global__ void __launch_bounds__(DqGeom<T, DPAD>::THREADS, DPAD == 64 ? 2 : 1)
         if (ja < jb) {
             const uint32_t leader = elect_leader();
             const uint32_t idesc_s = mma_idesc<T>(G::KT, false), idesc_q = mma_idesc<T>(f.dn, true);
-            const int n = jb - ja, ksteps = f.dn / 16;
+            const int n = jb - ja;
             const auto product = [&](uint32_t d, int rows_at, int cols_at) {
                 const uint64_t rd = desc_k(base + rows_at), cd = desc_k(base + cols_at);
 #pragma unroll
-                for (int k = 0; k < DPAD / 16; ++k)
-                    if (k < ksteps)
-                        mma_ss(tmem + d, desc_at(rd, (k / 4) * G::ROW_BLOCK + (k % 4) * 32),
-                               desc_at(cd, (k / 4) * G::COL_BLOCK + (k % 4) * 32), idesc_s, k > 0, leader);
+                for (int k = 0; k < DPAD / 16; ++k)  // features past d are zero; a branch between products costs more
+                    mma_ss(tmem + d, desc_at(rd, (k / 4) * G::ROW_BLOCK + (k % 4) * 32),
+                           desc_at(cd, (k / 4) * G::COL_BLOCK + (k % 4) * 32), idesc_s, k > 0, leader);
             };
             const auto k_at = [&](int i) { return G::OFF_RING + 2 * (i % G::STAGES) * G::COL_BYTES; };
             const auto scores = [&](int i) {
@@ -515,14 +514,12 @@ __global__ void __launch_bounds__(DkvGeom<T, DPAD>::THREADS, DPAD == 64 ? 2 : 1)
         if (n > 0) {
             const uint32_t leader = elect_leader();
             const uint32_t idesc_s = mma_idesc<T>(G::QT, false), idesc_o = mma_idesc<T>(f.dn, true);
-            const int ksteps = f.dn / 16;
             const auto product = [&](uint32_t d, int rows_at, int cols_at) {
                 const uint64_t rd = desc_k(base + rows_at), cd = desc_k(base + cols_at);
 #pragma unroll
-                for (int k = 0; k < DPAD / 16; ++k)
-                    if (k < ksteps)
-                        mma_ss(tmem + d, desc_at(rd, (k / 4) * G::ROW_BLOCK + (k % 4) * 32),
-                               desc_at(cd, (k / 4) * G::COL_BLOCK + (k % 4) * 32), idesc_s, k > 0, leader);
+                for (int k = 0; k < DPAD / 16; ++k)  // features past d are zero; a branch between products costs more
+                    mma_ss(tmem + d, desc_at(rd, (k / 4) * G::ROW_BLOCK + (k % 4) * 32),
+                           desc_at(cd, (k / 4) * G::COL_BLOCK + (k % 4) * 32), idesc_s, k > 0, leader);
             };
             // 64 columns of P or dS lie packed in the first 32 columns of their warpgroup's 64.
             const auto gradient = [&](uint32_t d, uint32_t src, int cols_at, bool more) {

@@ -200,6 +200,12 @@ __device__ __forceinline__ void settle(uint32_t (&r)[N])
     for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
 
+__device__ __forceinline__ void settle32(uint32_t* r)
+{
+#pragma unroll
+    for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
+}
+
 __device__ __forceinline__ uint32_t pack2(float lo, float hi, __half)
 {
     const __half2 h = __floats2half2_rn(lo, hi);
