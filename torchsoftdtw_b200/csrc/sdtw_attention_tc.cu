@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(Geom<DPAD, NT>::THREADS, NT == 1 ? 2 : 1)
         for (int j = ja_w; j < jb_w; ++j) {
             const int it = j - ja_w;
             const uint32_t ts = ts0 + (it & 1) * kStates;
-            ok = __all_sync(kFull, ok && mbar_wait(s_full + 16 * w + 8 * (it & 1), (it >> 1) & 1, bound));
+            ok = ok && mbar_wait(s_full + 16 * w + 8 * (it & 1), (it >> 1) & 1, bound);
             fence_after();
             const int off = j * kStates + 32 * half - ilo;
             const bool whole = __all_sync(kFull, off >= 0 && off + 32 <= width);
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(Geom<DPAD, NT>::THREADS, NT == 1 ? 2 : 1)
                 if (it > 0) {
                     // O holds the sum of the tiles before, once their products have completed. Its features go by 16 to
                     // the two threads of the row.
-                    ok = __all_sync(kFull, mbar_wait(pv_full + 8 * w, (it - 1) & 1, bound));
+                    ok = mbar_wait(pv_full + 8 * w, (it - 1) & 1, bound);
                     fence_after();
                     const float fix_up = top == -INFINITY ? 1.f : ex2f((m - top) * sl);
                     sum *= fix_up;

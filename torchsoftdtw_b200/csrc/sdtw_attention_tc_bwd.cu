@@ -3,10 +3,11 @@
 //   P = 2^(s scale / ln 2 - lse),  dS = P (dP - delta),  delta = do . (o + o_lo)
 //   dq = scale dS K;   dv = P^T dO,  dk = scale dS^T Q  (S^T = K Q^T and dP^T = V dO^T directly, states as rows)
 // Seven products where one launch with atomic sums of dq would take five: the price of sums in one fixed order.
-// P and dS go back over S and dP in tensor memory as the 16-bit A operand of the next product, so nothing of size
-// queries x states leaves the SM. One warp issues all products, in an order in which the products that wait for the
-// elementwise warps alternate with those that do not: in dk/dv  dV(i), S(i+1) | dK(i), dP(i+1), while the elementwise
-// warps form dS(i) | P(i+1).
+// P and dS go to tensor memory as the 16-bit A operand of the next product, so nothing of size queries x states leaves
+// the SM. A CTA keeps 128 rows (of Q and dO, or of K and V) and streams 64 columns (of the other two) at a time; eight
+// elementwise warps take two threads a row, 32 columns each. Products complete in no promised order among themselves, so
+// whatever one of them reads is only overwritten when it has been awaited: where tensor memory has room (d > 64), P and dS have
+// places of their own beside S and dP, and scores run a tile ahead; where two CTAs share it (d <= 64) they lie over S and dP.
 //
 // fp16: P is kept 2^10 larger and dS scaled by a power of two that brings the rows' |do| to [8, 16) (a row's own in
 // dq, where a row is a lane; the largest of the head in dk), so that neither under- nor overflows where the gradients do not.
@@ -45,46 +46,183 @@ __device__ __forceinline__ float gradient_scale(float norm2)
     return exp2f(3.f - floorf(0.5f * log2f(norm2)));
 }
 
-template <typename T, int DPAD>
-struct DqGeom {
-    static constexpr int KT = DPAD == 128 ? 128 : 64;  // states a tile
-    static constexpr int WGS = KT / 64;                // elementwise warpgroups, 64 columns each
-    static constexpr int ROW_BYTES = kTile * DPAD * 2; // Q, dO
-    static constexpr int COL_BYTES = KT * DPAD * 2;    // K, V
-    static constexpr int ROW_BLOCK = kTile * 128, COL_BLOCK = KT * 128;
+constexpr int kCols = 64;  // columns of a product: states in dq, queries in dk/dv
+constexpr int kElemWarps = 8;
+constexpr int kMmaWarp = kElemWarps, kTmaWarp = kElemWarps + 1;
+constexpr int kThreads = 32 * (kElemWarps + 2);
+
+// Shared memory: the two row operands, a ring of pairs of column tiles, statistics, barriers.
+template <int DPAD>
+struct Geom {
+    static constexpr int ROW_BYTES = kTile * DPAD * 2, COL_BYTES = kCols * DPAD * 2;
+    static constexpr int ROW_BLOCK = kTile * 128, COL_BLOCK = kCols * 128;  // 64 features of a tile
     static constexpr int NBLOCK = DPAD / 64;
-    static constexpr int STAGES = 2;
-    static constexpr int OFF_DO = ROW_BYTES;
-    static constexpr int OFF_RING = 2 * ROW_BYTES;  // STAGES of (K, V)
-    static constexpr int OFF_STAT = OFF_RING + STAGES * 2 * COL_BYTES;  // delta, |do|^2 of the rows
-    static constexpr int OFF_BAR = OFF_STAT + 2 * kTile * 4;
-    // row_full, fix, k_full[S], k_empty[S], v_full[S], v_empty[S], s_full, s_free, dp_full, dp_free, ds_full, ds_free, acc
-    static constexpr int NBAR = 2 + 4 * STAGES + 7;
+    static constexpr int STAGES = DPAD == 128 ? 4 : 3;
+    static constexpr int OFF_RING = 2 * ROW_BYTES;
+    static constexpr int OFF_STAT = OFF_RING + STAGES * 2 * COL_BYTES;
+    static constexpr int STAT_BYTES = 4 * (STAGES * 2 * kCols > 2 * kTile ? STAGES * 2 * kCols : 2 * kTile);
+    static constexpr int OFF_BAR = OFF_STAT + STAT_BYTES;
+    // row_full, fix, full[2][STAGES], empty[2][STAGES], and eight more
+    static constexpr int NBAR = 2 + 4 * STAGES + 9;
     static constexpr int OFF_MISC = OFF_BAR + 8 * NBAR;
     static constexpr int BYTES = OFF_MISC + 32 + 1024;
-    static constexpr uint32_t S_COL = 0, DP_COL = KT, DS_COL = 2 * KT, ACC_COL = 2 * KT + KT / 2;
-    static constexpr uint32_t TMEM_COLS = ACC_COL + DPAD <= 256 ? 256 : 512;
-    static constexpr int WARPS = 4 * WGS;
-    static constexpr int THREADS = 32 * (WARPS + 2);
-    static_assert(BYTES <= 227 * 1024, "shared memory");
+    static constexpr int CTAS = DPAD == 64 ? 2 : 1;  // an SM
+    static_assert(CTAS * (BYTES + 1024) <= 228 * 1024, "shared memory");
 };
 
+// A place in the ring and the parity of its present turn.
+template <int STAGES>
+struct Turn {
+    int at = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next()
+    {
+        if (++at == STAGES) {
+            at = 0;
+            phase ^= 1;
+        }
+    }
+};
+
+// 32 rows of a warp pair's results, features 16 half, 16 half + 32, .. of each from tensor memory at `acc` (times `back`, zero
+// where not `keep`), through shared memory (`rows`: 32 DPAD 16-bit values) to global rows `pitch` apart.
 template <typename T, int DPAD>
-__global__ void __launch_bounds__(DqGeom<T, DPAD>::THREADS, DPAD == 64 ? 2 : 1)
+__device__ __forceinline__ void store_rows(uint32_t acc, uint4* rows, int lane, int half, int pair, bool any, bool keep, bool broken,
+                                           float back, int dn, int d, T* out, int64_t pitch, int64_t rows_left)
+{
+    constexpr int UPR = DPAD / 8;
+    for (int c = 16 * half; c < dn; c += 32) {
+        uint32_t o[16];
+        if (any) {
+            tmem_ld16(acc + c, o);
+            wait_ld();
+            settle(o);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e += 8) {
+            uint32_t v[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                float v0 = any && keep ? __uint_as_float(o[e + 2 * x]) * back : 0.f;
+                float v1 = any && keep ? __uint_as_float(o[e + 2 * x + 1]) * back : 0.f;
+                if (broken) v0 = v1 = __int_as_float(0x7fc00000);
+                v[x] = pack2(v0, v1, T());
+            }
+            rows[lane * UPR + (((c + e) / 8) ^ (lane & 7))] = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+    }
+    asm volatile("barrier.cta.sync %0, 64;" ::"r"(pair) : "memory");
+#pragma unroll 4
+    for (int r = half * (32 / UPR) + lane / UPR; r < 32; r += 2 * (32 / UPR))
+        if (r < rows_left && lane % UPR * 8 < d)
+            *reinterpret_cast<uint4*>(out + r * pitch + lane % UPR * 8) = rows[r * UPR + ((lane % UPR) ^ (r & 7))];
+}
+
+// The TMA warp's part: both row tiles, then pairs of column tiles in the order of use. Rows of a column tile past the length
+// meet weights of zero but may hold NaN: the tile that the length ends in is cleared behind it before it is handed on.
+// stats(stage, step) writes a tile's statistics before its first load.
+template <int DPAD, typename COORDS, typename STATS>
+__device__ __forceinline__ void load_tiles(unsigned char* sm, uint32_t base, const CUtensorMap* r1, const CUtensorMap* r2,
+                                           const CUtensorMap* c1, const CUtensorMap* c2, int row0, int row_head, int b, int steps,
+                                           int64_t length, int64_t extent, uint32_t row_full, uint32_t fix, uint32_t full,
+                                           uint32_t empty, const Bound& bound, int lane, COORDS coords, STATS stats)
+{
+    using G = Geom<DPAD>;
+    if (steps <= 0) return;
+    if (lane == 0) {
+        mbar_expect_tx(row_full, 2 * G::ROW_BYTES);
+        for (int x = 0; x < G::NBLOCK; ++x) {
+            tma_load_4d(base + x * G::ROW_BLOCK, r1, row_full, 64 * x, row0, row_head, b);
+            tma_load_4d(base + G::ROW_BYTES + x * G::ROW_BLOCK, r2, row_full, 64 * x, row0, row_head, b);
+        }
+    }
+    Turn<G::STAGES> turn;
+    int issued[2] = {0, 0}, fixes = 0;
+    bool ok = true;
+    for (int t = 0; t < steps && ok; ++t) {
+        int c0, head;
+        coords(t, c0, head);
+        const int64_t left = length - c0;
+        const bool clear = left < kCols && length < extent;
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            const uint32_t fullb = full + 8 * (which * G::STAGES + turn.at), emptyb = empty + 8 * (which * G::STAGES + turn.at);
+            ok = ok && (t < G::STAGES || mbar_wait(emptyb, turn.phase ^ 1, bound));
+            if (!ok) break;
+            if (which == 0) {
+                stats(turn.at, t);
+                __syncwarp();
+            }
+            const int at = G::OFF_RING + (2 * turn.at + which) * G::COL_BYTES;
+            const uint32_t bar = clear ? fix : fullb;
+            if (lane == 0) {
+                mbar_expect_tx(bar, G::COL_BYTES);
+                for (int x = 0; x < G::NBLOCK; ++x)
+                    tma_load_4d(base + at + x * G::COL_BLOCK, which ? c2 : c1, bar, 64 * x, c0, head, b);
+            }
+            __syncwarp();
+            if (clear) {
+                ok = mbar_wait(fix, fixes & 1, bound);
+                ++fixes;
+                for (int x = 0; x < G::NBLOCK; ++x)
+                    for (int u = static_cast<int>(left) * 8 + lane; u < kCols * 8; u += 32)
+                        *reinterpret_cast<uint4*>(sm + at + x * G::COL_BLOCK + 16 * u) = make_uint4(0, 0, 0, 0);
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(fullb);
+            }
+            ++issued[which];
+        }
+        turn.next();
+    }
+    // Every load has landed before the CTA ends (also after an abort).
+    mbar_drain(row_full, 0, bound.timeout_ns);
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+        for (int t = issued[which] < G::STAGES ? 0 : issued[which] - G::STAGES; t < issued[which]; ++t)
+            mbar_drain(full + 8 * (which * G::STAGES + t % G::STAGES), (t / G::STAGES) & 1, bound.timeout_ns);
+}
+
+// d = rows cols^T over all features (those past d are zero; a branch between products costs more than they do).
+template <int DPAD>
+__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t rows_at, uint32_t cols_at, uint32_t idesc, uint32_t leader)
+{
+    using G = Geom<DPAD>;
+    const uint64_t rd = desc_k(rows_at), cd = desc_k(cols_at);
+#pragma unroll
+    for (int k = 0; k < DPAD / 16; ++k)
+        mma_ss(d, desc_at(rd, (k / 4) * G::ROW_BLOCK + (k % 4) * 32), desc_at(cd, (k / 4) * G::COL_BLOCK + (k % 4) * 32), idesc,
+               k > 0, leader);
+}
+// d += A cols, A the 128 x 64 operand at `a` in tensor memory: 32 columns of it packed in 16, `half` apart.
+template <int DPAD>
+__device__ __forceinline__ void mma_cols(uint32_t d, uint32_t a, uint32_t half, uint32_t cols_at, uint32_t idesc, bool more,
+                                         uint32_t leader)
+{
+    using G = Geom<DPAD>;
+    const uint64_t cd = desc_mn(cols_at, G::COL_BLOCK);
+#pragma unroll
+    for (int k = 0; k < kCols / 16; ++k)
+        mma_ts(d, a + (k / 2) * half + (k % 2) * 8, desc_at(cd, 2048 * k), idesc, more || k > 0, leader);
+}
+
+template <typename T, int DPAD>
+__global__ void __launch_bounds__(kThreads, Geom<DPAD>::CTAS)
     attend_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mg,
                         const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                         const __grid_constant__ BwdArgs f)
 {
-    using G = DqGeom<T, DPAD>;
+    using G = Geom<DPAD>;
+    constexpr uint32_t S_COL = 0, DP_COL = kCols, DS_COL = 2 * kCols, ACC_COL = 2 * kCols + kCols / 2;
+    constexpr uint32_t TMEM_COLS = ACC_COL + DPAD <= 256 ? 256 : 512;
     const AttnArgs& a = f.a;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* sm = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     const uint32_t base = smem_addr(sm);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t row_full = base + G::OFF_BAR, fix = row_full + 8, k_full = fix + 8, k_empty = k_full + 8 * G::STAGES;
-    const uint32_t v_full = k_empty + 8 * G::STAGES, v_empty = v_full + 8 * G::STAGES, s_full = v_empty + 8 * G::STAGES;
-    const uint32_t s_free = s_full + 8, dp_full = s_free + 8, dp_free = dp_full + 8, ds_full = dp_free + 8;
-    const uint32_t ds_free = ds_full + 8, acc_full = ds_free + 8;
+    const uint32_t row_full = base + G::OFF_BAR, fix = row_full + 8, full = fix + 8, empty = full + 16 * G::STAGES;
+    const uint32_t s_full = empty + 16 * G::STAGES, s_free = s_full + 8, dp_full = s_free + 8, dp_free = dp_full + 8;
+    const uint32_t ds_full = dp_free + 8, ds_free = ds_full + 8, acc_full = ds_free + 8;
     uint32_t* misc = reinterpret_cast<uint32_t*>(sm + G::OFF_MISC);
     float* s_delta = reinterpret_cast<float*>(sm + G::OFF_STAT);
     float* s_norm = s_delta + kTile;
@@ -99,12 +237,12 @@ __global__ void __launch_bounds__(DqGeom<T, DPAD>::THREADS, DPAD == 64 ? 2 : 1)
     if (tid == 0) {
         mbar_init(row_full, 1);
         mbar_init(fix, 1);
-        for (int s = 0; s < 4 * G::STAGES; ++s) mbar_init(k_full + 8 * s, 1);
+        for (int s = 0; s < 4 * G::STAGES; ++s) mbar_init(full + 8 * s, 1);
         mbar_init(s_full, 1);
-        mbar_init(s_free, G::WARPS);
+        mbar_init(s_free, kElemWarps);
         mbar_init(dp_full, 1);
-        mbar_init(dp_free, G::WARPS);
-        mbar_init(ds_full, G::WARPS);
+        mbar_init(dp_free, kElemWarps);
+        mbar_init(ds_full, kElemWarps);
         mbar_init(ds_free, 1);
         mbar_init(acc_full, 1);
         int first = 0, last = 0;
@@ -112,8 +250,8 @@ __global__ void __launch_bounds__(DqGeom<T, DPAD>::THREADS, DPAD == 64 ? 2 : 1)
             int64_t lo, hi, lo1, hi1;
             row_cells(a, row0, nx, ny, lo, hi);
             row_cells(a, (row0 + kTile < nx ? row0 + kTile : nx) - 1, nx, ny, lo1, hi1);
-            first = static_cast<int>(lo / G::KT);
-            last = static_cast<int>((hi1 + G::KT - 1) / G::KT);
+            first = static_cast<int>(lo / kCols);
+            last = static_cast<int>((hi1 + kCols - 1) / kCols);
         }
         misc[2] = first;
         misc[3] = last;
@@ -121,117 +259,64 @@ __global__ void __launch_bounds__(DqGeom<T, DPAD>::THREADS, DPAD == 64 ? 2 : 1)
         if (!good) atomicOr(a.err, kErrBadLength);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == G::WARPS) tmem_alloc(base + G::OFF_MISC, G::TMEM_COLS);
+    if (warp == kMmaWarp) tmem_alloc(base + G::OFF_MISC, TMEM_COLS);
     fence_before();
     __syncthreads();
     fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(misc);
     const int ja = static_cast<int>(*reinterpret_cast<volatile uint32_t*>(misc + 2));
-    const int jb = static_cast<int>(*reinterpret_cast<volatile uint32_t*>(misc + 3));
+    const int n = static_cast<int>(*reinterpret_cast<volatile uint32_t*>(misc + 3)) - ja;
 
-    if (warp == G::WARPS + 1) {
-        // ---------------- TMA ----------------
-        int issued_k = 0, issued_v = 0, fixes = 0;
-        bool ok = true;
-        if (ja < jb) {
-            if (lane == 0) {
-                mbar_expect_tx(row_full, 2 * G::ROW_BYTES);
-                for (int x = 0; x < G::NBLOCK; ++x) {
-                    tma_load_4d(base + x * G::ROW_BLOCK, &mq, row_full, 64 * x, row0, h, b);
-                    tma_load_4d(base + G::OFF_DO + x * G::ROW_BLOCK, &mg, row_full, 64 * x, row0, h, b);
-                }
-            }
-            for (int j = ja; j < jb && ok; ++j) {
-                const int n = j - ja, st = n % G::STAGES;
-                const int64_t left = ny - static_cast<int64_t>(j) * G::KT;
-                const bool clear = left < G::KT && ny < a.M;  // rows past the length may hold NaN
-                for (int is_v = 0; is_v < 2 && ok; ++is_v) {
-                    const uint32_t fullb = (is_v ? v_full : k_full) + 8 * st, emptyb = (is_v ? v_empty : k_empty) + 8 * st;
-                    if (n >= G::STAGES && !mbar_wait(emptyb, (n / G::STAGES - 1) & 1, bound)) {
-                        ok = false;
-                        break;
-                    }
-                    const int at = G::OFF_RING + (2 * st + is_v) * G::COL_BYTES;
-                    const uint32_t bar = clear ? fix : fullb;
-                    if (lane == 0) {
-                        mbar_expect_tx(bar, G::COL_BYTES);
-                        for (int x = 0; x < G::NBLOCK; ++x)
-                            tma_load_4d(base + at + x * G::COL_BLOCK, is_v ? &mv : &mk, bar, 64 * x, j * G::KT, hk, b);
-                    }
-                    __syncwarp();
-                    if (clear) {
-                        if (!mbar_wait(fix, fixes & 1, bound)) ok = false;
-                        ++fixes;
-                        for (int x = 0; x < G::NBLOCK; ++x)
-                            for (int u = static_cast<int>(left) * 8 + lane; u < G::KT * 8; u += 32)
-                                *reinterpret_cast<uint4*>(sm + at + x * G::COL_BLOCK + 16 * u) = make_uint4(0, 0, 0, 0);
-                        fence_async_shared();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(fullb);
-                    }
-                    ++(is_v ? issued_v : issued_k);
-                }
-            }
-            mbar_drain(row_full, 0, f.timeout_ns);
-            for (int n = issued_k < G::STAGES ? 0 : issued_k - G::STAGES; n < issued_k; ++n)
-                mbar_drain(k_full + 8 * (n % G::STAGES), (n / G::STAGES) & 1, f.timeout_ns);
-            for (int n = issued_v < G::STAGES ? 0 : issued_v - G::STAGES; n < issued_v; ++n)
-                mbar_drain(v_full + 8 * (n % G::STAGES), (n / G::STAGES) & 1, f.timeout_ns);
-        }
-    } else if (warp == G::WARPS) {
-        // ---------------- MMA ----------------
-        if (ja < jb) {
+    if (warp == kTmaWarp) {
+        load_tiles<DPAD>(
+            sm, base, &mq, &mg, &mk, &mv, row0, h, b, n, ny, a.M, row_full, fix, full, empty, bound, lane,
+            [&](int t, int& c0, int& head) {
+                c0 = (ja + t) * kCols;
+                head = hk;
+            },
+            [](int, int) {});
+    } else if (warp == kMmaWarp) {
+        if (n > 0) {
             const uint32_t leader = elect_leader();
-            const uint32_t idesc_s = mma_idesc<T>(G::KT, false), idesc_q = mma_idesc<T>(f.dn, true);
-            const int n = jb - ja;
-            const auto product = [&](uint32_t d, int rows_at, int cols_at) {
-                const uint64_t rd = desc_k(base + rows_at), cd = desc_k(base + cols_at);
-#pragma unroll
-                for (int k = 0; k < DPAD / 16; ++k)  // features past d are zero; a branch between products costs more
-                    mma_ss(tmem + d, desc_at(rd, (k / 4) * G::ROW_BLOCK + (k % 4) * 32),
-                           desc_at(cd, (k / 4) * G::COL_BLOCK + (k % 4) * 32), idesc_s, k > 0, leader);
-            };
-            const auto k_at = [&](int i) { return G::OFF_RING + 2 * (i % G::STAGES) * G::COL_BYTES; };
-            const auto scores = [&](int i) {
-                if (!mbar_wait(k_full + 8 * (i % G::STAGES), (i / G::STAGES) & 1, bound)) return false;
+            const uint32_t idesc_s = mma_idesc<T>(kCols, false), idesc_q = mma_idesc<T>(f.dn, true);
+            Turn<G::STAGES> ahead, now;
+            const auto ring = [&](int at, int which) { return base + G::OFF_RING + (2 * at + which) * G::COL_BYTES; };
+            // S and dP of the next tile, each as soon as the elementwise warps have read the last one's.
+            const auto next_products = [&](int i) {
+                if (!mbar_wait(full + 8 * ahead.at, ahead.phase, bound)) return false;
                 if (i > 0 && !mbar_wait(s_free, (i - 1) & 1, bound)) return false;
                 fence_after();
-                product(G::S_COL, 0, k_at(i));
+                mma_rows<DPAD>(tmem + S_COL, base, ring(ahead.at, 0), idesc_s, leader);
                 mma_commit(s_full, leader);
-                return true;
-            };
-            const auto dprobs = [&](int i) {
-                if (!mbar_wait(v_full + 8 * (i % G::STAGES), (i / G::STAGES) & 1, bound)) return false;
+                if (!mbar_wait(full + 8 * (G::STAGES + ahead.at), ahead.phase, bound)) return false;
                 if (i > 0 && !mbar_wait(dp_free, (i - 1) & 1, bound)) return false;
                 fence_after();
-                product(G::DP_COL, G::OFF_DO, k_at(i) + G::COL_BYTES);
+                mma_rows<DPAD>(tmem + DP_COL, base + G::ROW_BYTES, ring(ahead.at, 1), idesc_s, leader);
                 mma_commit(dp_full, leader);
-                mma_commit(v_empty + 8 * (i % G::STAGES), leader);
+                mma_commit(empty + 8 * (G::STAGES + ahead.at), leader);
+                ahead.next();
                 return true;
             };
-            bool ok = mbar_wait(row_full, 0, bound) && scores(0) && dprobs(0);
+            bool ok = mbar_wait(row_full, 0, bound) && next_products(0);
             for (int i = 0; ok && i < n; ++i) {
-                if (i + 1 < n) ok = scores(i + 1) && dprobs(i + 1);
-                ok = ok && mbar_wait(ds_full, i & 1, bound);
-                if (!ok) break;
+                if (i + 1 < n && !(ok = next_products(i + 1))) break;
+                if (!(ok = mbar_wait(ds_full, i & 1, bound))) break;
                 fence_after();
-                const uint64_t kd = desc_mn(base + k_at(i), G::COL_BLOCK);
-#pragma unroll
-                for (int k = 0; k < G::KT / 16; ++k)
-                    mma_ts(tmem + G::ACC_COL, tmem + G::DS_COL + 8 * k, desc_at(kd, 2048 * k), idesc_q, i > 0 || k > 0, leader);
+                mma_cols<DPAD>(tmem + ACC_COL, tmem + DS_COL, 16, ring(now.at, 0), idesc_q, i > 0, leader);
                 mma_commit(ds_free, leader);
-                mma_commit(k_empty + 8 * (i % G::STAGES), leader);
+                mma_commit(empty + 8 * now.at, leader);
+                now.next();
             }
             mma_commit(acc_full, leader);
             mbar_drain(acc_full, 0, f.timeout_ns);  // before the tensor memory is given back
         }
         __syncwarp();
     } else {
-        // ---------------- elementwise: one row a thread, 64 columns a warpgroup ----------------
+        // ---------------- elementwise: two threads a row, 32 columns each ----------------
         // delta and |do|^2 of the tile's rows: LPR lanes a row.
         constexpr int LPR = DPAD / 8, RPW = 32 / LPR;
 #pragma unroll 4
-        for (int r0 = warp * RPW; r0 < kTile; r0 += G::WARPS * RPW) {
+        for (int r0 = warp * RPW; r0 < kTile; r0 += kElemWarps * RPW) {
             const int r = r0 + lane / LPR, c = lane % LPR * 8;
             const int64_t i = row0 + r;
             float dot = 0.f, nrm = 0.f;
@@ -261,152 +346,105 @@ __global__ void __launch_bounds__(DqGeom<T, DPAD>::THREADS, DPAD == 64 ? 2 : 1)
                 if (is_half<T> && i < nx) atomicMax(f.peak + b * a.Hkv + hk, __float_as_uint(nrm));
             }
         }
-        asm volatile("bar.sync 1, %0;" ::"n"(32 * G::WARPS) : "memory");
-        const int wg = warp >> 2, r = tid & 127;
+        const int half = warp >> 2, r = 32 * (warp & 3) + lane;
         const int64_t i = row0 + r;
-        const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-        const uint32_t ts = tmem + lanes + G::S_COL + 64 * wg, tdp = tmem + lanes + G::DP_COL + 64 * wg;
-        const uint32_t tds = tmem + lanes + G::DS_COL + 32 * wg;
         int64_t lo = 0, hi = 0;
         if (i < nx && ny > 0) row_cells(a, i, nx, ny, lo, hi);
         const int ilo = static_cast<int>(lo), width = static_cast<int>(hi - lo);
         const float lse = width > 0 ? a.lse[(static_cast<int64_t>(b) * a.Hq + h) * a.N + i] : INFINITY;
+        asm volatile("barrier.cta.sync 1, %0;" ::"n"(32 * kElemWarps) : "memory");
+        const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+        const uint32_t ts = tmem + lanes + S_COL + 32 * half, tdp = tmem + lanes + DP_COL + 32 * half;
+        const uint32_t tds = tmem + lanes + DS_COL + 16 * half;
         const float gscale = is_half<T> ? gradient_scale(s_norm[r]) : 1.f;
         const float cf = is_half<T> ? gscale * exp2f(-kPShift<T>) : 1.f;
         const float delta = s_delta[r] * cf, bias = kPShift<T> - lse;
         bool ok = true;
-        for (int j = ja; j < jb; ++j) {
-            const int it = j - ja;
+        for (int it = 0; it < n; ++it) {
             if (!(ok = mbar_wait(s_full, it & 1, bound))) break;
             fence_after();
-            uint32_t s[64], p[64];
+            uint32_t s[32], p[32];
             tmem_ld32(ts, s);
-            tmem_ld32(ts + 32, s + 32);
             wait_ld();
             settle(s);
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(s_free);
-            const int off = j * G::KT + 64 * wg - ilo;
-            const bool whole = __all_sync(kFull, off >= 0 && off + 64 <= width);
+            const int off = (ja + it) * kCols + 32 * half - ilo;
+            const bool whole = __all_sync(kFull, off >= 0 && off + 32 <= width);
 #pragma unroll
-            for (int c = 0; c < 64; ++c)
+            for (int c = 0; c < 32; ++c)
                 s[c] = __float_as_uint(ex2f(fmaf(__uint_as_float(s[c]), a.scale_log2, bias)));
             if (!whole) {
 #pragma unroll
-                for (int c = 0; c < 64; ++c)
+                for (int c = 0; c < 32; ++c)
                     if (static_cast<unsigned>(off + c) >= static_cast<unsigned>(width)) s[c] = 0;
             }
             if (!(ok = mbar_wait(dp_full, it & 1, bound))) break;
             fence_after();
             tmem_ld32(tdp, p);
-            tmem_ld32(tdp + 32, p + 32);
             wait_ld();
             settle(p);
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(dp_free);
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float p0 = __uint_as_float(p[2 * e]), p1 = __uint_as_float(p[2 * e + 1]);
+                const float d0 = is_half<T> ? fmaf(p0, cf, -delta) : p0 - delta;
+                const float d1 = is_half<T> ? fmaf(p1, cf, -delta) : p1 - delta;
+                w[e] = pack2(__uint_as_float(s[2 * e]) * d0, __uint_as_float(s[2 * e + 1]) * d1, T());
+            }
             if (it > 0 && !(ok = mbar_wait(ds_free, (it - 1) & 1, bound))) break;
             fence_after();
-#pragma unroll
-            for (int c = 0; c < 64; c += 32) {
-                uint32_t w[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int x = c + 2 * e;
-                    const float d0 = is_half<T> ? fmaf(__uint_as_float(p[x]), cf, -delta) : __uint_as_float(p[x]) - delta;
-                    const float d1 = is_half<T> ? fmaf(__uint_as_float(p[x + 1]), cf, -delta) : __uint_as_float(p[x + 1]) - delta;
-                    w[e] = pack2(__uint_as_float(s[x]) * d0, __uint_as_float(s[x + 1]) * d1, T());
-                }
-                tmem_st16(tds + c / 2, w);
-            }
+            tmem_st16(tds, w);
             wait_st();
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(ds_full);
         }
-        if (ok && jb > ja) ok = mbar_wait(acc_full, 0, bound);
+        if (ok && n > 0) ok = mbar_wait(acc_full, 0, bound);
         fence_after();
-        ok = __all_sync(kFull, ok);
-        const float back = a.scale / gscale;
-        T* out = static_cast<T*>(a.dq) + ((static_cast<int64_t>(b) * a.N + i) * a.Hq + h) * a.d;
-#pragma unroll
-        for (int c = (DPAD / G::WGS) * wg; c < (DPAD / G::WGS) * (wg + 1); c += 16) {
-            uint32_t o[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = 0;
-            if (c >= f.dn) break;
-            if (jb > ja && ok) {
-                tmem_ld16(tmem + lanes + G::ACC_COL + c, o);
-                wait_ld();
-                settle(o);
-            }
-            if (i >= a.N) continue;
-#pragma unroll
-            for (int e = 0; e < 16; e += 8) {
-                if (c + e >= a.d) break;
-                uint32_t w[4];
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    float v0 = width > 0 ? __uint_as_float(o[e + 2 * x]) * back : 0.f;
-                    float v1 = width > 0 ? __uint_as_float(o[e + 2 * x + 1]) * back : 0.f;
-                    if (!ok) v0 = v1 = __int_as_float(0x7fc00000);
-                    w[x] = pack2(v0, v1, T());
-                }
-                *reinterpret_cast<uint4*>(out + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-        }
+        // Q's place holds the rows on their way out: all scores are done.
+        const int64_t i0 = row0 + 32 * (warp & 3);
+        store_rows<T, DPAD>(tmem + lanes + ACC_COL, reinterpret_cast<uint4*>(sm) + (warp & 3) * 32 * (DPAD / 8), lane, half,
+                            2 + (warp & 3), n > 0 && ok, width > 0, !ok, a.scale / gscale, f.dn, a.d,
+                            static_cast<T*>(a.dq) + ((static_cast<int64_t>(b) * a.N + i0) * a.Hq + h) * a.d,
+                            static_cast<int64_t>(a.Hq) * a.d, a.N - i0);
         fence_before();
     }
     __syncthreads();
-    if (warp == G::WARPS) {
+    if (warp == kMmaWarp) {
         fence_after();
-        tmem_free(tmem, G::TMEM_COLS);
+        tmem_free(tmem, TMEM_COLS);
     }
 }
 
 template <typename T, int DPAD>
-struct DkvGeom {
-    static constexpr int QT = DPAD == 128 ? 128 : 64;  // queries a tile
-    static constexpr int WGS = QT / 64;
-    static constexpr int ROW_BYTES = kTile * DPAD * 2;  // K, V
-    static constexpr int COL_BYTES = QT * DPAD * 2;     // Q, dO
-    static constexpr int ROW_BLOCK = kTile * 128, COL_BLOCK = QT * 128;
-    static constexpr int NBLOCK = DPAD / 64;
-    static constexpr int STAGES = 2;
-    static constexpr int OFF_V = ROW_BYTES;
-    static constexpr int OFF_RING = 2 * ROW_BYTES;  // STAGES of (Q, dO)
-    static constexpr int OFF_STAT = OFF_RING + STAGES * 2 * COL_BYTES;  // STAGES of lse, delta of the tile's queries
-    static constexpr int OFF_BAR = OFF_STAT + STAGES * 2 * QT * 4;
-    // row_full, fix, q_full[S], q_empty[S], g_full[S], g_empty[S], s_full, p_full, dp_full, ds_full, acc
-    static constexpr int NBAR = 2 + 4 * STAGES + 5;
-    static constexpr int OFF_MISC = OFF_BAR + 8 * NBAR;
-    static constexpr int BYTES = OFF_MISC + 32 + 1024;
-    static constexpr uint32_t S_COL = 0, DP_COL = QT, DV_COL = 2 * QT, DK_COL = 2 * QT + DPAD;
-    static constexpr uint32_t TMEM_COLS = DK_COL + DPAD <= 256 ? 256 : 512;
-    static constexpr int WARPS = 4 * WGS;
-    static constexpr int THREADS = 32 * (WARPS + 2);
-    static_assert(BYTES <= 227 * 1024, "shared memory");
-    static_assert(DK_COL + DPAD <= 512, "tensor memory");
-};
-
-template <typename T, int DPAD>
-__global__ void __launch_bounds__(DkvGeom<T, DPAD>::THREADS, DPAD == 64 ? 2 : 1)
+__global__ void __launch_bounds__(kThreads, Geom<DPAD>::CTAS)
     attend_dkdv_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                           const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mg,
                           const __grid_constant__ BwdArgs f)
 {
-    using G = DkvGeom<T, DPAD>;
+    using G = Geom<DPAD>;
+    constexpr bool APART = DPAD == 128;  // P and dS have places of their own
+    constexpr uint32_t S_COL = 0, DP_COL = kCols, DV_COL = 2 * kCols, DK_COL = 2 * kCols + DPAD;
+    constexpr uint32_t P_COL = APART ? DK_COL + DPAD : S_COL, DS_COL = APART ? P_COL + kCols / 2 : DP_COL;
+    constexpr uint32_t A_HALF = APART ? 16 : 32;  // columns from one warpgroup's P (dS) to the other's
+    constexpr uint32_t TMEM_COLS = APART ? 512 : 256;
+    static_assert(!APART || DS_COL + kCols / 2 <= 512, "tensor memory");
     const AttnArgs& a = f.a;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* sm = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     const uint32_t base = smem_addr(sm);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t row_full = base + G::OFF_BAR, fix = row_full + 8, q_full = fix + 8, q_empty = q_full + 8 * G::STAGES;
-    const uint32_t g_full = q_empty + 8 * G::STAGES, g_empty = g_full + 8 * G::STAGES, s_full = g_empty + 8 * G::STAGES;
-    const uint32_t p_full = s_full + 8, dp_full = p_full + 8, ds_full = dp_full + 8, acc_full = ds_full + 8;
+    const uint32_t row_full = base + G::OFF_BAR, fix = row_full + 8, full = fix + 8, empty = full + 16 * G::STAGES;
+    const uint32_t s_full = empty + 16 * G::STAGES, s_free = s_full + 8, p_full = s_free + 8, dp_full = p_full + 8;
+    const uint32_t dp_free = dp_full + 8, ds_full = dp_free + 8, dv_done = ds_full + 8, dk_done = dv_done + 8;
+    const uint32_t acc_full = dk_done + 8;
     uint32_t* misc = reinterpret_cast<uint32_t*>(sm + G::OFF_MISC);
-    float* stats = reinterpret_cast<float*>(sm + G::OFF_STAT);
+    float* stats = reinterpret_cast<float*>(sm + G::OFF_STAT);  // STAGES of (shift - lse, delta) of 64 queries
     const Bound bound{f.timeout_ns, reinterpret_cast<volatile int*>(misc + 1), a.err};
 
     const int kt = static_cast<int>(blockIdx.x % f.tiles);
@@ -417,19 +455,23 @@ __global__ void __launch_bounds__(DkvGeom<T, DPAD>::THREADS, DPAD == 64 ? 2 : 1)
     if (tid == 0) {
         mbar_init(row_full, 1);
         mbar_init(fix, 1);
-        for (int s = 0; s < 4 * G::STAGES; ++s) mbar_init(q_full + 8 * s, 1);
+        for (int s = 0; s < 4 * G::STAGES; ++s) mbar_init(full + 8 * s, 1);
         mbar_init(s_full, 1);
-        mbar_init(p_full, G::WARPS);
+        mbar_init(s_free, kElemWarps);
+        mbar_init(p_full, kElemWarps);
         mbar_init(dp_full, 1);
-        mbar_init(ds_full, G::WARPS);
+        mbar_init(dp_free, kElemWarps);
+        mbar_init(ds_full, kElemWarps);
+        mbar_init(dv_done, 1);
+        mbar_init(dk_done, 1);
         mbar_init(acc_full, 1);
         int first = 0, last = 0;
         if (row0 < ny && nx > 0) {
             int64_t lo, hi, lo1, hi1;
             column_cells(a, row0, nx, ny, lo, hi);
             column_cells(a, (row0 + kTile < ny ? row0 + kTile : ny) - 1, nx, ny, lo1, hi1);
-            first = static_cast<int>(lo / G::QT);
-            last = static_cast<int>((hi1 + G::QT - 1) / G::QT);
+            first = static_cast<int>(lo / kCols);
+            last = static_cast<int>((hi1 + kCols - 1) / kCols);
         }
         misc[2] = first;
         misc[3] = last;
@@ -437,7 +479,7 @@ __global__ void __launch_bounds__(DkvGeom<T, DPAD>::THREADS, DPAD == 64 ? 2 : 1)
         if (!good) atomicOr(a.err, kErrBadLength);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == G::WARPS) tmem_alloc(base + G::OFF_MISC, G::TMEM_COLS);
+    if (warp == kMmaWarp) tmem_alloc(base + G::OFF_MISC, TMEM_COLS);
     fence_before();
     __syncthreads();
     fence_after();
@@ -449,144 +491,109 @@ __global__ void __launch_bounds__(DkvGeom<T, DPAD>::THREADS, DPAD == 64 ? 2 : 1)
     const float gscale = is_half<T> ? gradient_scale(__uint_as_float(f.peak[b * a.Hkv + hk])) : 1.f;
     const float cf = is_half<T> ? gscale * exp2f(-kPShift<T>) : 1.f;
 
-    if (warp == G::WARPS + 1) {
-        // ---------------- TMA, and the queries' statistics ----------------
-        int issued_q = 0, issued_g = 0, fixes = 0;
-        bool ok = true;
-        if (n > 0) {
-            if (lane == 0) {
-                mbar_expect_tx(row_full, 2 * G::ROW_BYTES);
-                for (int x = 0; x < G::NBLOCK; ++x) {
-                    tma_load_4d(base + x * G::ROW_BLOCK, &mk, row_full, 64 * x, row0, hk, b);
-                    tma_load_4d(base + G::OFF_V + x * G::ROW_BLOCK, &mv, row_full, 64 * x, row0, hk, b);
+    if (warp == kTmaWarp) {
+        int head = hk * a.group, tile = -1;  // of the step that coords() was last asked for
+        load_tiles<DPAD>(
+            sm, base, &mk, &mv, &mq, &mg, row0, hk, b, n, nx, a.N, row_full, fix, full, empty, bound, lane,
+            [&](int, int& c0, int& hd) {
+                if (++tile == nq) {
+                    tile = 0;
+                    ++head;
                 }
-            }
-            for (int it = 0; it < n && ok; ++it) {
-                const int st = it % G::STAGES, h = hk * a.group + it / nq, i0 = (ia + it % nq) * G::QT;
-                const int64_t left = nx - i0;
-                const bool clear = left < G::QT && nx < a.N;  // rows past the length may hold NaN
-                for (int is_g = 0; is_g < 2 && ok; ++is_g) {
-                    const uint32_t fullb = (is_g ? g_full : q_full) + 8 * st, emptyb = (is_g ? g_empty : q_empty) + 8 * st;
-                    if (it >= G::STAGES && !mbar_wait(emptyb, (it / G::STAGES - 1) & 1, bound)) {
-                        ok = false;
-                        break;
-                    }
-                    if (!is_g) {
-                        // A query past the length has P = 2^-inf = 0.
-                        const int64_t at = (static_cast<int64_t>(b) * a.Hq + h) * a.N + i0;
+                c0 = (ia + tile) * kCols;
+                hd = head;
+            },
+            [&](int stage, int) {
+                const int i0 = (ia + tile) * kCols;
+                const int64_t at = (static_cast<int64_t>(b) * a.Hq + head) * a.N + i0;
+                float* st = stats + stage * 2 * kCols;
 #pragma unroll
-                        for (int c = 0; c < G::QT; c += 32) {
-                            const bool on = c + lane < left;
-                            stats[st * 2 * G::QT + c + lane] = on ? kPShift<T> - a.lse[at + c + lane] : -INFINITY;
-                            stats[st * 2 * G::QT + G::QT + c + lane] = on ? a.delta[at + c + lane] * cf : 0.f;
-                        }
-                        __syncwarp();
-                    }
-                    const int at = G::OFF_RING + (2 * st + is_g) * G::COL_BYTES;
-                    const uint32_t bar = clear ? fix : fullb;
-                    if (lane == 0) {
-                        mbar_expect_tx(bar, G::COL_BYTES);
-                        for (int x = 0; x < G::NBLOCK; ++x)
-                            tma_load_4d(base + at + x * G::COL_BLOCK, is_g ? &mg : &mq, bar, 64 * x, i0, h, b);
-                    }
-                    __syncwarp();
-                    if (clear) {
-                        if (!mbar_wait(fix, fixes & 1, bound)) ok = false;
-                        ++fixes;
-                        for (int x = 0; x < G::NBLOCK; ++x)
-                            for (int u = static_cast<int>(left) * 8 + lane; u < G::QT * 8; u += 32)
-                                *reinterpret_cast<uint4*>(sm + at + x * G::COL_BLOCK + 16 * u) = make_uint4(0, 0, 0, 0);
-                        fence_async_shared();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(fullb);
-                    }
-                    ++(is_g ? issued_g : issued_q);
+                for (int c = lane; c < kCols; c += 32) {
+                    const bool on = i0 + c < nx;  // a query past the length has P = 2^-inf = 0
+                    st[c] = on ? kPShift<T> - a.lse[at + c] : -INFINITY;
+                    st[kCols + c] = on ? a.delta[at + c] * cf : 0.f;
                 }
-            }
-            mbar_drain(row_full, 0, f.timeout_ns);
-            for (int x = issued_q < G::STAGES ? 0 : issued_q - G::STAGES; x < issued_q; ++x)
-                mbar_drain(q_full + 8 * (x % G::STAGES), (x / G::STAGES) & 1, f.timeout_ns);
-            for (int x = issued_g < G::STAGES ? 0 : issued_g - G::STAGES; x < issued_g; ++x)
-                mbar_drain(g_full + 8 * (x % G::STAGES), (x / G::STAGES) & 1, f.timeout_ns);
-        }
-    } else if (warp == G::WARPS) {
-        // ---------------- MMA ----------------
+            });
+    } else if (warp == kMmaWarp) {
         if (n > 0) {
             const uint32_t leader = elect_leader();
-            const uint32_t idesc_s = mma_idesc<T>(G::QT, false), idesc_o = mma_idesc<T>(f.dn, true);
-            const auto product = [&](uint32_t d, int rows_at, int cols_at) {
-                const uint64_t rd = desc_k(base + rows_at), cd = desc_k(base + cols_at);
-#pragma unroll
-                for (int k = 0; k < DPAD / 16; ++k)  // features past d are zero; a branch between products costs more
-                    mma_ss(tmem + d, desc_at(rd, (k / 4) * G::ROW_BLOCK + (k % 4) * 32),
-                           desc_at(cd, (k / 4) * G::COL_BLOCK + (k % 4) * 32), idesc_s, k > 0, leader);
-            };
-            // 64 columns of P or dS lie packed in the first 32 columns of their warpgroup's 64.
-            const auto gradient = [&](uint32_t d, uint32_t src, int cols_at, bool more) {
-                const uint64_t cd = desc_mn(base + cols_at, G::COL_BLOCK);
-#pragma unroll
-                for (int k = 0; k < G::QT / 16; ++k)
-                    mma_ts(tmem + d, tmem + src + (k / 4) * 64 + (k % 4) * 8, desc_at(cd, 2048 * k), idesc_o, more || k > 0, leader);
-            };
-            const auto q_at = [&](int i) { return G::OFF_RING + 2 * (i % G::STAGES) * G::COL_BYTES; };
+            const uint32_t idesc_s = mma_idesc<T>(kCols, false), idesc_o = mma_idesc<T>(f.dn, true);
+            Turn<G::STAGES> sq, sg, now;  // the next S, the next dP, the tile whose sums are due
+            const auto ring = [&](int at, int which) { return base + G::OFF_RING + (2 * at + which) * G::COL_BYTES; };
+            // S (dP) of tile i, when the elementwise warps have read the last one, and, where P (dS) lies over it, the
+            // product that reads that has completed.
             const auto scores = [&](int i) {
-                if (!mbar_wait(q_full + 8 * (i % G::STAGES), (i / G::STAGES) & 1, bound)) return false;
+                if (!mbar_wait(full + 8 * sq.at, sq.phase, bound)) return false;
+                if (i > 0 && !mbar_wait(APART ? s_free : dv_done, (i - 1) & 1, bound)) return false;
                 fence_after();
-                product(G::S_COL, 0, q_at(i));
+                mma_rows<DPAD>(tmem + S_COL, base, ring(sq.at, 0), idesc_s, leader);
                 mma_commit(s_full, leader);
+                sq.next();
                 return true;
             };
             const auto dprobs = [&](int i) {
-                if (!mbar_wait(g_full + 8 * (i % G::STAGES), (i / G::STAGES) & 1, bound)) return false;
+                if (!mbar_wait(full + 8 * (G::STAGES + sg.at), sg.phase, bound)) return false;
+                if (i > 0 && !mbar_wait(APART ? dp_free : dk_done, (i - 1) & 1, bound)) return false;
                 fence_after();
-                product(G::DP_COL, G::OFF_V, q_at(i) + G::COL_BYTES);
+                mma_rows<DPAD>(tmem + DP_COL, base + G::ROW_BYTES, ring(sg.at, 1), idesc_s, leader);
                 mma_commit(dp_full, leader);
+                sg.next();
                 return true;
             };
             bool ok = mbar_wait(row_full, 0, bound) && scores(0) && dprobs(0);
             for (int i = 0; ok && i < n; ++i) {
-                ok = mbar_wait(p_full, i & 1, bound);
-                if (!ok) break;
+                const bool more = i + 1 < n;
+                if (APART && more && !(ok = scores(i + 1))) break;
+                if (!(ok = mbar_wait(p_full, i & 1, bound))) break;
                 fence_after();
-                gradient(G::DV_COL, G::S_COL, q_at(i) + G::COL_BYTES, i > 0);
-                mma_commit(g_empty + 8 * (i % G::STAGES), leader);
-                if (i + 1 < n && !(ok = scores(i + 1))) break;
-                ok = mbar_wait(ds_full, i & 1, bound);
-                if (!ok) break;
+                mma_cols<DPAD>(tmem + DV_COL, tmem + P_COL, A_HALF, ring(now.at, 1), idesc_o, i > 0, leader);
+                mma_commit(dv_done, leader);
+                mma_commit(empty + 8 * (G::STAGES + now.at), leader);
+                if (!APART && more && !(ok = scores(i + 1))) break;
+                if (APART && more && !(ok = dprobs(i + 1))) break;
+                if (!(ok = mbar_wait(ds_full, i & 1, bound))) break;
                 fence_after();
-                gradient(G::DK_COL, G::DP_COL, q_at(i), i > 0);
-                mma_commit(q_empty + 8 * (i % G::STAGES), leader);
-                if (i + 1 < n) ok = dprobs(i + 1);
+                mma_cols<DPAD>(tmem + DK_COL, tmem + DS_COL, A_HALF, ring(now.at, 0), idesc_o, i > 0, leader);
+                mma_commit(dk_done, leader);
+                mma_commit(empty + 8 * now.at, leader);
+                if (!APART && more) ok = dprobs(i + 1);
+                now.next();
             }
             mma_commit(acc_full, leader);
             mbar_drain(acc_full, 0, f.timeout_ns);  // before the tensor memory is given back
         }
         __syncwarp();
     } else {
-        // ---------------- elementwise: one state a thread, 64 queries a warpgroup ----------------
-        const int wg = warp >> 2;
-        const int64_t j = row0 + (tid & 127);
+        // ---------------- elementwise: two threads a state, 32 queries each ----------------
+        const int half = warp >> 2;
+        const int64_t j = row0 + 32 * (warp & 3) + lane;
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-        const uint32_t ts = tmem + lanes + G::S_COL + 64 * wg, tdp = tmem + lanes + G::DP_COL + 64 * wg;
+        const uint32_t ts = tmem + lanes + S_COL + 32 * half, tdp = tmem + lanes + DP_COL + 32 * half;
+        const uint32_t tp = tmem + lanes + P_COL + A_HALF * half, tds = tmem + lanes + DS_COL + A_HALF * half;
         int64_t lo = 0, hi = 0;
         if (j < ny && nx > 0) column_cells(a, j, nx, ny, lo, hi);
         const int ilo = static_cast<int>(lo), width = static_cast<int>(hi - lo);
         bool ok = true;
+        Turn<G::STAGES> turn;
+        int tile = 0;
         for (int it = 0; it < n; ++it) {
-            const int st = it % G::STAGES;
-            if (!(ok = mbar_wait(q_full + 8 * st, (it / G::STAGES) & 1, bound) && mbar_wait(s_full, it & 1, bound))) break;
+            if (!(ok = mbar_wait(full + 8 * turn.at, turn.phase, bound) && mbar_wait(s_full, it & 1, bound))) break;
             fence_after();
-            const float* lse = stats + st * 2 * G::QT + 64 * wg;
-            const float* delta = lse + G::QT;
-            uint32_t s[64], p[64];
+            const float* lse = stats + turn.at * 2 * kCols + 32 * half;
+            const float* delta = lse + kCols;
+            uint32_t s[32], p[32];
             tmem_ld32(ts, s);
-            tmem_ld32(ts + 32, s + 32);
             wait_ld();
             settle(s);
-            const int off = (ia + it % nq) * G::QT + 64 * wg - ilo;
-            const bool whole = __all_sync(kFull, off >= 0 && off + 64 <= width);
+            if (APART) {
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_free);
+            }
+            const int off = (ia + tile) * kCols + 32 * half - ilo;
+            const bool whole = __all_sync(kFull, off >= 0 && off + 32 <= width);
 #pragma unroll
-            for (int c = 0; c < 64; c += 4) {
+            for (int c = 0; c < 32; c += 4) {
                 const float4 b4 = *reinterpret_cast<const float4*>(lse + c);
                 s[c] = __float_as_uint(ex2f(fmaf(__uint_as_float(s[c]), a.scale_log2, b4.x)));
                 s[c + 1] = __float_as_uint(ex2f(fmaf(__uint_as_float(s[c + 1]), a.scale_log2, b4.y)));
@@ -595,16 +602,15 @@ __global__ void __launch_bounds__(DkvGeom<T, DPAD>::THREADS, DPAD == 64 ? 2 : 1)
             }
             if (!whole) {
 #pragma unroll
-                for (int c = 0; c < 64; ++c)
+                for (int c = 0; c < 32; ++c)
                     if (static_cast<unsigned>(off + c) >= static_cast<unsigned>(width)) s[c] = 0;
             }
+            uint32_t w[16];
 #pragma unroll
-            for (int c = 0; c < 64; c += 32) {
-                uint32_t w[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) w[e] = pack2(__uint_as_float(s[c + 2 * e]), __uint_as_float(s[c + 2 * e + 1]), T());
-                tmem_st16(ts + c / 2, w);
-            }
+            for (int e = 0; e < 16; ++e) w[e] = pack2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]), T());
+            if (APART && it > 0 && !(ok = mbar_wait(dv_done, (it - 1) & 1, bound))) break;
+            fence_after();
+            tmem_st16(tp, w);
             wait_st();
             fence_before();
             __syncwarp();
@@ -612,72 +618,52 @@ __global__ void __launch_bounds__(DkvGeom<T, DPAD>::THREADS, DPAD == 64 ? 2 : 1)
             if (!(ok = mbar_wait(dp_full, it & 1, bound))) break;
             fence_after();
             tmem_ld32(tdp, p);
-            tmem_ld32(tdp + 32, p + 32);
             wait_ld();
             settle(p);
-#pragma unroll
-            for (int c = 0; c < 64; c += 32) {
-                uint32_t w[16];
-#pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                    const int x = c + 2 * e;
-                    const float4 d4 = *reinterpret_cast<const float4*>(delta + x);
-                    const float dd[4] = {d4.x, d4.y, d4.z, d4.w};
-                    float v[4];
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                        const float dp = __uint_as_float(p[x + y]);
-                        v[y] = __uint_as_float(s[x + y]) * (is_half<T> ? fmaf(dp, cf, -dd[y]) : dp - dd[y]);
-                    }
-                    w[e] = pack2(v[0], v[1], T());
-                    w[e + 1] = pack2(v[2], v[3], T());
-                }
-                tmem_st16(tdp + c / 2, w);
+            if (APART) {
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(dp_free);
             }
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+                const float4 d4 = *reinterpret_cast<const float4*>(delta + 2 * e);
+                const float dd[4] = {d4.x, d4.y, d4.z, d4.w};
+                float v[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const float dp = __uint_as_float(p[2 * e + y]);
+                    v[y] = __uint_as_float(s[2 * e + y]) * (is_half<T> ? fmaf(dp, cf, -dd[y]) : dp - dd[y]);
+                }
+                w[e] = pack2(v[0], v[1], T());
+                w[e + 1] = pack2(v[2], v[3], T());
+            }
+            if (APART && it > 0 && !(ok = mbar_wait(dk_done, (it - 1) & 1, bound))) break;
+            fence_after();
+            tmem_st16(tds, w);
             wait_st();
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(ds_full);
+            turn.next();
+            if (++tile == nq) tile = 0;
         }
         if (ok && n > 0) ok = mbar_wait(acc_full, 0, bound);
         fence_after();
-        ok = __all_sync(kFull, ok);
-        const float back_k = a.scale / gscale, back_v = is_half<T> ? exp2f(-kPShift<T>) : 1.f;
-        const int64_t at = ((static_cast<int64_t>(b) * a.M + j) * a.Hkv + hk) * a.d;
-        for (int u = wg; u < 2 * (f.dn / 16); u += G::WGS) {  // 16 features of dv or dk at a time
-            const bool is_k = u >= f.dn / 16;
-            const int c = (is_k ? u - f.dn / 16 : u) * 16;
-            const float back = is_k ? back_k : back_v;
-            uint32_t o[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = 0;
-            if (n > 0 && ok) {
-                tmem_ld16(tmem + lanes + (is_k ? G::DK_COL : G::DV_COL) + c, o);
-                wait_ld();
-                settle(o);
-            }
-            if (j >= a.M) continue;
-            T* out = static_cast<T*>(is_k ? a.dk : a.dv) + at + c;
-#pragma unroll
-            for (int e = 0; e < 16; e += 8) {
-                if (c + e >= a.d) break;
-                uint32_t w[4];
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    float v0 = width > 0 ? __uint_as_float(o[e + 2 * x]) * back : 0.f;
-                    float v1 = width > 0 ? __uint_as_float(o[e + 2 * x + 1]) * back : 0.f;
-                    if (!ok) v0 = v1 = __int_as_float(0x7fc00000);
-                    w[x] = pack2(v0, v1, T());
-                }
-                *reinterpret_cast<uint4*>(out + e) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-        }
+        // K's and V's places hold the rows on their way out: all products are done.
+        const int64_t j0 = row0 + 32 * (warp & 3);
+        const int64_t at = ((static_cast<int64_t>(b) * a.M + j0) * a.Hkv + hk) * a.d, pitch = static_cast<int64_t>(a.Hkv) * a.d;
+        uint4* rows = reinterpret_cast<uint4*>(sm) + (warp & 3) * 32 * (DPAD / 8);
+        store_rows<T, DPAD>(tmem + lanes + DK_COL, rows, lane, half, 2 + (warp & 3), n > 0 && ok, width > 0, !ok, a.scale / gscale,
+                            f.dn, a.d, static_cast<T*>(a.dk) + at, pitch, a.M - j0);
+        store_rows<T, DPAD>(tmem + lanes + DV_COL, rows + G::ROW_BYTES / 16, lane, half, 2 + (warp & 3), n > 0 && ok, width > 0, !ok,
+                            is_half<T> ? exp2f(-kPShift<T>) : 1.f, f.dn, a.d, static_cast<T*>(a.dv) + at, pitch, a.M - j0);
         fence_before();
     }
     __syncthreads();
-    if (warp == G::WARPS) {
+    if (warp == kMmaWarp) {
         fence_after();
-        tmem_free(tmem, G::TMEM_COLS);
+        tmem_free(tmem, TMEM_COLS);
     }
 }
 
@@ -690,38 +676,36 @@ cudaError_t allow_smem(K kernel, int bytes)
 template <typename T, int DPAD>
 cudaError_t backward_d(BwdArgs& f, cudaStream_t s)
 {
-    using GQ = DqGeom<T, DPAD>;
-    using GK = DkvGeom<T, DPAD>;
+    using G = Geom<DPAD>;
     const AttnArgs& a = f.a;
-    static_assert(GQ::KT == GK::QT, "one set of maps serves both launches");
     constexpr bool half = is_half<T>;
-    // As rows of a product (128 a tile) and as columns (KT a tile).
+    // As rows of a product (128 a tile) and as columns (64 a tile).
     CUtensorMap q_rows, g_rows, k_cols, v_cols, k_rows, v_rows, q_cols, g_cols;
     const cudaError_t bad = cudaErrorInvalidValue;
     cudaError_t e;
     if (a.N > 0 && a.M > 0) {
         if (!attention_tile_map(&q_rows, half, a.q, a.qs, a.B, a.N, a.Hq, a.d, kTile) ||
             !attention_tile_map(&g_rows, half, a.dout, a.gs, a.B, a.N, a.Hq, a.d, kTile) ||
-            !attention_tile_map(&k_cols, half, a.k, a.ks, a.B, a.M, a.Hkv, a.d, GQ::KT) ||
-            !attention_tile_map(&v_cols, half, a.v, a.vs, a.B, a.M, a.Hkv, a.d, GQ::KT) ||
+            !attention_tile_map(&k_cols, half, a.k, a.ks, a.B, a.M, a.Hkv, a.d, kCols) ||
+            !attention_tile_map(&v_cols, half, a.v, a.vs, a.B, a.M, a.Hkv, a.d, kCols) ||
             !attention_tile_map(&k_rows, half, a.k, a.ks, a.B, a.M, a.Hkv, a.d, kTile) ||
             !attention_tile_map(&v_rows, half, a.v, a.vs, a.B, a.M, a.Hkv, a.d, kTile) ||
-            !attention_tile_map(&q_cols, half, a.q, a.qs, a.B, a.N, a.Hq, a.d, GK::QT) ||
-            !attention_tile_map(&g_cols, half, a.dout, a.gs, a.B, a.N, a.Hq, a.d, GK::QT))
+            !attention_tile_map(&q_cols, half, a.q, a.qs, a.B, a.N, a.Hq, a.d, kCols) ||
+            !attention_tile_map(&g_cols, half, a.dout, a.gs, a.B, a.N, a.Hq, a.d, kCols))
             return bad;
     }
     if (half) {
         e = cudaMemsetAsync(f.peak, 0, sizeof(uint32_t) * static_cast<size_t>(a.B) * a.Hkv, s);
         if (e != cudaSuccess) return e;
     }
-    if ((e = allow_smem(attend_dq_tc_kernel<T, DPAD>, GQ::BYTES)) != cudaSuccess) return e;
-    if ((e = allow_smem(attend_dkdv_tc_kernel<T, DPAD>, GK::BYTES)) != cudaSuccess) return e;
+    if ((e = allow_smem(attend_dq_tc_kernel<T, DPAD>, G::BYTES)) != cudaSuccess) return e;
+    if ((e = allow_smem(attend_dkdv_tc_kernel<T, DPAD>, G::BYTES)) != cudaSuccess) return e;
     f.tiles = static_cast<int>((a.N + kTile - 1) / kTile);
-    attend_dq_tc_kernel<T, DPAD><<<static_cast<unsigned>(static_cast<int64_t>(a.B) * a.Hq * f.tiles), GQ::THREADS, GQ::BYTES, s>>>(
+    attend_dq_tc_kernel<T, DPAD><<<static_cast<unsigned>(static_cast<int64_t>(a.B) * a.Hq * f.tiles), kThreads, G::BYTES, s>>>(
         q_rows, g_rows, k_cols, v_cols, f);
     count_launch();
     f.tiles = static_cast<int>((a.M + kTile - 1) / kTile);
-    attend_dkdv_tc_kernel<T, DPAD><<<static_cast<unsigned>(static_cast<int64_t>(a.B) * a.Hkv * f.tiles), GK::THREADS, GK::BYTES, s>>>(
+    attend_dkdv_tc_kernel<T, DPAD><<<static_cast<unsigned>(static_cast<int64_t>(a.B) * a.Hkv * f.tiles), kThreads, G::BYTES, s>>>(
         k_rows, v_rows, q_cols, g_cols, f);
     count_launch();
     return cudaGetLastError();

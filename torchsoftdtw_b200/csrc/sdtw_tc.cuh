@@ -41,7 +41,7 @@ struct Bound {
 
 // Waits for the phase with the given parity. False when it ran out of time, or another role of the CTA did. The
 // clock is first read after 256 tries (each of which the hardware suspends for a while): waits of a healthy CTA never pay for it.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const Bound& w)
+__device__ __forceinline__ bool mbar_wait_lane(uint32_t bar, uint32_t parity, const Bound& w)
 {
 #pragma unroll 1
     for (int i = 0; i < 256; ++i)
@@ -58,6 +58,11 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const B
             return false;
         }
     }
+}
+// The same by a whole warp, with one answer for all its lanes.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const Bound& w)
+{
+    return __all_sync(kFull, mbar_wait_lane(bar, parity, w));
 }
 // The same wait for one's own operations in flight, which goes on after an abort.
 __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity, uint64_t timeout_ns)
