@@ -5,9 +5,10 @@
 // Seven products where one launch with atomic sums of dq would take five: the price of sums in one fixed order.
 // P and dS go to tensor memory as the 16-bit A operand of the next product, so nothing of size queries x states leaves
 // the SM. A CTA keeps 128 rows (of Q and dO, or of K and V) and streams 64 columns (of the other two) at a time; eight
-// elementwise warps take two threads a row, 32 columns each. Products complete in no promised order among themselves, so
-// whatever one of them reads is only overwritten when it has been awaited: where tensor memory has room (d > 64), P and dS have
-// places of their own beside S and dP, and scores run a tile ahead; where two CTAs share it (d <= 64) they lie over S and dP.
+// elementwise warps take a tile, two threads a row, 32 columns each. Products complete in no promised order among themselves,
+// so whatever one of them reads is only overwritten when it has been awaited. To have work for the tensor core meanwhile, two
+// tiles are in flight on an SM: of two CTAs (d <= 64), or of one that has two groups of elementwise warps and two sets of S and
+// dP in tensor memory, for the even and the odd tiles (BUFS = 2).
 //
 // fp16: P is kept 2^10 larger and dS scaled by a power of two that brings the rows' |do| to [8, 16) (a row's own in
 // dq, where a row is a lane; the largest of the head in dk), so that neither under- nor overflows where the gradients do not.
@@ -47,9 +48,6 @@ __device__ __forceinline__ float gradient_scale(float norm2)
 }
 
 constexpr int kCols = 64;  // columns of a product: states in dq, queries in dk/dv
-constexpr int kElemWarps = 8;
-constexpr int kMmaWarp = kElemWarps, kTmaWarp = kElemWarps + 1;
-constexpr int kThreads = 32 * (kElemWarps + 2);
 
 // Shared memory: the two row operands, a ring of pairs of column tiles, statistics, barriers.
 template <int DPAD>
@@ -58,12 +56,15 @@ struct Geom {
     static constexpr int ROW_BLOCK = kTile * 128, COL_BLOCK = kCols * 128;  // 64 features of a tile
     static constexpr int NBLOCK = DPAD / 64;
     static constexpr int STAGES = DPAD == 128 ? 4 : 3;
+    static constexpr int BUFS = DPAD == 128 ? 2 : 1;  // tiles in flight
+    static constexpr int ELEM_WARPS = 8 * BUFS, MMA_WARP = ELEM_WARPS, TMA_WARP = ELEM_WARPS + 1;
+    static constexpr int THREADS = 32 * (ELEM_WARPS + 2);
     static constexpr int OFF_RING = 2 * ROW_BYTES;
     static constexpr int OFF_STAT = OFF_RING + STAGES * 2 * COL_BYTES;
     static constexpr int STAT_BYTES = 4 * (STAGES * 2 * kCols > 2 * kTile ? STAGES * 2 * kCols : 2 * kTile);
     static constexpr int OFF_BAR = OFF_STAT + STAT_BYTES;
-    // row_full, fix, full[2][STAGES], empty[2][STAGES], and eight more
-    static constexpr int NBAR = 2 + 4 * STAGES + 9;
+    // row_full, fix, full[2][STAGES], empty[2][STAGES], acc_full, and six a buffer
+    static constexpr int NBAR = 3 + 4 * STAGES + 6 * BUFS;
     static constexpr int OFF_MISC = OFF_BAR + 8 * NBAR;
     static constexpr int BYTES = OFF_MISC + 32 + 1024;
     static constexpr int CTAS = DPAD == 64 ? 2 : 1;  // an SM
@@ -207,22 +208,25 @@ __device__ __forceinline__ void mma_cols(uint32_t d, uint32_t a, uint32_t half, 
 }
 
 template <typename T, int DPAD>
-__global__ void __launch_bounds__(kThreads, Geom<DPAD>::CTAS)
+__global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
     attend_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mg,
                         const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                         const __grid_constant__ BwdArgs f)
 {
     using G = Geom<DPAD>;
-    constexpr uint32_t S_COL = 0, DP_COL = kCols, DS_COL = 2 * kCols, ACC_COL = 2 * kCols + kCols / 2;
+    // Each buffer: S, dP, dS.
+    constexpr uint32_t DP_COL = kCols, DS_COL = 2 * kCols, BUF_COLS = 2 * kCols + kCols / 2, ACC_COL = G::BUFS * BUF_COLS;
     constexpr uint32_t TMEM_COLS = ACC_COL + DPAD <= 256 ? 256 : 512;
+    static_assert(ACC_COL + DPAD <= 512, "tensor memory");
     const AttnArgs& a = f.a;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* sm = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     const uint32_t base = smem_addr(sm);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t row_full = base + G::OFF_BAR, fix = row_full + 8, full = fix + 8, empty = full + 16 * G::STAGES;
-    const uint32_t s_full = empty + 16 * G::STAGES, s_free = s_full + 8, dp_full = s_free + 8, dp_free = dp_full + 8;
-    const uint32_t ds_full = dp_free + 8, ds_free = ds_full + 8, acc_full = ds_free + 8;
+    const uint32_t acc_full = empty + 16 * G::STAGES, s_full = acc_full + 8, s_free = s_full + 8 * G::BUFS;
+    const uint32_t dp_full = s_free + 8 * G::BUFS, dp_free = dp_full + 8 * G::BUFS, ds_full = dp_free + 8 * G::BUFS;
+    const uint32_t ds_free = ds_full + 8 * G::BUFS;
     uint32_t* misc = reinterpret_cast<uint32_t*>(sm + G::OFF_MISC);
     float* s_delta = reinterpret_cast<float*>(sm + G::OFF_STAT);
     float* s_norm = s_delta + kTile;
@@ -238,13 +242,15 @@ __global__ void __launch_bounds__(kThreads, Geom<DPAD>::CTAS)
         mbar_init(row_full, 1);
         mbar_init(fix, 1);
         for (int s = 0; s < 4 * G::STAGES; ++s) mbar_init(full + 8 * s, 1);
-        mbar_init(s_full, 1);
-        mbar_init(s_free, kElemWarps);
-        mbar_init(dp_full, 1);
-        mbar_init(dp_free, kElemWarps);
-        mbar_init(ds_full, kElemWarps);
-        mbar_init(ds_free, 1);
         mbar_init(acc_full, 1);
+        for (int x = 0; x < G::BUFS; ++x) {
+            mbar_init(s_full + 8 * x, 1);
+            mbar_init(s_free + 8 * x, 8);
+            mbar_init(dp_full + 8 * x, 1);
+            mbar_init(dp_free + 8 * x, 8);
+            mbar_init(ds_full + 8 * x, 8);
+            mbar_init(ds_free + 8 * x, 1);
+        }
         int first = 0, last = 0;
         if (row0 < nx && ny > 0) {
             int64_t lo, hi, lo1, hi1;
@@ -259,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, Geom<DPAD>::CTAS)
         if (!good) atomicOr(a.err, kErrBadLength);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kMmaWarp) tmem_alloc(base + G::OFF_MISC, TMEM_COLS);
+    if (warp == G::MMA_WARP) tmem_alloc(base + G::OFF_MISC, TMEM_COLS);
     fence_before();
     __syncthreads();
     fence_after();
@@ -267,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, Geom<DPAD>::CTAS)
     const int ja = static_cast<int>(*reinterpret_cast<volatile uint32_t*>(misc + 2));
     const int n = static_cast<int>(*reinterpret_cast<volatile uint32_t*>(misc + 3)) - ja;
 
-    if (warp == kTmaWarp) {
+    if (warp == G::TMA_WARP) {
         load_tiles<DPAD>(
             sm, base, &mq, &mg, &mk, &mv, row0, h, b, n, ny, a.M, row_full, fix, full, empty, bound, lane,
             [&](int t, int& c0, int& head) {
@@ -275,35 +281,39 @@ __global__ void __launch_bounds__(kThreads, Geom<DPAD>::CTAS)
                 head = hk;
             },
             [](int, int) {});
-    } else if (warp == kMmaWarp) {
+    } else if (warp == G::MMA_WARP) {
         if (n > 0) {
             const uint32_t leader = elect_leader();
             const uint32_t idesc_s = mma_idesc<T>(kCols, false), idesc_q = mma_idesc<T>(f.dn, true);
             Turn<G::STAGES> ahead, now;
             const auto ring = [&](int at, int which) { return base + G::OFF_RING + (2 * at + which) * G::COL_BYTES; };
-            // S and dP of the next tile, each as soon as the elementwise warps have read the last one's.
+            // S and dP of tile i, each as soon as the elementwise warps have read the last ones of its buffer.
             const auto next_products = [&](int i) {
+                const int x = i % G::BUFS;
+                const uint32_t before = (i / G::BUFS - 1) & 1, col = tmem + x * BUF_COLS;
                 if (!mbar_wait(full + 8 * ahead.at, ahead.phase, bound)) return false;
-                if (i > 0 && !mbar_wait(s_free, (i - 1) & 1, bound)) return false;
+                if (i >= G::BUFS && !mbar_wait(s_free + 8 * x, before, bound)) return false;
                 fence_after();
-                mma_rows<DPAD>(tmem + S_COL, base, ring(ahead.at, 0), idesc_s, leader);
-                mma_commit(s_full, leader);
+                mma_rows<DPAD>(col, base, ring(ahead.at, 0), idesc_s, leader);
+                mma_commit(s_full + 8 * x, leader);
                 if (!mbar_wait(full + 8 * (G::STAGES + ahead.at), ahead.phase, bound)) return false;
-                if (i > 0 && !mbar_wait(dp_free, (i - 1) & 1, bound)) return false;
+                if (i >= G::BUFS && !mbar_wait(dp_free + 8 * x, before, bound)) return false;
                 fence_after();
-                mma_rows<DPAD>(tmem + DP_COL, base + G::ROW_BYTES, ring(ahead.at, 1), idesc_s, leader);
-                mma_commit(dp_full, leader);
+                mma_rows<DPAD>(col + DP_COL, base + G::ROW_BYTES, ring(ahead.at, 1), idesc_s, leader);
+                mma_commit(dp_full + 8 * x, leader);
                 mma_commit(empty + 8 * (G::STAGES + ahead.at), leader);
                 ahead.next();
                 return true;
             };
-            bool ok = mbar_wait(row_full, 0, bound) && next_products(0);
+            bool ok = mbar_wait(row_full, 0, bound);
+            for (int i = 0; i < G::BUFS && i < n; ++i) ok = ok && next_products(i);
             for (int i = 0; ok && i < n; ++i) {
-                if (i + 1 < n && !(ok = next_products(i + 1))) break;
-                if (!(ok = mbar_wait(ds_full, i & 1, bound))) break;
+                const int x = i % G::BUFS;
+                if (i + G::BUFS < n && !(ok = next_products(i + G::BUFS))) break;
+                if (!(ok = mbar_wait(ds_full + 8 * x, (i / G::BUFS) & 1, bound))) break;
                 fence_after();
-                mma_cols<DPAD>(tmem + ACC_COL, tmem + DS_COL, 16, ring(now.at, 0), idesc_q, i > 0, leader);
-                mma_commit(ds_free, leader);
+                mma_cols<DPAD>(tmem + ACC_COL, tmem + x * BUF_COLS + DS_COL, 16, ring(now.at, 0), idesc_q, i > 0, leader);
+                mma_commit(ds_free + 8 * x, leader);
                 mma_commit(empty + 8 * now.at, leader);
                 now.next();
             }
@@ -316,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, Geom<DPAD>::CTAS)
         // delta and |do|^2 of the tile's rows: LPR lanes a row.
         constexpr int LPR = DPAD / 8, RPW = 32 / LPR;
 #pragma unroll 4
-        for (int r0 = warp * RPW; r0 < kTile; r0 += kElemWarps * RPW) {
+        for (int r0 = warp * RPW; r0 < kTile; r0 += G::ELEM_WARPS * RPW) {
             const int r = r0 + lane / LPR, c = lane % LPR * 8;
             const int64_t i = row0 + r;
             float dot = 0.f, nrm = 0.f;
@@ -346,22 +356,23 @@ __global__ void __launch_bounds__(kThreads, Geom<DPAD>::CTAS)
                 if (is_half<T> && i < nx) atomicMax(f.peak + b * a.Hkv + hk, __float_as_uint(nrm));
             }
         }
-        const int half = warp >> 2, r = 32 * (warp & 3) + lane;
+        const int x = warp >> 3, half = (warp >> 2) & 1, r = 32 * (warp & 3) + lane;  // x: the buffer of this group of warps
         const int64_t i = row0 + r;
         int64_t lo = 0, hi = 0;
         if (i < nx && ny > 0) row_cells(a, i, nx, ny, lo, hi);
         const int ilo = static_cast<int>(lo), width = static_cast<int>(hi - lo);
         const float lse = width > 0 ? a.lse[(static_cast<int64_t>(b) * a.Hq + h) * a.N + i] : INFINITY;
-        asm volatile("barrier.cta.sync 1, %0;" ::"n"(32 * kElemWarps) : "memory");
+        asm volatile("barrier.cta.sync 1, %0;" ::"n"(32 * G::ELEM_WARPS) : "memory");
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-        const uint32_t ts = tmem + lanes + S_COL + 32 * half, tdp = tmem + lanes + DP_COL + 32 * half;
-        const uint32_t tds = tmem + lanes + DS_COL + 16 * half;
+        const uint32_t ts = tmem + lanes + x * BUF_COLS + 32 * half, tdp = ts + DP_COL;
+        const uint32_t tds = tmem + lanes + x * BUF_COLS + DS_COL + 16 * half;
         const float gscale = is_half<T> ? gradient_scale(s_norm[r]) : 1.f;
         const float cf = is_half<T> ? gscale * exp2f(-kPShift<T>) : 1.f;
         const float delta = s_delta[r] * cf, bias = kPShift<T> - lse;
         bool ok = true;
-        for (int it = 0; it < n; ++it) {
-            if (!(ok = mbar_wait(s_full, it & 1, bound))) break;
+        for (int it = x; it < n; it += G::BUFS) {
+            const uint32_t phase = (it / G::BUFS) & 1;
+            if (!(ok = mbar_wait(s_full + 8 * x, phase, bound))) break;
             fence_after();
             uint32_t s[32], p[32];
             tmem_ld32(ts, s);
@@ -369,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, Geom<DPAD>::CTAS)
             settle(s);
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(s_free);
+            if (lane == 0) mbar_arrive(s_free + 8 * x);
             const int off = (ja + it) * kCols + 32 * half - ilo;
             const bool whole = __all_sync(kFull, off >= 0 && off + 32 <= width);
 #pragma unroll
@@ -380,14 +391,14 @@ __global__ void __launch_bounds__(kThreads, Geom<DPAD>::CTAS)
                 for (int c = 0; c < 32; ++c)
                     if (static_cast<unsigned>(off + c) >= static_cast<unsigned>(width)) s[c] = 0;
             }
-            if (!(ok = mbar_wait(dp_full, it & 1, bound))) break;
+            if (!(ok = mbar_wait(dp_full + 8 * x, phase, bound))) break;
             fence_after();
             tmem_ld32(tdp, p);
             wait_ld();
             settle(p);
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(dp_free);
+            if (lane == 0) mbar_arrive(dp_free + 8 * x);
             uint32_t w[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -396,53 +407,52 @@ __global__ void __launch_bounds__(kThreads, Geom<DPAD>::CTAS)
                 const float d1 = is_half<T> ? fmaf(p1, cf, -delta) : p1 - delta;
                 w[e] = pack2(__uint_as_float(s[2 * e]) * d0, __uint_as_float(s[2 * e + 1]) * d1, T());
             }
-            if (it > 0 && !(ok = mbar_wait(ds_free, (it - 1) & 1, bound))) break;
+            if (it >= G::BUFS && !(ok = mbar_wait(ds_free + 8 * x, phase ^ 1, bound))) break;
             fence_after();
             tmem_st16(tds, w);
             wait_st();
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(ds_full);
+            if (lane == 0) mbar_arrive(ds_full + 8 * x);
         }
         if (ok && n > 0) ok = mbar_wait(acc_full, 0, bound);
         fence_after();
         // Q's place holds the rows on their way out: all scores are done.
         const int64_t i0 = row0 + 32 * (warp & 3);
-        store_rows<T, DPAD>(tmem + lanes + ACC_COL, reinterpret_cast<uint4*>(sm) + (warp & 3) * 32 * (DPAD / 8), lane, half,
+        if (x == 0)
+            store_rows<T, DPAD>(tmem + lanes + ACC_COL, reinterpret_cast<uint4*>(sm) + (warp & 3) * 32 * (DPAD / 8), lane, half,
                             2 + (warp & 3), n > 0 && ok, width > 0, !ok, a.scale / gscale, f.dn, a.d,
                             static_cast<T*>(a.dq) + ((static_cast<int64_t>(b) * a.N + i0) * a.Hq + h) * a.d,
                             static_cast<int64_t>(a.Hq) * a.d, a.N - i0);
         fence_before();
     }
     __syncthreads();
-    if (warp == kMmaWarp) {
+    if (warp == G::MMA_WARP) {
         fence_after();
         tmem_free(tmem, TMEM_COLS);
     }
 }
 
 template <typename T, int DPAD>
-__global__ void __launch_bounds__(kThreads, Geom<DPAD>::CTAS)
+__global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
     attend_dkdv_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                           const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mg,
                           const __grid_constant__ BwdArgs f)
 {
     using G = Geom<DPAD>;
-    constexpr bool APART = DPAD == 128;  // P and dS have places of their own
-    constexpr uint32_t S_COL = 0, DP_COL = kCols, DV_COL = 2 * kCols, DK_COL = 2 * kCols + DPAD;
-    constexpr uint32_t P_COL = APART ? DK_COL + DPAD : S_COL, DS_COL = APART ? P_COL + kCols / 2 : DP_COL;
-    constexpr uint32_t A_HALF = APART ? 16 : 32;  // columns from one warpgroup's P (dS) to the other's
-    constexpr uint32_t TMEM_COLS = APART ? 512 : 256;
-    static_assert(!APART || DS_COL + kCols / 2 <= 512, "tensor memory");
+    // Each buffer: S, then P packed at the start of each half's columns; dP, then dS.
+    constexpr uint32_t DP_COL = kCols, BUF_COLS = 2 * kCols, DV_COL = G::BUFS * BUF_COLS, DK_COL = DV_COL + DPAD;
+    constexpr uint32_t TMEM_COLS = DK_COL + DPAD <= 256 ? 256 : 512;
+    static_assert(DK_COL + DPAD <= 512, "tensor memory");
     const AttnArgs& a = f.a;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* sm = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     const uint32_t base = smem_addr(sm);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t row_full = base + G::OFF_BAR, fix = row_full + 8, full = fix + 8, empty = full + 16 * G::STAGES;
-    const uint32_t s_full = empty + 16 * G::STAGES, s_free = s_full + 8, p_full = s_free + 8, dp_full = p_full + 8;
-    const uint32_t dp_free = dp_full + 8, ds_full = dp_free + 8, dv_done = ds_full + 8, dk_done = dv_done + 8;
-    const uint32_t acc_full = dk_done + 8;
+    const uint32_t acc_full = empty + 16 * G::STAGES, s_full = acc_full + 8, p_full = s_full + 8 * G::BUFS;
+    const uint32_t dp_full = p_full + 8 * G::BUFS, ds_full = dp_full + 8 * G::BUFS, dv_done = ds_full + 8 * G::BUFS;
+    const uint32_t dk_done = dv_done + 8 * G::BUFS;
     uint32_t* misc = reinterpret_cast<uint32_t*>(sm + G::OFF_MISC);
     float* stats = reinterpret_cast<float*>(sm + G::OFF_STAT);  // STAGES of (shift - lse, delta) of 64 queries
     const Bound bound{f.timeout_ns, reinterpret_cast<volatile int*>(misc + 1), a.err};
@@ -456,15 +466,15 @@ __global__ void __launch_bounds__(kThreads, Geom<DPAD>::CTAS)
         mbar_init(row_full, 1);
         mbar_init(fix, 1);
         for (int s = 0; s < 4 * G::STAGES; ++s) mbar_init(full + 8 * s, 1);
-        mbar_init(s_full, 1);
-        mbar_init(s_free, kElemWarps);
-        mbar_init(p_full, kElemWarps);
-        mbar_init(dp_full, 1);
-        mbar_init(dp_free, kElemWarps);
-        mbar_init(ds_full, kElemWarps);
-        mbar_init(dv_done, 1);
-        mbar_init(dk_done, 1);
         mbar_init(acc_full, 1);
+        for (int x = 0; x < G::BUFS; ++x) {
+            mbar_init(s_full + 8 * x, 1);
+            mbar_init(p_full + 8 * x, 8);
+            mbar_init(dp_full + 8 * x, 1);
+            mbar_init(ds_full + 8 * x, 8);
+            mbar_init(dv_done + 8 * x, 1);
+            mbar_init(dk_done + 8 * x, 1);
+        }
         int first = 0, last = 0;
         if (row0 < ny && nx > 0) {
             int64_t lo, hi, lo1, hi1;
@@ -479,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, Geom<DPAD>::CTAS)
         if (!good) atomicOr(a.err, kErrBadLength);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kMmaWarp) tmem_alloc(base + G::OFF_MISC, TMEM_COLS);
+    if (warp == G::MMA_WARP) tmem_alloc(base + G::OFF_MISC, TMEM_COLS);
     fence_before();
     __syncthreads();
     fence_after();
@@ -491,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, Geom<DPAD>::CTAS)
     const float gscale = is_half<T> ? gradient_scale(__uint_as_float(f.peak[b * a.Hkv + hk])) : 1.f;
     const float cf = is_half<T> ? gscale * exp2f(-kPShift<T>) : 1.f;
 
-    if (warp == kTmaWarp) {
+    if (warp == G::TMA_WARP) {
         int head = hk * a.group, tile = -1;  // of the step that coords() was last asked for
         load_tiles<DPAD>(
             sm, base, &mk, &mv, &mq, &mg, row0, hk, b, n, nx, a.N, row_full, fix, full, empty, bound, lane,
@@ -514,49 +524,53 @@ __global__ void __launch_bounds__(kThreads, Geom<DPAD>::CTAS)
                     st[kCols + c] = on ? a.delta[at + c] * cf : 0.f;
                 }
             });
-    } else if (warp == kMmaWarp) {
+    } else if (warp == G::MMA_WARP) {
         if (n > 0) {
             const uint32_t leader = elect_leader();
             const uint32_t idesc_s = mma_idesc<T>(kCols, false), idesc_o = mma_idesc<T>(f.dn, true);
             Turn<G::STAGES> sq, sg, now;  // the next S, the next dP, the tile whose sums are due
             const auto ring = [&](int at, int which) { return base + G::OFF_RING + (2 * at + which) * G::COL_BYTES; };
-            // S (dP) of tile i, when the elementwise warps have read the last one, and, where P (dS) lies over it, the
-            // product that reads that has completed.
+            // S (dP) of tile i, when the product that read P (dS) there has completed.
             const auto scores = [&](int i) {
+                const int x = i % G::BUFS;
                 if (!mbar_wait(full + 8 * sq.at, sq.phase, bound)) return false;
-                if (i > 0 && !mbar_wait(APART ? s_free : dv_done, (i - 1) & 1, bound)) return false;
+                if (i >= G::BUFS && !mbar_wait(dv_done + 8 * x, (i / G::BUFS - 1) & 1, bound)) return false;
                 fence_after();
-                mma_rows<DPAD>(tmem + S_COL, base, ring(sq.at, 0), idesc_s, leader);
-                mma_commit(s_full, leader);
+                mma_rows<DPAD>(tmem + x * BUF_COLS, base, ring(sq.at, 0), idesc_s, leader);
+                mma_commit(s_full + 8 * x, leader);
                 sq.next();
                 return true;
             };
             const auto dprobs = [&](int i) {
+                const int x = i % G::BUFS;
                 if (!mbar_wait(full + 8 * (G::STAGES + sg.at), sg.phase, bound)) return false;
-                if (i > 0 && !mbar_wait(APART ? dp_free : dk_done, (i - 1) & 1, bound)) return false;
+                if (i >= G::BUFS && !mbar_wait(dk_done + 8 * x, (i / G::BUFS - 1) & 1, bound)) return false;
                 fence_after();
-                mma_rows<DPAD>(tmem + DP_COL, base + G::ROW_BYTES, ring(sg.at, 1), idesc_s, leader);
-                mma_commit(dp_full, leader);
+                mma_rows<DPAD>(tmem + x * BUF_COLS + DP_COL, base + G::ROW_BYTES, ring(sg.at, 1), idesc_s, leader);
+                mma_commit(dp_full + 8 * x, leader);
                 sg.next();
                 return true;
             };
-            bool ok = mbar_wait(row_full, 0, bound) && scores(0) && dprobs(0);
+            bool ok = mbar_wait(row_full, 0, bound);
+            for (int i = 0; i < G::BUFS && i < n; ++i) ok = ok && scores(i) && dprobs(i);
             for (int i = 0; ok && i < n; ++i) {
-                const bool more = i + 1 < n;
-                if (APART && more && !(ok = scores(i + 1))) break;
-                if (!(ok = mbar_wait(p_full, i & 1, bound))) break;
+                const int x = i % G::BUFS;
+                const uint32_t phase = (i / G::BUFS) & 1;
+                const bool more = i + G::BUFS < n;
+                if (!(ok = mbar_wait(p_full + 8 * x, phase, bound))) break;
                 fence_after();
-                mma_cols<DPAD>(tmem + DV_COL, tmem + P_COL, A_HALF, ring(now.at, 1), idesc_o, i > 0, leader);
-                mma_commit(dv_done, leader);
+                mma_cols<DPAD>(tmem + DV_COL, tmem + x * BUF_COLS, 32, ring(now.at, 1), idesc_o, i > 0, leader);
+                mma_commit(dv_done + 8 * x, leader);
                 mma_commit(empty + 8 * (G::STAGES + now.at), leader);
-                if (!APART && more && !(ok = scores(i + 1))) break;
-                if (APART && more && !(ok = dprobs(i + 1))) break;
-                if (!(ok = mbar_wait(ds_full, i & 1, bound))) break;
+                // One buffer: the scores at once, while dS is formed. Two: behind dK, so that nothing waits for dV alone.
+                if (G::BUFS == 1 && more && !(ok = scores(i + G::BUFS))) break;
+                if (!(ok = mbar_wait(ds_full + 8 * x, phase, bound))) break;
                 fence_after();
-                mma_cols<DPAD>(tmem + DK_COL, tmem + DS_COL, A_HALF, ring(now.at, 0), idesc_o, i > 0, leader);
-                mma_commit(dk_done, leader);
+                mma_cols<DPAD>(tmem + DK_COL, tmem + x * BUF_COLS + DP_COL, 32, ring(now.at, 0), idesc_o, i > 0, leader);
+                mma_commit(dk_done + 8 * x, leader);
                 mma_commit(empty + 8 * now.at, leader);
-                if (!APART && more) ok = dprobs(i + 1);
+                if (G::BUFS > 1 && more && !(ok = scores(i + G::BUFS))) break;
+                if (more) ok = dprobs(i + G::BUFS);
                 now.next();
             }
             mma_commit(acc_full, leader);
@@ -565,19 +579,21 @@ __global__ void __launch_bounds__(kThreads, Geom<DPAD>::CTAS)
         __syncwarp();
     } else {
         // ---------------- elementwise: two threads a state, 32 queries each ----------------
-        const int half = warp >> 2;
+        const int x = warp >> 3, half = (warp >> 2) & 1;  // x: the buffer of this group of warps
         const int64_t j = row0 + 32 * (warp & 3) + lane;
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-        const uint32_t ts = tmem + lanes + S_COL + 32 * half, tdp = tmem + lanes + DP_COL + 32 * half;
-        const uint32_t tp = tmem + lanes + P_COL + A_HALF * half, tds = tmem + lanes + DS_COL + A_HALF * half;
+        const uint32_t ts = tmem + lanes + x * BUF_COLS + 32 * half, tdp = ts + DP_COL;
         int64_t lo = 0, hi = 0;
         if (j < ny && nx > 0) column_cells(a, j, nx, ny, lo, hi);
         const int ilo = static_cast<int>(lo), width = static_cast<int>(hi - lo);
         bool ok = true;
         Turn<G::STAGES> turn;
-        int tile = 0;
-        for (int it = 0; it < n; ++it) {
-            if (!(ok = mbar_wait(full + 8 * turn.at, turn.phase, bound) && mbar_wait(s_full, it & 1, bound))) break;
+        int tile = x;
+        if (x == 1) turn.next();
+        for (int it = x; it < n; it += G::BUFS) {
+            while (tile >= nq) tile -= nq;
+            const uint32_t phase = (it / G::BUFS) & 1;
+            if (!(ok = mbar_wait(full + 8 * turn.at, turn.phase, bound) && mbar_wait(s_full + 8 * x, phase, bound))) break;
             fence_after();
             const float* lse = stats + turn.at * 2 * kCols + 32 * half;
             const float* delta = lse + kCols;
@@ -585,11 +601,6 @@ __global__ void __launch_bounds__(kThreads, Geom<DPAD>::CTAS)
             tmem_ld32(ts, s);
             wait_ld();
             settle(s);
-            if (APART) {
-                fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(s_free);
-            }
             const int off = (ia + tile) * kCols + 32 * half - ilo;
             const bool whole = __all_sync(kFull, off >= 0 && off + 32 <= width);
 #pragma unroll
@@ -608,23 +619,16 @@ __global__ void __launch_bounds__(kThreads, Geom<DPAD>::CTAS)
             uint32_t w[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) w[e] = pack2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]), T());
-            if (APART && it > 0 && !(ok = mbar_wait(dv_done, (it - 1) & 1, bound))) break;
-            fence_after();
-            tmem_st16(tp, w);
+            tmem_st16(ts, w);
             wait_st();
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_full);
-            if (!(ok = mbar_wait(dp_full, it & 1, bound))) break;
+            if (lane == 0) mbar_arrive(p_full + 8 * x);
+            if (!(ok = mbar_wait(dp_full + 8 * x, phase, bound))) break;
             fence_after();
             tmem_ld32(tdp, p);
             wait_ld();
             settle(p);
-            if (APART) {
-                fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(dp_free);
-            }
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
                 const float4 d4 = *reinterpret_cast<const float4*>(delta + 2 * e);
@@ -638,15 +642,13 @@ __global__ void __launch_bounds__(kThreads, Geom<DPAD>::CTAS)
                 w[e] = pack2(v[0], v[1], T());
                 w[e + 1] = pack2(v[2], v[3], T());
             }
-            if (APART && it > 0 && !(ok = mbar_wait(dk_done, (it - 1) & 1, bound))) break;
-            fence_after();
-            tmem_st16(tds, w);
+            tmem_st16(tdp, w);
             wait_st();
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(ds_full);
-            turn.next();
-            if (++tile == nq) tile = 0;
+            if (lane == 0) mbar_arrive(ds_full + 8 * x);
+            for (int y = 0; y < G::BUFS; ++y) turn.next();
+            tile += G::BUFS;
         }
         if (ok && n > 0) ok = mbar_wait(acc_full, 0, bound);
         fence_after();
@@ -654,14 +656,17 @@ __global__ void __launch_bounds__(kThreads, Geom<DPAD>::CTAS)
         const int64_t j0 = row0 + 32 * (warp & 3);
         const int64_t at = ((static_cast<int64_t>(b) * a.M + j0) * a.Hkv + hk) * a.d, pitch = static_cast<int64_t>(a.Hkv) * a.d;
         uint4* rows = reinterpret_cast<uint4*>(sm) + (warp & 3) * 32 * (DPAD / 8);
-        store_rows<T, DPAD>(tmem + lanes + DK_COL, rows, lane, half, 2 + (warp & 3), n > 0 && ok, width > 0, !ok, a.scale / gscale,
-                            f.dn, a.d, static_cast<T*>(a.dk) + at, pitch, a.M - j0);
-        store_rows<T, DPAD>(tmem + lanes + DV_COL, rows + G::ROW_BYTES / 16, lane, half, 2 + (warp & 3), n > 0 && ok, width > 0, !ok,
-                            is_half<T> ? exp2f(-kPShift<T>) : 1.f, f.dn, a.d, static_cast<T*>(a.dv) + at, pitch, a.M - j0);
+        const bool any = n > 0 && ok;
+        if (x == 0)
+            store_rows<T, DPAD>(tmem + lanes + DK_COL, rows, lane, half, 2 + (warp & 3), any, width > 0, !ok, a.scale / gscale, f.dn,
+                                a.d, static_cast<T*>(a.dk) + at, pitch, a.M - j0);
+        if (x == G::BUFS - 1)
+            store_rows<T, DPAD>(tmem + lanes + DV_COL, rows + G::ROW_BYTES / 16, lane, half, 6 + (warp & 3), any, width > 0, !ok,
+                                is_half<T> ? exp2f(-kPShift<T>) : 1.f, f.dn, a.d, static_cast<T*>(a.dv) + at, pitch, a.M - j0);
         fence_before();
     }
     __syncthreads();
-    if (warp == kMmaWarp) {
+    if (warp == G::MMA_WARP) {
         fence_after();
         tmem_free(tmem, TMEM_COLS);
     }
@@ -701,11 +706,11 @@ cudaError_t backward_d(BwdArgs& f, cudaStream_t s)
     if ((e = allow_smem(attend_dq_tc_kernel<T, DPAD>, G::BYTES)) != cudaSuccess) return e;
     if ((e = allow_smem(attend_dkdv_tc_kernel<T, DPAD>, G::BYTES)) != cudaSuccess) return e;
     f.tiles = static_cast<int>((a.N + kTile - 1) / kTile);
-    attend_dq_tc_kernel<T, DPAD><<<static_cast<unsigned>(static_cast<int64_t>(a.B) * a.Hq * f.tiles), kThreads, G::BYTES, s>>>(
+    attend_dq_tc_kernel<T, DPAD><<<static_cast<unsigned>(static_cast<int64_t>(a.B) * a.Hq * f.tiles), G::THREADS, G::BYTES, s>>>(
         q_rows, g_rows, k_cols, v_cols, f);
     count_launch();
     f.tiles = static_cast<int>((a.M + kTile - 1) / kTile);
-    attend_dkdv_tc_kernel<T, DPAD><<<static_cast<unsigned>(static_cast<int64_t>(a.B) * a.Hkv * f.tiles), kThreads, G::BYTES, s>>>(
+    attend_dkdv_tc_kernel<T, DPAD><<<static_cast<unsigned>(static_cast<int64_t>(a.B) * a.Hkv * f.tiles), G::THREADS, G::BYTES, s>>>(
         k_rows, v_rows, q_cols, g_cols, f);
     count_launch();
     return cudaGetLastError();

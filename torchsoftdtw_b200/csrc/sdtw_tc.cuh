@@ -39,37 +39,57 @@ struct Bound {
     uint32_t* err;
 };
 
-// Waits for the phase with the given parity. False when it ran out of time, or another role of the CTA did. The
-// clock is first read after 256 tries (each of which the hardware suspends for a while): waits of a healthy CTA never pay for it.
-__device__ __forceinline__ bool mbar_wait_lane(uint32_t bar, uint32_t parity, const Bound& w)
+// Up to 1024 tries (each of which the hardware suspends for a while). A wait for a phase that is already complete costs 44
+// cycles as a single try, 85 with the vote and this loop behind it, 216 as a loop in C++: the MMA warps make half a dozen a tile.
+__device__ __forceinline__ bool mbar_spin(uint32_t bar, uint32_t parity)
 {
-#pragma unroll 1
-    for (int i = 0; i < 256; ++i)
-        if (mbar_try_wait(bar, parity)) return true;
+    uint32_t ok;
+    asm volatile(
+        "{ .reg .pred p, q; .reg .u32 n; mov.u32 n, 0;\n"
+        "AGAIN_%=: mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "@p bra DONE_%=;\n"
+        "add.u32 n, n, 1; setp.lt.u32 q, n, 1024;\n"
+        "@q bra AGAIN_%=;\n"
+        "DONE_%=: selp.b32 %0, 1, 0, p; }"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
+// A wait that has not ended in mbar_spin: goes on until the phase completes, the time runs out or another role gives up.
+static __device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, Bound w)
+{
     const uint64_t t0 = global_ns();
+    bool mine = false;
     while (true) {
 #pragma unroll 1
-        for (int i = 0; i < 64; ++i)
-            if (mbar_try_wait(bar, parity)) return true;
-        if (*w.abort) return false;
-        if (global_ns() - t0 > w.timeout_ns) {
-            *w.abort = 1;
-            atomicOr(w.err, kErrTimeout);
+        for (int i = 0; i < 64 && !mine; ++i) mine = mbar_try_wait(bar, parity);
+        __syncwarp();
+        if (__all_sync(kFull, mine)) return true;
+        const bool late = global_ns() - t0 > w.timeout_ns;
+        if (__any_sync(kFull, late || *w.abort)) {
+            if ((threadIdx.x & 31) == 0 && !*w.abort) {
+                *w.abort = 1;
+                atomicOr(w.err, kErrTimeout);
+            }
             return false;
         }
     }
 }
-// The same by a whole warp, with one answer for all its lanes.
+
+// Waits, as a whole warp, for the phase with the given parity. False, for all its lanes, when it ran out of time, or
+// another role of the CTA did.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const Bound& w)
 {
-    return __all_sync(kFull, mbar_wait_lane(bar, parity, w));
+    if (__all_sync(kFull, mbar_try_wait(bar, parity))) return true;
+    if (__all_sync(kFull, mbar_spin(bar, parity))) return true;
+    return mbar_wait_long(bar, parity, w);
 }
 // The same wait for one's own operations in flight, which goes on after an abort.
 __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity, uint64_t timeout_ns)
 {
-#pragma unroll 1
-    for (int i = 0; i < 256; ++i)
-        if (mbar_try_wait(bar, parity)) return;
+    if (mbar_spin(bar, parity)) return;
     const uint64_t t0 = global_ns();
     while (!mbar_try_wait(bar, parity) && global_ns() - t0 <= timeout_ns) {
     }
