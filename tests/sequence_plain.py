@@ -133,7 +133,10 @@ def norm_rotate(x, weight, lengths, positions, rotary, base, interleaved, eps, d
     y = torch.where(keep, turn(Z), 0.0)
     # An angle is a position times a frequency whose power and quotient by 2 pi are rounded to 64 bits, and so is the
     # product: three relative errors of 2^-53; the plain angle above carries two.
-    turn_err = 2 * 2**-22 + 5 * 2.0**-53 * angle.abs().unsqueeze(2)
+    # 16-bit results take cos and sin from __sincosf, off by at most 2^-21.19 (CUDA's bound on [-pi, pi]), of an angle
+    # rounded thrice more.
+    hw = 2.0**-20 if x.dtype != torch.float32 else 0.0
+    turn_err = 2 * 2**-22 + hw + 5 * 2.0**-53 * angle.abs().unsqueeze(2)
     y_err = (rel + turn_err) * (Z.abs() + Z[..., partner].abs()) * keep
     vals, errs = {"y": y}, {"y": y_err + u * (y.abs() + y_err)}
     if dy is None:

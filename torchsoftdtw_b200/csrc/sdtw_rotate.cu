@@ -6,10 +6,10 @@
 //
 // Bound by memory: x in and y out; x and dy in, dx out. A head (d features) belongs to a group of G lanes, a
 // lane to V neighbouring pairs (two vectors of V features), so the mean is log2 G shuffles and a pair never
-// leaves its lane. A group takes one token and walks `hpu` of its heads: the angles (64-bit products, so that
-// far positions keep theirs; then one sincospi a pair) are formed once for them. dw: every lane adds the products of its
-// own features over all its tokens in 32 bits, the CTA joins its groups, a second launch joins the CTAs, each
-// in a fixed order.
+// leaves its lane. A unit of work is `hpu` heads of one token, whose angles are formed once (64-bit products, so that far
+// positions keep theirs); units go round the groups, so that the GPU sweeps memory in order, and a group loads U heads ahead
+// of their arithmetic. dw: every lane adds the products of its own features over its run in 32 bits,
+// the CTA joins its groups, a second launch joins the CTAs, each in a fixed order.
 #include <cmath>
 #include <mutex>
 
@@ -20,7 +20,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxPairs = 128;  // d <= 256
-constexpr int kCtasPerSm = 4;
 constexpr int kMaxGradCtas = 1024;
 
 struct RotArgs {
@@ -38,7 +37,7 @@ struct RotArgs {
     uint32_t* err;
     int64_t tokens, N;
     int H, d, rotary, interleaved;
-    int hpu, units_per_token;  // heads per unit of work
+    int hpu, token_units;  // heads a unit, units a token
     float eps;
     float* dw;           // (grid, d) partial sums
     double turns[kMaxPairs];  // turns per position of pair p: base^(-2p / rotary) / (2 pi)
@@ -61,14 +60,16 @@ __device__ __forceinline__ float group_sum(float v)
     return v;
 }
 
-// Features of pair group `pg` (V pairs from p0 = pg V): the offsets of its two vectors, and whether it turns.
-// The host only chooses V > 1 when V divides rotary / 2 and 2 V divides d, so a group is all of one kind.
-template <int V>
+// Features of pair group `pg` (V pairs from p0 = pg V): where its two vectors of V features begin, and whether it turns.
+// The host only chooses V > 1 when V divides rotary / 2 and 2 V divides d, so a group is all of one kind. Pairs that turn are
+// the two vectors' features side by side in the split layout (`apart`); in the interleaved one, and for features that
+// stay, the two vectors are 2V neighbours and a pair is two of those.
+template <int V, bool SPLIT>
 __device__ __forceinline__ void pair_offsets(const RotArgs& a, int pg, int& oa, int& ob, bool& turned)
 {
     const int p0 = pg * V, half = a.rotary / 2;
     turned = p0 < half;
-    if (turned && !a.interleaved) {
+    if (SPLIT && turned) {
         oa = p0;
         ob = p0 + half;
     } else {
@@ -76,184 +77,282 @@ __device__ __forceinline__ void pair_offsets(const RotArgs& a, int pg, int& oa, 
         ob = 2 * p0 + V;
     }
 }
-
-// The 2V features of a lane: both vectors, the second from V on.
-template <typename T, int V>
-__device__ __forceinline__ void load_pairs(const T* row, int oa, int ob, int d, float (&f)[2 * V])
+// Place of the first (second) feature of pair i of a group among its 2V features, the second vector from V on.
+template <int V, bool SPLIT>
+__device__ __forceinline__ constexpr int place(int i, bool second)
 {
-    if constexpr (V == 1) {
-        f[0] = oa < d ? to_f(row[oa]) : 0.f;
-        f[1] = ob < d ? to_f(row[ob]) : 0.f;
-    } else {
-        const Vec<T, V> va = *reinterpret_cast<const Vec<T, V>*>(row + oa);
-        const Vec<T, V> vb = *reinterpret_cast<const Vec<T, V>*>(row + ob);
+    return SPLIT ? (second ? V + i : i) : 2 * i + (second ? 1 : 0);
+}
+
+// Two numbers in one instruction.
+struct F2 {
+    float x, y;
+};
+__device__ __forceinline__ uint64_t bits(F2 a)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+    return r;
+}
+__device__ __forceinline__ F2 both(uint64_t r)
+{
+    F2 a;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(r));
+    return a;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b)
+{
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+    return both(r);
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+    return both(r);
+}
+__device__ __forceinline__ F2 twice(float a) { return {a, a}; }
+__device__ __forceinline__ F2 minus(F2 a) { return {-a.x, -a.y}; }
+
+// The features of one head that a lane holds, as they lie in memory: K groups of two vectors.
+template <typename T, int V, int K>
+struct Raw {
+    Vec<T, V> v[K][2];
+};
+
+template <typename T, int V, int K>
+__device__ __forceinline__ void load_raw(Raw<T, V, K>& r, const T* row, const int (&oa)[K], const int (&ob)[K], const bool (&live)[K],
+                                         int d, bool on)
+{
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            f[i] = to_f(va.e[i]);
-            f[V + i] = to_f(vb.e[i]);
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) r.v[k][0].e[i] = r.v[k][1].e[i] = from_f<T>(0.f);
+        if (on && live[k]) {
+            if constexpr (V == 1) {
+                if (oa[k] < d) r.v[k][0].e[0] = row[oa[k]];
+                if (ob[k] < d) r.v[k][1].e[0] = row[ob[k]];
+            } else {
+                r.v[k][0] = *reinterpret_cast<const Vec<T, V>*>(row + oa[k]);
+                r.v[k][1] = *reinterpret_cast<const Vec<T, V>*>(row + ob[k]);
+            }
         }
     }
 }
-
-template <typename T, int V>
-__device__ __forceinline__ void store_pairs(T* row, int oa, int ob, int d, const float (&f)[2 * V])
-{
-    if constexpr (V == 1) {
-        if (oa < d) row[oa] = from_f<T>(f[0]);
-        if (ob < d) row[ob] = from_f<T>(f[1]);
-    } else {
-        Vec<T, V> va, vb;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            va.e[i] = from_f<T>(f[i]);
-            vb.e[i] = from_f<T>(f[V + i]);
-        }
-        *reinterpret_cast<Vec<T, V>*>(row + oa) = va;
-        *reinterpret_cast<Vec<T, V>*>(row + ob) = vb;
-    }
-}
-
-// Turn the V pairs by (c, s); sign -1 turns back.
-template <int V>
-__device__ __forceinline__ void turn(float (&f)[2 * V], const float (&c)[V], const float (&s)[V], bool split,
-                                     float sign)
+template <typename T, int V, int K>
+__device__ __forceinline__ void store_raw(const Raw<T, V, K>& r, T* row, const int (&oa)[K], const int (&ob)[K], const bool (&live)[K],
+                                          int d, bool on)
 {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const float sn = sign * s[i];
-        if (split) {
-            const float p = f[i], q = f[V + i];
-            f[i] = p * c[i] - q * sn;
-            f[V + i] = p * sn + q * c[i];
+    for (int k = 0; k < K; ++k) {
+        if (!on || !live[k]) continue;
+        if constexpr (V == 1) {
+            if (oa[k] < d) row[oa[k]] = r.v[k][0].e[0];
+            if (ob[k] < d) row[ob[k]] = r.v[k][1].e[0];
         } else {
-            const float p = f[2 * i], q = f[2 * i + 1];
-            f[2 * i] = p * c[i] - q * sn;
-            f[2 * i + 1] = p * sn + q * c[i];
+            *reinterpret_cast<Vec<T, V>*>(row + oa[k]) = r.v[k][0];
+            *reinterpret_cast<Vec<T, V>*>(row + ob[k]) = r.v[k][1];
         }
     }
+}
+
+// A lane's pairs, two by two: the firsts in p, the seconds in q (NP = pairs a lane, even).
+template <typename T, int V, int K, bool SPLIT>
+__device__ __forceinline__ void unpack(const Raw<T, V, K>& r, F2 (&p)[V * K / 2], F2 (&q)[V * K / 2])
+{
+    const auto at = [&](int pair, bool second) {
+        const int k = pair / V, o = place<V, SPLIT>(pair % V, second);
+        return to_f(o < V ? r.v[k][0].e[o] : r.v[k][1].e[o - V]);
+    };
+#pragma unroll
+    for (int i = 0; i < V * K / 2; ++i) {
+        p[i] = {at(2 * i, false), at(2 * i + 1, false)};
+        q[i] = {at(2 * i, true), at(2 * i + 1, true)};
+    }
+}
+template <typename T, int V, int K, bool SPLIT>
+__device__ __forceinline__ void repack(Raw<T, V, K>& r, const F2 (&p)[V * K / 2], const F2 (&q)[V * K / 2])
+{
+    const auto put = [&](int pair, bool second, float x) {
+        const int k = pair / V, o = place<V, SPLIT>(pair % V, second);
+        (o < V ? r.v[k][0].e[o] : r.v[k][1].e[o - V]) = from_f<T>(x);
+    };
+#pragma unroll
+    for (int i = 0; i < V * K / 2; ++i) {
+        put(2 * i, false, p[i].x);
+        put(2 * i + 1, false, p[i].y);
+        put(2 * i, true, q[i].x);
+        put(2 * i + 1, true, q[i].y);
+    }
+}
+
+// How many heads a lane has in flight, and how many CTAs of an SM the registers that this takes leave room for.
+template <int V, bool GRAD>
+constexpr int kAhead = V == 1 ? 1 : (GRAD ? 1 : 2);
+template <int V, bool GRAD>
+constexpr int kCtasPerSm = V == 8 && GRAD ? 2 : 3;
+
+// cos and sin of `turns` whole turns, |turns| <= 1/2. 16-bit results: the hardware's functions, off by at most 2^-21 on
+// [-pi, pi], far below half a step.
+template <typename T>
+__device__ __forceinline__ void cos_sin(float turns, float& c, float& s)
+{
+    if constexpr (sizeof(T) == 2)
+        __sincosf(turns * 6.283185307179586f, &s, &c);
+    else
+        sincospif(2.f * turns, &s, &c);
 }
 
 // K pair groups a lane (1, or 4 with V = 1 and G = 32: any d up to 256, odd or unaligned).
-template <typename T, int V, int G, int K, bool GRAD>
-__global__ void __launch_bounds__(kThreads) norm_rotate_kernel(const __grid_constant__ RotArgs a)
+template <typename T, int V, int G, int K, bool SPLIT, bool GRAD>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm<V, GRAD>) norm_rotate_kernel(const __grid_constant__ RotArgs a)
 {
     constexpr int kGroups = kThreads / G;
+    constexpr int U = kAhead<V, GRAD>;
+    constexpr int NP = V * K / 2;  // twos of pairs
     __shared__ float red[GRAD ? kGroups * G * K * 2 * V : 1];
     const int gl = threadIdx.x % G, group = threadIdx.x / G;
     const int pair_groups = (a.d + 2 * V - 1) / (2 * V);
     int oa[K], ob[K];
     bool turned[K], live[K];
-    float w[K][2 * V], dw[K][2 * V];
+    F2 wp[NP], wq[NP], dwp[NP], dwq[NP];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const int pg = gl + k * G;
-        live[k] = pg < pair_groups;
-        pair_offsets<V>(a, live[k] ? pg : 0, oa[k], ob[k], turned[k]);
+        live[k] = gl + k * G < pair_groups;
+        pair_offsets<V, SPLIT>(a, live[k] ? gl + k * G : 0, oa[k], ob[k], turned[k]);
+        turned[k] = turned[k] && live[k];
+    }
+    // Vector o of group k holds feature (o < V ? oa : ob - V) + o.
+    const auto feature = [&](int pair, bool second) {
+        const int o = place<V, SPLIT>(pair % V, second);
+        return (o < V ? oa[pair / V] : ob[pair / V] - V) + o;
+    };
+    const auto weight_at = [&](int pair, bool second) {
+        const int o = feature(pair, second);
+        if (a.weight == nullptr || !live[pair / V] || o >= a.d) return 1.f;
+        return a.weight_f32 ? static_cast<const float*>(a.weight)[o] : to_f(static_cast<const T*>(a.weight)[o]);
+    };
 #pragma unroll
-        for (int i = 0; i < 2 * V; ++i) {
-            const int o = i < V ? oa[k] + i : ob[k] + i - V;
-            dw[k][i] = 0.f;
-            w[k][i] = 1.f;
-            if (a.weight != nullptr && live[k] && o < a.d)
-                w[k][i] = a.weight_f32 ? static_cast<const float*>(a.weight)[o] : to_f(static_cast<const T*>(a.weight)[o]);
-        }
+    for (int i = 0; i < NP; ++i) {
+        wp[i] = {weight_at(2 * i, false), weight_at(2 * i + 1, false)};
+        wq[i] = {weight_at(2 * i, true), weight_at(2 * i + 1, true)};
+        dwp[i] = dwq[i] = {0.f, 0.f};
     }
     const float inv_d = 1.f / static_cast<float>(a.d);
-    const bool split = !a.interleaved;
-    const int64_t units = a.tokens * a.units_per_token;
+    const int64_t units = a.tokens * a.token_units, stride = static_cast<int64_t>(gridDim.x) * kGroups;
     // Every lane of a warp makes the same number of rounds (the shuffles need them all).
-    const int64_t stride = static_cast<int64_t>(gridDim.x) * kGroups;
     for (int64_t u0 = static_cast<int64_t>(blockIdx.x) * kGroups; u0 < units; u0 += stride) {
-        const int64_t u = u0 + group;
-        const bool on = u < units;
-        const int64_t token = on ? u / a.units_per_token : 0;
-        const int h0 = on ? static_cast<int>(u - token * a.units_per_token) * a.hpu : 0;
-        const int64_t b = token / a.N, n = token - b * a.N;
+        const bool on = u0 + group < units;
+        const unsigned unit = static_cast<unsigned>(on ? u0 + group : 0);  // fewer than 2^31, as the host checks
+        const unsigned token = unit / static_cast<unsigned>(a.token_units), b = token / static_cast<unsigned>(a.N);
+        const int64_t n = token - b * static_cast<unsigned>(a.N);
+        const int first = static_cast<int>(unit - token * static_cast<unsigned>(a.token_units)) * a.hpu;
+        const int last = on ? min(first + a.hpu, a.H) : first;
         const int64_t len = a.len.get(b, a.N);
         if (on && len < 0 && gl == 0) atomicOr(a.err, kErrBadLength);
-        const bool valid = on && n < len;
-        float c[K][V], s[K][V];
-        const double pos = valid ? position(a, b, n) : 0.0;
+        const bool work = on && n < len;
+        const T* xr = static_cast<const T*>(a.x) + static_cast<int64_t>(b) * a.sb + n * a.sn + first * a.sh;
+        const T* gr = GRAD ? static_cast<const T*>(a.dy) + static_cast<int64_t>(b) * a.gb + n * a.gn + first * a.gh : nullptr;
+        T* yr = static_cast<T*>(a.y) + (static_cast<int64_t>(token) * a.H + first) * a.d;
+        F2 c[NP], s[NP];
+        bool fresh = true;
+        for (int h0 = first; h0 < first + a.hpu; h0 += U) {
+            Raw<T, V, K> rx[U], rg[GRAD ? U : 1];
 #pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                c[k][i] = 1.f;
-                s[k][i] = 0.f;
-                if (live[k] && turned[k]) {
-                    const double t = pos * a.turns[(gl + k * G) * V + i];
-                    const float f = static_cast<float>(t - rint(t));  // turns beyond whole ones, in [-1/2, 1/2]
-                    sincospif(2.f * f, &s[k][i], &c[k][i]);
-                }
-            }
-        const float fill = on && len < 0 && !GRAD ? __int_as_float(0x7fc00000) : 0.f;
-        for (int hh = 0; hh < a.hpu; ++hh) {
-            const int h = h0 + hh;
-            const bool head = on && h < a.H, work = valid && h < a.H;
-            float f[K][2 * V], g[K][2 * V];
-            float ss = 0.f, dot = 0.f;
-            const T* xr = static_cast<const T*>(a.x) + b * a.sb + n * a.sn + h * a.sh;
-            const T* gr = GRAD ? static_cast<const T*>(a.dy) + b * a.gb + n * a.gn + h * a.gh : nullptr;
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-#pragma unroll
-                for (int i = 0; i < 2 * V; ++i) f[k][i] = g[k][i] = 0.f;
-                if (work && live[k]) {
-                    load_pairs<T, V>(xr, oa[k], ob[k], a.d, f[k]);
-                    if constexpr (GRAD) load_pairs<T, V>(gr, oa[k], ob[k], a.d, g[k]);
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
+            for (int u = 0; u < U; ++u) {
+                load_raw<T, V, K>(rx[u], xr, oa, ob, live, a.d, work && h0 + u < last);
+                xr += a.sh;
                 if constexpr (GRAD) {
-                    if (turned[k]) turn<V>(g[k], c[k], s[k], split, -1.f);
-                }
-#pragma unroll
-                for (int i = 0; i < 2 * V; ++i) {
-                    ss = fmaf(f[k][i], f[k][i], ss);
-                    if constexpr (GRAD) dot = fmaf(g[k][i] * w[k][i], f[k][i], dot);
+                    load_raw<T, V, K>(rg[u], gr, oa, ob, live, a.d, work && h0 + u < last);
+                    gr += a.gh;
                 }
             }
-            ss = group_sum<G>(ss);
-            if constexpr (GRAD) dot = group_sum<G>(dot);
-            const float r = rsqrtf(ss * inv_d + a.eps);
-            const float back = GRAD ? dot * inv_d * r * r : 0.f;
-            T* yr = static_cast<T*>(a.y) + (token * a.H + h) * a.d;
+            if (fresh) {  // the angles, once a unit, behind its first loads
+                const double pos = work ? position(a, b, n) : 0.0;
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                if constexpr (GRAD) {
-#pragma unroll
-                    for (int i = 0; i < 2 * V; ++i) {
-                        if (work) dw[k][i] = fmaf(g[k][i], f[k][i] * r, dw[k][i]);
-                        g[k][i] = work ? r * (g[k][i] * w[k][i] - f[k][i] * back) : 0.f;
+                for (int i = 0; i < 2 * NP; ++i) {
+                    float ci = 1.f, si = 0.f;
+                    if (turned[i / V]) {
+                        const double t = pos * a.turns[(gl + i / V * G) * V + i % V];
+                        cos_sin<T>(static_cast<float>(t - rint(t)), ci, si);  // turns beyond whole ones, in [-1/2, 1/2]
                     }
-                    if (head && live[k]) store_pairs<T, V>(yr, oa[k], ob[k], a.d, g[k]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 2 * V; ++i) f[k][i] = work ? f[k][i] * r * w[k][i] : fill;
-                    if (work && turned[k]) turn<V>(f[k], c[k], s[k], split, 1.f);
-                    if (head && live[k]) store_pairs<T, V>(yr, oa[k], ob[k], a.d, f[k]);
+                    (i & 1 ? c[i / 2].y : c[i / 2].x) = ci;
+                    (i & 1 ? s[i / 2].y : s[i / 2].x) = si;
                 }
+                fresh = false;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                F2 p[NP], q[NP], ss2 = {0.f, 0.f};
+                unpack<T, V, K, SPLIT>(rx[u], p, q);
+#pragma unroll
+                for (int i = 0; i < NP; ++i) ss2 = fma2(q[i], q[i], fma2(p[i], p[i], ss2));
+                const float ss = group_sum<G>(ss2.x + ss2.y);
+                // Rows that are not worked on were read as zeros and stay so; those of a bad sample become NaN.
+                const float r = work ? rsqrtf(fmaf(ss, inv_d, a.eps)) : (len < 0 && !GRAD ? __int_as_float(0x7fc00000) : 0.f);
+                Raw<T, V, K> ry;
+                if constexpr (GRAD) {
+                    F2 g[NP], e[NP], dot2 = {0.f, 0.f};
+                    unpack<T, V, K, SPLIT>(rg[u], g, e);
+#pragma unroll
+                    for (int i = 0; i < NP; ++i) {  // turned back
+                        const F2 y0 = g[i], y1 = e[i];
+                        g[i] = fma2(y1, s[i], y0 * c[i]);
+                        e[i] = fma2(minus(y0), s[i], y1 * c[i]);
+                    }
+                    F2 gp[NP], gq[NP];
+#pragma unroll
+                    for (int i = 0; i < NP; ++i) {
+                        gp[i] = g[i] * p[i];
+                        gq[i] = e[i] * q[i];
+                        dot2 = fma2(gq[i], wq[i], fma2(gp[i], wp[i], dot2));
+                    }
+                    const float dot = group_sum<G>(dot2.x + dot2.y);
+                    const F2 back = twice(-dot * inv_d * r * r * r), r2 = twice(r);
+#pragma unroll
+                    for (int i = 0; i < NP; ++i) {
+                        dwp[i] = fma2(gp[i], r2, dwp[i]);
+                        dwq[i] = fma2(gq[i], r2, dwq[i]);
+                        p[i] = fma2(g[i] * wp[i], r2, p[i] * back);
+                        q[i] = fma2(e[i] * wq[i], r2, q[i] * back);
+                    }
+                } else {
+                    const F2 r2 = twice(r);
+#pragma unroll
+                    for (int i = 0; i < NP; ++i) {
+                        const F2 z0 = p[i] * r2 * wp[i], z1 = q[i] * r2 * wq[i];
+                        p[i] = fma2(minus(z1), s[i], z0 * c[i]);
+                        q[i] = fma2(z0, s[i], z1 * c[i]);
+                    }
+                }
+                repack<T, V, K, SPLIT>(ry, p, q);
+                store_raw<T, V, K>(ry, yr, oa, ob, live, a.d, h0 + u < last);
+                yr += a.d;
             }
         }
     }
     if constexpr (GRAD) {
         if (a.dw == nullptr) return;
-        // red[group][lane][k][i]; then the features' sums over the groups, in order.
+        // red[group][lane][pair][first, second]; then the features' sums over the groups, in order.
         float* mine = red + (group * G + gl) * (K * 2 * V);
 #pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int i = 0; i < 2 * V; ++i) mine[k * 2 * V + i] = dw[k][i];
+        for (int i = 0; i < NP; ++i) {
+            mine[4 * i] = dwp[i].x;
+            mine[4 * i + 1] = dwq[i].x;
+            mine[4 * i + 2] = dwp[i].y;
+            mine[4 * i + 3] = dwq[i].y;
+        }
         __syncthreads();
         for (int e = threadIdx.x; e < G * K * 2 * V; e += kThreads) {
-            const int lane = e / (K * 2 * V), k = (e / (2 * V)) % K, i = e % (2 * V);
-            const int pg = lane + k * G;
+            const int lane = e / (K * 2 * V), pair = e / 2 % (K * V), pg = lane + pair / V * G;
             if (pg >= pair_groups) continue;
             int fa, fb;
             bool tn;
-            pair_offsets<V>(a, pg, fa, fb, tn);
-            const int o = i < V ? fa + i : fb + i - V;
+            pair_offsets<V, SPLIT>(a, pg, fa, fb, tn);
+            const int at = place<V, SPLIT>(pair % V, e & 1);
+            const int o = at < V ? fa + at : fb + at - V;
             if (o >= a.d) continue;
             float t = 0.f;
             for (int gidx = 0; gidx < kGroups; ++gidx) t += red[gidx * (G * K * 2 * V) + e];
@@ -278,22 +377,24 @@ __global__ void __launch_bounds__(kThreads) join_dweight_kernel(const float* par
 template <typename T, int V, int G, int K, bool GRAD>
 void launch(const RotArgs& a, int grid, cudaStream_t s)
 {
-    norm_rotate_kernel<T, V, G, K, GRAD><<<grid, kThreads, 0, s>>>(a);
+    if (a.interleaved)
+        norm_rotate_kernel<T, V, G, K, false, GRAD><<<grid, kThreads, 0, s>>>(a);
+    else
+        norm_rotate_kernel<T, V, G, K, true, GRAD><<<grid, kThreads, 0, s>>>(a);
     count_launch();
 }
 
 template <typename T, int V, bool GRAD>
-bool launch_v(const RotArgs& a, int G, int grid, cudaStream_t s)
+void launch_v(const RotArgs& a, int G, int grid, cudaStream_t s)
 {
     switch (G) {
-        case 1: launch<T, V, 1, 1, GRAD>(a, grid, s); return true;
-        case 2: launch<T, V, 2, 1, GRAD>(a, grid, s); return true;
-        case 4: launch<T, V, 4, 1, GRAD>(a, grid, s); return true;
-        case 8: launch<T, V, 8, 1, GRAD>(a, grid, s); return true;
-        case 16: launch<T, V, 16, 1, GRAD>(a, grid, s); return true;
-        case 32: launch<T, V, 32, 1, GRAD>(a, grid, s); return true;
+        case 1: launch<T, V, 1, 1, GRAD>(a, grid, s); break;
+        case 2: launch<T, V, 2, 1, GRAD>(a, grid, s); break;
+        case 4: launch<T, V, 4, 1, GRAD>(a, grid, s); break;
+        case 8: launch<T, V, 8, 1, GRAD>(a, grid, s); break;
+        case 16: launch<T, V, 16, 1, GRAD>(a, grid, s); break;
+        default: launch<T, V, 32, 1, GRAD>(a, grid, s); break;
     }
-    return false;
 }
 
 // Turns per position of each pair, kept for the last (base, rotary) of the thread: 128 pow calls cost more
@@ -334,16 +435,17 @@ sdtw_status run(RotArgs& a, void* dweight, cudaStream_t s)
     int G = 32;
     if (V > 1)
         for (G = 1; G * 2 * V < a.d;) G *= 2;
-    // Heads a unit: all of a token's, so that they share its angles, unless that leaves lanes of the GPU idle.
+    // A unit is a token, unless that leaves the groups with few and unequal shares of them: then parts of one.
+    const int64_t groups = static_cast<int64_t>(sms) * kCtasPerSm<kWide, GRAD> * (kThreads / G);
     a.hpu = a.H;
-    const int64_t groups = static_cast<int64_t>(sms) * kCtasPerSm * (kThreads / G);
-    while (a.hpu > 1 && a.tokens * ((a.H + a.hpu - 1) / a.hpu) < 2 * groups) a.hpu = (a.hpu + 1) / 2;
-    a.units_per_token = (a.H + a.hpu - 1) / a.hpu;
-    const int64_t units = a.tokens * a.units_per_token;
-    const int64_t need = (units + kThreads / G - 1) / (kThreads / G);
-    int64_t grid = sms * static_cast<int64_t>(kCtasPerSm);
+    while (a.hpu > 2 && a.tokens * ((a.H + a.hpu - 1) / a.hpu) < 8 * groups) a.hpu = (a.hpu + 3) / 4 * 2;
+    if (a.tokens * a.H < groups) a.hpu = 1;
+    a.token_units = (a.H + a.hpu - 1) / a.hpu;
+    const int64_t units = a.tokens * a.token_units;
+    if (units >= (int64_t{1} << 31)) return SDTW_EINVAL;
+    int64_t grid = (units + kThreads / G - 1) / (kThreads / G);
+    if (grid > sms * kCtasPerSm<kWide, GRAD>) grid = sms * kCtasPerSm<kWide, GRAD>;
     if (grid > kMaxGradCtas) grid = kMaxGradCtas;
-    if (grid > need) grid = need;
     if (V == 1)
         launch<T, 1, 32, 4, GRAD>(a, static_cast<int>(grid), s);
     else if (V == 4)
