@@ -4,8 +4,9 @@
 // Bound by memory: one read for the norm, one read and one write for the scaling (no read or write where the
 // factor is one and the tensors are scaled in place). Two launches: the first leaves one partial result per
 // CTA, the second combines the partials in every CTA (in one fixed order, so each run and each CTA gets the
-// same bits) and scales. Tensors are cut into chunks of kChunkElems entries; CTA c takes chunks c, c + grid,
-// and the second launch walks them backwards, so that what the first one read last is still in L2.
+// same bits) and scales. Tensors are cut into chunks of 64 KB, or less where there would be fewer than four chunks a
+// CTA; CTA c takes chunks c, c + grid, and the second launch walks them backwards, so that what the first one read last is
+// still in L2.
 #include <cmath>
 #include <cstring>
 
@@ -15,7 +16,7 @@ namespace sdtw {
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kChunkElems = 32768;
+constexpr int kMinChunk = 8192, kMaxChunk = 65536;  // bytes
 constexpr int kCtasPerSm = 3;
 constexpr int kMaxCtas = 1024;       // partial results per launch
 constexpr int kSmallCap = 64;        // tensors per launch: the table is a kernel argument (32 KB at most)
@@ -37,7 +38,13 @@ struct Table {
     int32_t chunks;
     int32_t wide;  // some tensor is float64: every square is formed in 64 bits, its range extended
     int32_t kind;  // 0: Euclidean, 1: largest magnitude
+    int32_t chunk_bytes;
 };
+
+__host__ __device__ __forceinline__ int chunk_entries(int bytes, int dtype)
+{
+    return bytes >> (dtype == SDTW_F64 ? 3 : (dtype == SDTW_F32 ? 2 : 1));
+}
 
 template <int CAP>
 __device__ __forceinline__ int find_entry(const Table<CAP>& t, int chunk)
@@ -193,8 +200,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) clip_partials_kernel(con
     unsigned long long top = 0;
     for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
         const Entry& e = t.e[find_entry(t, c)];
-        const int64_t at = static_cast<int64_t>(c - e.first_chunk) * kChunkElems;
-        const int n = static_cast<int>(min(static_cast<int64_t>(kChunkElems), e.n - at));
+        const int chunk = chunk_entries(t.chunk_bytes, e.dtype);
+        const int64_t at = static_cast<int64_t>(c - e.first_chunk) * chunk;
+        const int n = static_cast<int>(min(static_cast<int64_t>(chunk), e.n - at));
         const bool wide = t.wide != 0;
         if (t.kind == 0) {
             switch (e.dtype) {
@@ -307,8 +315,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) clip_scale_kernel(const 
     for (int c = t.chunks - 1 - static_cast<int>(blockIdx.x); c >= 0; c -= static_cast<int>(gridDim.x)) {
         const Entry& e = t.e[find_entry(t, c)];
         if (coef == 1.0 && e.src == e.dst) continue;
-        const int64_t at = static_cast<int64_t>(c - e.first_chunk) * kChunkElems;
-        const int n = static_cast<int>(min(static_cast<int64_t>(kChunkElems), e.n - at));
+        const int chunk = chunk_entries(t.chunk_bytes, e.dtype);
+        const int64_t at = static_cast<int64_t>(c - e.first_chunk) * chunk;
+        const int n = static_cast<int>(min(static_cast<int64_t>(chunk), e.n - at));
         switch (e.dtype) {
             case SDTW_F32:
                 scale_chunk(static_cast<const float*>(e.src) + at, static_cast<float*>(e.dst) + at, n, coef);
@@ -337,6 +346,10 @@ sdtw_status clip_run(const sdtw_tensor_ref* refs, int64_t count, int kind, bool 
     Table<CAP> t;
     t.wide = wide;
     t.kind = kind;
+    int64_t bytes = 0;
+    for (int64_t i = 0; i < count; ++i) bytes += refs[i].numel * static_cast<int64_t>(dtype_size(refs[i].dtype));
+    t.chunk_bytes = kMaxChunk;
+    while (t.chunk_bytes > kMinChunk && bytes / t.chunk_bytes < 4 * sms * kCtasPerSm) t.chunk_bytes /= 2;
     int64_t at = 0;
     auto fill = [&]() -> sdtw_status {
         t.count = 0;
@@ -344,7 +357,7 @@ sdtw_status clip_run(const sdtw_tensor_ref* refs, int64_t count, int kind, bool 
         for (; at < count && t.count < CAP; ++at) {
             const int64_t n = refs[at].numel;
             if (n == 0) continue;
-            const int64_t chunks = (n + kChunkElems - 1) / kChunkElems;
+            const int64_t chunk = chunk_entries(t.chunk_bytes, refs[at].dtype), chunks = (n + chunk - 1) / chunk;
             if (chunks > (1 << 28) || t.chunks > (1 << 28)) return SDTW_EINVAL;
             t.e[t.count++] = {refs[at].src, refs[at].dst, n, t.chunks, refs[at].dtype};
             t.chunks += static_cast<int32_t>(chunks);
