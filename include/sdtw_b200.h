@@ -288,6 +288,7 @@ sdtw_status sdtw_grad_dist(sdtw_dtype dtype, int kind, const void* X, const void
  *   A length outside [0, N] / [0, M] raises SDTW_ERR_BAD_LENGTH; that sample's rows are NaN, its gradients 0.
  *   backward: dout (B, N, Hq, d) with any strides; dq, dk, dv contiguous, each written in full, in one fixed
  *   order of sums (no atomics). out and lse are the forward's for the same problem.
+ *   Every output starts on 16 bytes (SDTW_EINVAL otherwise), and so do out and out_lo where the backward reads them.
  * workspace: *_workspace_bytes(problem) bytes, 256-byte aligned, any content; one call at a time.
  * ------------------------------------------------------------------------------------------------- */
 typedef struct {

@@ -34,6 +34,10 @@ SHAPES = [
     (2, 1000, 300, 2, 2, 32, 5),
     (1, 257, 1025, 3, 1, 72, 64),
     (3, 100, 90, 2, 2, 8, 0),
+    (1, 40, 5000, 2, 1, 64, -1),
+    (2, 30, 4001, 2, 2, 128, 100),
+    (1, 600, 700, 1, 1, 128, -1),
+    (1, 700, 600, 2, 1, 64, 40),
 ]
 
 
@@ -121,6 +125,61 @@ def test_strides(cuda, dtype, layout):
         t = [rnd(B, n, d, H).transpose(2, 3) for n in (N, M, M, N)]
     lx, ly = torch.tensor([N, N - 37]), torch.tensor([M - 3, M])
     compare(t, lx, ly, bw, run(t, lx, ly, bw))
+
+
+def test_many_samples(cuda):
+    """More samples and heads than one dimension of a grid may hold."""
+    B, N, M, H, d = 20000, 2, 3, 4, 16
+    q, k, v = (torch.randn(B, n, H, d, device=cuda, dtype=torch.bfloat16).requires_grad_(True) for n in (N, M, M))
+    out = T.cross_attention(q, k, v)
+    grads = torch.autograd.grad(out, (q, k, v), torch.ones_like(out))
+    for b in (0, 9999, B - 1):
+        vals, errs = plain.attention(q[b:b + 1].detach(), k[b:b + 1].detach(), v[b:b + 1].detach(), torch.tensor([N]),
+                                     torch.tensor([M]), -1, 0.25, torch.ones_like(out[b:b + 1]))
+        for name, got in zip(("out", "dq", "dk", "dv"), (out, *grads)):
+            plain.check(name, got[b:b + 1].detach(), vals[name], errs[name])
+
+
+def test_one_tensor_in_all_places(cuda):
+    """Self attention: the gradients of the three uses add up."""
+    x = torch.randn(2, 150, 2, 64, device=cuda, dtype=torch.bfloat16).requires_grad_(True)
+    dout = torch.randn_like(x)
+    (dx,) = torch.autograd.grad(T.cross_attention(x, x, x, bandwidth=9), x, dout)
+    leaves = [x.detach().clone().requires_grad_(True) for _ in range(3)]
+    parts = torch.autograd.grad(T.cross_attention(*leaves, bandwidth=9), leaves, dout)
+    bound = 2**-8 * sum(p.double().abs() for p in parts)  # two bf16 sums, half a step of each partial one
+    assert ((dx.double() - sum(p.double() for p in parts)).abs() <= bound).all()
+
+
+def test_inference_mode_and_no_grad(cuda):
+    t, lx, ly = make((2, 100, 120, 4, 2, 64, 9), torch.bfloat16, 67, True)
+    want = run(t, lx, ly, 9, grads=False)["out"]
+    leaves = [x.detach().requires_grad_(True) for x in t[:3]]
+    for mode in (torch.inference_mode, torch.no_grad):
+        with mode():
+            out = T.cross_attention(*leaves, lx.cuda(), ly.cuda(), bandwidth=9)
+        assert torch.equal(out, want) and not out.requires_grad
+
+
+def test_refusals(cuda):
+    q, k = torch.zeros(2, 3, 4, 8, device=cuda), torch.zeros(2, 5, 2, 8, device=cuda)
+    for kw, message in (
+        (dict(v=k.cpu()), "same device"),
+        (dict(lengths_x=torch.tensor([1, 2])), "lengths_x must be on"),
+        (dict(lengths_y=torch.tensor([1.0, 2.0], device=cuda)), "lengths_y must be int32 or int64"),
+        (dict(lengths_x=torch.tensor([1, 2, 3], device=cuda)), "lengths_x must have shape"),
+        (dict(v=k.half()), "same dtype"),
+    ):
+        with pytest.raises(RuntimeError, match=message):
+            T.cross_attention(q, k, kw.pop("v", k), **kw)
+    with pytest.raises(RuntimeError, match="positions must have shape"):
+        T.norm_rotate(q, positions=torch.zeros(3, 2, device=cuda))
+    with pytest.raises(RuntimeError, match="positions must be float32"):
+        T.norm_rotate(q, positions=torch.zeros(2, 3, device=cuda, dtype=torch.float64))
+    with pytest.raises(RuntimeError, match="weight must have shape"):
+        T.norm_rotate(q, torch.ones(4, device=cuda))
+    with pytest.raises(RuntimeError, match="rotary_dim"):
+        T.norm_rotate(q, rotary_dim=3)
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
@@ -313,8 +372,8 @@ def test_only_the_wanted_gradients(cuda):
     k = t[1].detach().requires_grad_(True)
     out = T.cross_attention(t[0], k, t[2])
     (dk,) = torch.autograd.grad(out.sum(), k, create_graph=True)
-    with pytest.raises(RuntimeError):
-        torch.autograd.grad(dk.sum(), k)  # differentiable once
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(dk.sum(), k)
 
 
 def test_a_training_step_together(cuda):

@@ -108,6 +108,11 @@ def test_c_attention_refuses_missing_buffers():
     assert lib.sdtw_cross_attention_backward_workspace_bytes(ctypes.byref(p)) > 0
     assert lib.sdtw_cross_attention_backward(ctypes.byref(p), 16, None, 16, 16, stride, 16, 16, 16, None, 0, None) == EWORKSPACE
     assert lib.sdtw_cross_attention_backward(ctypes.byref(p), 16, None, 16, 16, None, 16, 16, 16, 16, 1 << 20, None) == EINVAL
+    assert lib.sdtw_cross_attention(ctypes.byref(p), 24, None, 16, None, 0, None) == EINVAL  # outputs start on 16 bytes
+    assert lib.sdtw_cross_attention(ctypes.byref(p), 16, 24, 16, None, 0, None) == EINVAL
+    for bad in range(3):
+        outs = [24 if n == bad else 16 for n in range(3)]
+        assert lib.sdtw_cross_attention_backward(ctypes.byref(p), 16, None, 16, 16, stride, *outs, 16, 1 << 20, None) == EINVAL
     empty = attention_problem(B=0)
     assert lib.sdtw_cross_attention(ctypes.byref(empty), None, None, None, None, 0, None) == 0
 

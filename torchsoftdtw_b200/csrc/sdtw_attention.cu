@@ -30,6 +30,8 @@ sdtw_status checked(const sdtw_attention_problem* p)
     return SDTW_OK;
 }
 
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
 AttnArgs args_of(const sdtw_attention_problem* p)
 {
     AttnArgs a{};
@@ -55,18 +57,28 @@ AttnArgs args_of(const sdtw_attention_problem* p)
     return a;
 }
 
-// The tensor-core kernels take 16-bit operands that TMA can read; below kSplitRows packed rows a key head the kernel that
-// splits the states is faster.
-constexpr int64_t kSplitRows = 64;
-
 bool takes_tc(const sdtw_attention_problem* p, const AttnArgs& a)
 {
     return p->dtype != SDTW_F32 && p->M > 0 && attention_tc_takes(a.q, a.qs, a.B, a.N, a.Hq, a.d) &&
            attention_tc_takes(a.k, a.ks, a.B, a.M, a.Hkv, a.d) && attention_tc_takes(a.v, a.vs, a.B, a.M, a.Hkv, a.d);
 }
+// Whether the forward runs on the tcgen05 kernel. Up to 16 packed rows a key head read the cache at its bandwidth in the kernel
+// that splits the states, whatever the batch. Above, that kernel takes about 2.6 us (d <= 64; 3.7 us above) a 64-row block
+// and 64 states on each of two places an SM, beside 18 us; the tcgen05 kernel 0.85 us a 64-state step and wave of CTAs (128 rows,
+// two CTAs an SM; d > 64: 256 rows, one), beside 5 us. Both measured in bf16 at 8 heads, 512 and 4096 states:
+// N = 64, B = 1 and 64, M = 4096, d = 64: 24 and 269 us split, 52 and 132 us on tcgen05.
 bool forward_tc(const sdtw_attention_problem* p, const AttnArgs& a)
 {
-    return a.N * a.group > kSplitRows && takes_tc(p, a);
+    if (a.N * a.group <= 16 || !takes_tc(p, a)) return false;
+    int dev = 0, sms = 0;
+    if (current_sms(dev, sms) != cudaSuccess || sms <= 0) sms = 148;
+    const bool wide = a.d > 64;
+    const int64_t rows = wide ? 256 : 128, places = wide ? sms : 2 * sms, steps = (a.M + 63) / 64;
+    const int64_t ctas = static_cast<int64_t>(a.B) * a.Hq * ((a.N + rows - 1) / rows), waves = (ctas + places - 1) / places;
+    const int64_t blocks = static_cast<int64_t>(a.B) * a.Hkv * ((a.N * a.group + 63) / 64);
+    const double tc = static_cast<double>(waves) * (0.85 * static_cast<double>(steps) + 5.0);
+    const double split = 18.0 + (wide ? 3.7 : 2.6) * static_cast<double>(blocks) * static_cast<double>(steps) / (2.0 * sms);
+    return tc < split;
 }
 
 }  // namespace
@@ -88,7 +100,7 @@ sdtw_status sdtw_cross_attention(const sdtw_attention_problem* p, void* out, voi
     using namespace sdtw;
     const sdtw_status st = checked(p);
     if (st != SDTW_OK || p->B == 0 || p->N == 0) return st;
-    if (out == nullptr) return SDTW_EINVAL;
+    if (out == nullptr || !aligned16(out) || !aligned16(out_lo)) return SDTW_EINVAL;
     const size_t need = sdtw_cross_attention_workspace_bytes(p);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return SDTW_EWORKSPACE;
     AttnArgs a = args_of(p);
@@ -117,6 +129,7 @@ sdtw_status sdtw_cross_attention_backward(const sdtw_attention_problem* p, const
     if (p->N > 0 && (out == nullptr || lse == nullptr || dout == nullptr || dout_stride == nullptr || dq == nullptr))
         return SDTW_EINVAL;
     if (p->M > 0 && (dk == nullptr || dv == nullptr)) return SDTW_EINVAL;
+    if (!aligned16(out) || !aligned16(out_lo) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv)) return SDTW_EINVAL;
     const size_t need = sdtw_cross_attention_backward_workspace_bytes(p);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return SDTW_EWORKSPACE;
     AttnArgs a = args_of(p);

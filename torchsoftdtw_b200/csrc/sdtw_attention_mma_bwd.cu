@@ -236,8 +236,9 @@ cudaError_t launch(Args& f, cudaStream_t s)
     static_assert(G::BYTES <= 113 * 1024, "two CTAs an SM");
     const auto dq = attend_backward_mma_kernel<T, DPAD, VB, false>;
     const auto dkv = attend_backward_mma_kernel<T, DPAD, VB, true>;
-    cudaError_t e = cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, G::BYTES);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, G::BYTES);
+    static std::atomic<bool> allowed[2][128];
+    cudaError_t e = allow_smem(dq, G::BYTES, allowed[0]);
+    if (e == cudaSuccess) e = allow_smem(dkv, G::BYTES, allowed[1]);
     if (e != cudaSuccess) return e;
     if (f.a.N > 0) {
         f.tiles = static_cast<int>((f.a.N + kRows - 1) / kRows);

@@ -363,13 +363,6 @@ __global__ void __launch_bounds__(kThreads) join_splits_kernel(const __grid_cons
     if (lane == 0) store_lse(a, b, hk, r, top == -INFINITY ? -INFINITY : top + log2f(all));
 }
 
-int device_sms()
-{
-    int dev = 0, sms = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess) (void)cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    return sms;
-}
-
 struct Plan {
     int row_warps, rows_per_cta, row_blocks, splits;
     bool cluster;
@@ -385,7 +378,9 @@ Plan plan_of(const AttnArgs& a, bool f32)
     p.rows_per_cta = 16 * p.row_warps;
     p.row_blocks = static_cast<int>((rows + p.rows_per_cta - 1) / p.rows_per_cta);
     const int64_t units = static_cast<int64_t>(a.B) * a.Hkv * p.row_blocks;
-    const int64_t slots = 2 * device_sms();
+    int dev = 0, sms = 0;
+    if (current_sms(dev, sms) != cudaSuccess) sms = 148;
+    const int64_t slots = 2 * sms;
     int64_t cells = a.M;
     if (a.bw >= 0 && a.N > 1) {  // what the rows of a CTA reach when the lengths are full
         const double slope = static_cast<double>(a.M) / static_cast<double>(a.N);
@@ -418,7 +413,8 @@ cudaError_t launch(const SplitArgs& f, cudaStream_t s)
     using G = Geom<T, DPAD, ROWWARPS>;
     static_assert(G::BYTES <= 113 * 1024, "two CTAs an SM");
     const auto kernel = attend_split_kernel<T, DPAD, ROWWARPS, VB>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::BYTES);
+    static std::atomic<bool> allowed[128];
+    cudaError_t e = allow_smem(kernel, G::BYTES, allowed);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t c{};
     c.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(f.a.B) * f.a.Hkv * f.row_blocks * f.splits));

@@ -453,20 +453,9 @@ template <typename T, int DPAD, int NT>
 cudaError_t launch_forward(FwdArgs& f, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t s)
 {
     using G = Geom<DPAD, NT>;
-    static std::mutex mu;
-    static bool set[128] = {};
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
+    static std::atomic<bool> allowed[128];
+    const cudaError_t e = allow_smem(attend_tc_kernel<T, DPAD, NT>, G::BYTES, allowed);
     if (e != cudaSuccess) return e;
-    if (dev >= 128) return cudaErrorInvalidDevice;
-    {
-        std::lock_guard<std::mutex> lock(mu);
-        if (!set[dev]) {
-            e = cudaFuncSetAttribute(attend_tc_kernel<T, DPAD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::BYTES);
-            if (e != cudaSuccess) return e;
-            set[dev] = true;
-        }
-    }
     f.tiles = static_cast<int>((f.a.N + kTile * NT - 1) / (kTile * NT));
     const int64_t grid = static_cast<int64_t>(f.a.B) * f.a.Hq * f.tiles;
     attend_tc_kernel<T, DPAD, NT><<<static_cast<unsigned>(grid), G::THREADS, G::BYTES, s>>>(mq, mk, mv, f);

@@ -55,16 +55,18 @@ struct Geom {
     static constexpr int ROW_BYTES = kTile * DPAD * 2, COL_BYTES = kCols * DPAD * 2;
     static constexpr int ROW_BLOCK = kTile * 128, COL_BLOCK = kCols * 128;  // 64 features of a tile
     static constexpr int NBLOCK = DPAD / 64;
-    static constexpr int STAGES = DPAD == 128 ? 4 : 3;
+    // Tiles in flight of the columns' first operand (K, or Q: scores run up to three tiles ahead of its last use) and second.
+    static constexpr int S0 = DPAD == 128 ? 6 : 3, S1 = 3;
     static constexpr int BUFS = DPAD == 128 ? 2 : 1;  // tiles in flight
     static constexpr int ELEM_WARPS = 8 * BUFS, MMA_WARP = ELEM_WARPS, TMA_WARP = ELEM_WARPS + 1;
     static constexpr int THREADS = 32 * (ELEM_WARPS + 2);
     static constexpr int OFF_RING = 2 * ROW_BYTES;
-    static constexpr int OFF_STAT = OFF_RING + STAGES * 2 * COL_BYTES;
-    static constexpr int STAT_BYTES = 4 * (STAGES * 2 * kCols > 2 * kTile ? STAGES * 2 * kCols : 2 * kTile);
+    static constexpr int OFF_STAT = OFF_RING + (S0 + S1) * COL_BYTES;
+    static constexpr int STAT_BYTES = 4 * (S0 * 2 * kCols > 2 * kTile ? S0 * 2 * kCols : 2 * kTile);
     static constexpr int OFF_BAR = OFF_STAT + STAT_BYTES;
-    // row_full, fix, full[2][STAGES], empty[2][STAGES], acc_full, and six a buffer
-    static constexpr int NBAR = 3 + 4 * STAGES + 6 * BUFS;
+    // row_full, fix, full[S0 + S1], empty[S0 + S1], acc_full, and six a buffer
+    static constexpr int NBAR = 3 + 2 * (S0 + S1) + 6 * BUFS;
+    static_assert(S0 % BUFS == 0, "a group of elementwise warps sees every turn of its stages");
     static constexpr int OFF_MISC = OFF_BAR + 8 * NBAR;
     static constexpr int BYTES = OFF_MISC + 32 + 1024;
     static constexpr int CTAS = DPAD == 64 ? 2 : 1;  // an SM
@@ -137,7 +139,8 @@ __device__ __forceinline__ void load_tiles(unsigned char* sm, uint32_t base, con
             tma_load_4d(base + G::ROW_BYTES + x * G::ROW_BLOCK, r2, row_full, 64 * x, row0, row_head, b);
         }
     }
-    Turn<G::STAGES> turn;
+    Turn<G::S0> turn0;
+    Turn<G::S1> turn1;
     int issued[2] = {0, 0}, fixes = 0;
     bool ok = true;
     for (int t = 0; t < steps && ok; ++t) {
@@ -147,14 +150,15 @@ __device__ __forceinline__ void load_tiles(unsigned char* sm, uint32_t base, con
         const bool clear = left < kCols && length < extent;
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
-            const uint32_t fullb = full + 8 * (which * G::STAGES + turn.at), emptyb = empty + 8 * (which * G::STAGES + turn.at);
-            ok = ok && (t < G::STAGES || mbar_wait(emptyb, turn.phase ^ 1, bound));
+            const int place = which ? G::S0 + turn1.at : turn0.at;
+            const uint32_t fullb = full + 8 * place, emptyb = empty + 8 * place;
+            ok = ok && (t < (which ? G::S1 : G::S0) || mbar_wait(emptyb, (which ? turn1.phase : turn0.phase) ^ 1, bound));
             if (!ok) break;
             if (which == 0) {
-                stats(turn.at, t);
+                stats(turn0.at, t);
                 __syncwarp();
             }
-            const int at = G::OFF_RING + (2 * turn.at + which) * G::COL_BYTES;
+            const int at = G::OFF_RING + place * G::COL_BYTES;
             const uint32_t bar = clear ? fix : fullb;
             if (lane == 0) {
                 mbar_expect_tx(bar, G::COL_BYTES);
@@ -174,14 +178,15 @@ __device__ __forceinline__ void load_tiles(unsigned char* sm, uint32_t base, con
             }
             ++issued[which];
         }
-        turn.next();
+        turn0.next();
+        turn1.next();
     }
     // Every load has landed before the CTA ends (also after an abort).
     mbar_drain(row_full, 0, bound.timeout_ns);
-#pragma unroll
-    for (int which = 0; which < 2; ++which)
-        for (int t = issued[which] < G::STAGES ? 0 : issued[which] - G::STAGES; t < issued[which]; ++t)
-            mbar_drain(full + 8 * (which * G::STAGES + t % G::STAGES), (t / G::STAGES) & 1, bound.timeout_ns);
+    for (int t = issued[0] < G::S0 ? 0 : issued[0] - G::S0; t < issued[0]; ++t)
+        mbar_drain(full + 8 * (t % G::S0), (t / G::S0) & 1, bound.timeout_ns);
+    for (int t = issued[1] < G::S1 ? 0 : issued[1] - G::S1; t < issued[1]; ++t)
+        mbar_drain(full + 8 * (G::S0 + t % G::S1), (t / G::S1) & 1, bound.timeout_ns);
 }
 
 // d = rows cols^T over all features (those past d are zero; a branch between products costs more than they do).
@@ -223,8 +228,8 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
     unsigned char* sm = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     const uint32_t base = smem_addr(sm);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t row_full = base + G::OFF_BAR, fix = row_full + 8, full = fix + 8, empty = full + 16 * G::STAGES;
-    const uint32_t acc_full = empty + 16 * G::STAGES, s_full = acc_full + 8, s_free = s_full + 8 * G::BUFS;
+    const uint32_t row_full = base + G::OFF_BAR, fix = row_full + 8, full = fix + 8, empty = full + 8 * (G::S0 + G::S1);
+    const uint32_t acc_full = empty + 8 * (G::S0 + G::S1), s_full = acc_full + 8, s_free = s_full + 8 * G::BUFS;
     const uint32_t dp_full = s_free + 8 * G::BUFS, dp_free = dp_full + 8 * G::BUFS, ds_full = dp_free + 8 * G::BUFS;
     const uint32_t ds_free = ds_full + 8 * G::BUFS;
     uint32_t* misc = reinterpret_cast<uint32_t*>(sm + G::OFF_MISC);
@@ -241,7 +246,7 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
     if (tid == 0) {
         mbar_init(row_full, 1);
         mbar_init(fix, 1);
-        for (int s = 0; s < 4 * G::STAGES; ++s) mbar_init(full + 8 * s, 1);
+        for (int s = 0; s < 2 * (G::S0 + G::S1); ++s) mbar_init(full + 8 * s, 1);
         mbar_init(acc_full, 1);
         for (int x = 0; x < G::BUFS; ++x) {
             mbar_init(s_full + 8 * x, 1);
@@ -285,37 +290,55 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
         if (n > 0) {
             const uint32_t leader = elect_leader();
             const uint32_t idesc_s = mma_idesc<T>(kCols, false), idesc_q = mma_idesc<T>(f.dn, true);
-            Turn<G::STAGES> ahead, now;
-            const auto ring = [&](int at, int which) { return base + G::OFF_RING + (2 * at + which) * G::COL_BYTES; };
-            // S and dP of tile i, each as soon as the elementwise warps have read the last ones of its buffer.
-            const auto next_products = [&](int i) {
+            Turn<G::S0> now;
+            const auto ring = [&](int at, int which) { return base + G::OFF_RING + ((which ? G::S0 : 0) + at) * G::COL_BYTES; };
+            // S, and dP, of tile i, when the elementwise warps have read the last one of its buffer; then tile i's share of dq.
+            Turn<G::S0> ks;
+            Turn<G::S1> vs;
+            const auto scores = [&](int i) {
                 const int x = i % G::BUFS;
-                const uint32_t before = (i / G::BUFS - 1) & 1, col = tmem + x * BUF_COLS;
-                if (!mbar_wait(full + 8 * ahead.at, ahead.phase, bound)) return false;
-                if (i >= G::BUFS && !mbar_wait(s_free + 8 * x, before, bound)) return false;
+                if (!mbar_wait(full + 8 * ks.at, ks.phase, bound)) return false;
+                if (i >= G::BUFS && !mbar_wait(s_free + 8 * x, (i / G::BUFS - 1) & 1, bound)) return false;
                 fence_after();
-                mma_rows<DPAD>(col, base, ring(ahead.at, 0), idesc_s, leader);
+                mma_rows<DPAD>(tmem + x * BUF_COLS, base, ring(ks.at, 0), idesc_s, leader);
                 mma_commit(s_full + 8 * x, leader);
-                if (!mbar_wait(full + 8 * (G::STAGES + ahead.at), ahead.phase, bound)) return false;
-                if (i >= G::BUFS && !mbar_wait(dp_free + 8 * x, before, bound)) return false;
-                fence_after();
-                mma_rows<DPAD>(col + DP_COL, base + G::ROW_BYTES, ring(ahead.at, 1), idesc_s, leader);
-                mma_commit(dp_full + 8 * x, leader);
-                mma_commit(empty + 8 * (G::STAGES + ahead.at), leader);
-                ahead.next();
+                ks.next();
                 return true;
             };
-            bool ok = mbar_wait(row_full, 0, bound);
-            for (int i = 0; i < G::BUFS && i < n; ++i) ok = ok && next_products(i);
-            for (int i = 0; ok && i < n; ++i) {
+            const auto dprobs = [&](int i) {
                 const int x = i % G::BUFS;
-                if (i + G::BUFS < n && !(ok = next_products(i + G::BUFS))) break;
-                if (!(ok = mbar_wait(ds_full + 8 * x, (i / G::BUFS) & 1, bound))) break;
+                if (!mbar_wait(full + 8 * (G::S0 + vs.at), vs.phase, bound)) return false;
+                if (i >= G::BUFS && !mbar_wait(dp_free + 8 * x, (i / G::BUFS - 1) & 1, bound)) return false;
+                fence_after();
+                mma_rows<DPAD>(tmem + x * BUF_COLS + DP_COL, base + G::ROW_BYTES, ring(vs.at, 1), idesc_s, leader);
+                mma_commit(dp_full + 8 * x, leader);
+                mma_commit(empty + 8 * (G::S0 + vs.at), leader);
+                vs.next();
+                return true;
+            };
+            const auto sums = [&](int i) {
+                const int x = i % G::BUFS;
+                if (!mbar_wait(ds_full + 8 * x, (i / G::BUFS) & 1, bound)) return false;
                 fence_after();
                 mma_cols<DPAD>(tmem + ACC_COL, tmem + x * BUF_COLS + DS_COL, 16, ring(now.at, 0), idesc_q, i > 0, leader);
                 mma_commit(ds_free + 8 * x, leader);
                 mma_commit(empty + 8 * now.at, leader);
                 now.next();
+                return true;
+            };
+            bool ok = mbar_wait(row_full, 0, bound);
+            for (int i = 0; i < G::BUFS && i < n; ++i) ok = ok && scores(i) && dprobs(i);
+            if (G::BUFS == 1) {
+                for (int i = 0; ok && i < n; ++i) {
+                    if (i + 1 < n) ok = scores(i + 1) && dprobs(i + 1);
+                    ok = ok && sums(i);
+                }
+            } else {
+                // (Sums of tile i - 1 between S and dP of the next: 10% slower, for the two groups then wait for each other.)
+                for (int i = 0; ok && i < n; ++i) {
+                    if (i + 2 < n) ok = scores(i + 2) && dprobs(i + 2);
+                    ok = ok && sums(i);
+                }
             }
             mma_commit(acc_full, leader);
             mbar_drain(acc_full, 0, f.timeout_ns);  // before the tensor memory is given back
@@ -323,37 +346,44 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
         __syncwarp();
     } else {
         // ---------------- elementwise: two threads a row, 32 columns each ----------------
-        // delta and |do|^2 of the tile's rows: LPR lanes a row.
-        constexpr int LPR = DPAD / 8, RPW = 32 / LPR;
-#pragma unroll 4
-        for (int r0 = warp * RPW; r0 < kTile; r0 += G::ELEM_WARPS * RPW) {
-            const int r = r0 + lane / LPR, c = lane % LPR * 8;
-            const int64_t i = row0 + r;
-            float dot = 0.f, nrm = 0.f;
-            if (i < nx && c < a.d && ny > 0) {
-                const T* gp = static_cast<const T*>(a.dout) + b * a.gs.b + i * a.gs.n + h * a.gs.h + c;
+        // delta and |do|^2 of the tile's rows: LPR lanes a row, all loads ahead of the sums (rows and features outside read a
+        // place inside, and count as zero).
+        constexpr int LPR = DPAD / 8, RPW = 32 / LPR, ROUNDS = kTile / (G::ELEM_WARPS * RPW);
+        if (n > 0) {
+            Vec<T, 8> g[ROUNDS], o[ROUNDS], lo[ROUNDS];
+            const int c = lane % LPR * 8 < a.d ? lane % LPR * 8 : 0;
+#pragma unroll
+            for (int t = 0; t < ROUNDS; ++t) {
+                const int64_t i1 = row0 + (t * G::ELEM_WARPS + warp) * RPW + lane / LPR, i = i1 < nx ? i1 : row0;
                 const int64_t at = ((static_cast<int64_t>(b) * a.N + i) * a.Hq + h) * a.d + c;
-                const Vec<T, 8> g = *reinterpret_cast<const Vec<T, 8>*>(gp);
-                const Vec<T, 8> o = *reinterpret_cast<const Vec<T, 8>*>(static_cast<const T*>(a.o) + at);
-                Vec<T, 8> lo{};
-                if (a.o_lo) lo = *reinterpret_cast<const Vec<T, 8>*>(static_cast<const T*>(a.o_lo) + at);
+                g[t] = *reinterpret_cast<const Vec<T, 8>*>(static_cast<const T*>(a.dout) + b * a.gs.b + i * a.gs.n + h * a.gs.h + c);
+                o[t] = *reinterpret_cast<const Vec<T, 8>*>(static_cast<const T*>(a.o) + at);
+                lo[t] = a.o_lo ? *reinterpret_cast<const Vec<T, 8>*>(static_cast<const T*>(a.o_lo) + at) : Vec<T, 8>{};
+            }
+#pragma unroll
+            for (int t = 0; t < ROUNDS; ++t) {
+                const int r = (t * G::ELEM_WARPS + warp) * RPW + lane / LPR;
+                const bool on = row0 + r < nx && lane % LPR * 8 < a.d;
+                float dot = 0.f, nrm = 0.f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float gf = to_f(g.e[e]);
-                    dot = fmaf(gf, to_f(o.e[e]) + to_f(lo.e[e]), dot);
+                    const float gf = on ? to_f(g[t].e[e]) : 0.f;
+                    dot = on ? fmaf(gf, to_f(o[t].e[e]) + to_f(lo[t].e[e]), dot) : 0.f;
                     nrm = fmaf(gf, gf, nrm);
                 }
-            }
 #pragma unroll
-            for (int x = LPR / 2; x > 0; x >>= 1) {
-                dot += __shfl_xor_sync(kFull, dot, x);
-                nrm += __shfl_xor_sync(kFull, nrm, x);
-            }
-            if (lane % LPR == 0) {
-                s_delta[r] = dot;
-                s_norm[r] = nrm;
-                if (i < a.N) a.delta[(static_cast<int64_t>(b) * a.Hq + h) * a.N + i] = dot;
-                if (is_half<T> && i < nx) atomicMax(f.peak + b * a.Hkv + hk, __float_as_uint(nrm));
+                for (int x = LPR / 2; x > 0; x >>= 1) {
+                    dot += __shfl_xor_sync(kFull, dot, x);
+                    nrm += __shfl_xor_sync(kFull, nrm, x);
+                }
+                if (lane % LPR == 0) {
+                    s_delta[r] = dot;
+                    s_norm[r] = nrm;
+                    if (row0 + r < nx) {
+                        a.delta[(static_cast<int64_t>(b) * a.Hq + h) * a.N + row0 + r] = dot;
+                        if (is_half<T>) atomicMax(f.peak + b * a.Hkv + hk, __float_as_uint(nrm));
+                    }
+                }
             }
         }
         const int x = warp >> 3, half = (warp >> 2) & 1, r = 32 * (warp & 3) + lane;  // x: the buffer of this group of warps
@@ -449,12 +479,12 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
     unsigned char* sm = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     const uint32_t base = smem_addr(sm);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t row_full = base + G::OFF_BAR, fix = row_full + 8, full = fix + 8, empty = full + 16 * G::STAGES;
-    const uint32_t acc_full = empty + 16 * G::STAGES, s_full = acc_full + 8, p_full = s_full + 8 * G::BUFS;
+    const uint32_t row_full = base + G::OFF_BAR, fix = row_full + 8, full = fix + 8, empty = full + 8 * (G::S0 + G::S1);
+    const uint32_t acc_full = empty + 8 * (G::S0 + G::S1), s_full = acc_full + 8, p_full = s_full + 8 * G::BUFS;
     const uint32_t dp_full = p_full + 8 * G::BUFS, ds_full = dp_full + 8 * G::BUFS, dv_done = ds_full + 8 * G::BUFS;
     const uint32_t dk_done = dv_done + 8 * G::BUFS;
     uint32_t* misc = reinterpret_cast<uint32_t*>(sm + G::OFF_MISC);
-    float* stats = reinterpret_cast<float*>(sm + G::OFF_STAT);  // STAGES of (shift - lse, delta) of 64 queries
+    float* stats = reinterpret_cast<float*>(sm + G::OFF_STAT);  // S0 of (shift - lse, delta) of 64 queries
     const Bound bound{f.timeout_ns, reinterpret_cast<volatile int*>(misc + 1), a.err};
 
     const int kt = static_cast<int>(blockIdx.x % f.tiles);
@@ -465,7 +495,7 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
     if (tid == 0) {
         mbar_init(row_full, 1);
         mbar_init(fix, 1);
-        for (int s = 0; s < 4 * G::STAGES; ++s) mbar_init(full + 8 * s, 1);
+        for (int s = 0; s < 2 * (G::S0 + G::S1); ++s) mbar_init(full + 8 * s, 1);
         mbar_init(acc_full, 1);
         for (int x = 0; x < G::BUFS; ++x) {
             mbar_init(s_full + 8 * x, 1);
@@ -528,8 +558,9 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
         if (n > 0) {
             const uint32_t leader = elect_leader();
             const uint32_t idesc_s = mma_idesc<T>(kCols, false), idesc_o = mma_idesc<T>(f.dn, true);
-            Turn<G::STAGES> sq, sg, now;  // the next S, the next dP, the tile whose sums are due
-            const auto ring = [&](int at, int which) { return base + G::OFF_RING + (2 * at + which) * G::COL_BYTES; };
+            Turn<G::S0> sq;  // the next S
+            Turn<G::S1> sg;  // the next dP
+            const auto ring = [&](int at, int which) { return base + G::OFF_RING + ((which ? G::S0 : 0) + at) * G::COL_BYTES; };
             // S (dP) of tile i, when the product that read P (dS) there has completed.
             const auto scores = [&](int i) {
                 const int x = i % G::BUFS;
@@ -543,7 +574,7 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
             };
             const auto dprobs = [&](int i) {
                 const int x = i % G::BUFS;
-                if (!mbar_wait(full + 8 * (G::STAGES + sg.at), sg.phase, bound)) return false;
+                if (!mbar_wait(full + 8 * (G::S0 + sg.at), sg.phase, bound)) return false;
                 if (i >= G::BUFS && !mbar_wait(dk_done + 8 * x, (i / G::BUFS - 1) & 1, bound)) return false;
                 fence_after();
                 mma_rows<DPAD>(tmem + x * BUF_COLS + DP_COL, base + G::ROW_BYTES, ring(sg.at, 1), idesc_s, leader);
@@ -551,27 +582,41 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
                 sg.next();
                 return true;
             };
+            Turn<G::S1> vt;  // the tiles whose shares of dv and of dk are due
+            Turn<G::S0> kt;
+            const auto sums_v = [&](int i) {
+                const int x = i % G::BUFS;
+                if (!mbar_wait(p_full + 8 * x, (i / G::BUFS) & 1, bound)) return false;
+                fence_after();
+                mma_cols<DPAD>(tmem + DV_COL, tmem + x * BUF_COLS, 32, ring(vt.at, 1), idesc_o, i > 0, leader);
+                mma_commit(dv_done + 8 * x, leader);
+                mma_commit(empty + 8 * (G::S0 + vt.at), leader);
+                vt.next();
+                return true;
+            };
+            const auto sums_k = [&](int i) {
+                const int x = i % G::BUFS;
+                if (!mbar_wait(ds_full + 8 * x, (i / G::BUFS) & 1, bound)) return false;
+                fence_after();
+                mma_cols<DPAD>(tmem + DK_COL, tmem + x * BUF_COLS + DP_COL, 32, ring(kt.at, 0), idesc_o, i > 0, leader);
+                mma_commit(dk_done + 8 * x, leader);
+                mma_commit(empty + 8 * kt.at, leader);
+                kt.next();
+                return true;
+            };
             bool ok = mbar_wait(row_full, 0, bound);
             for (int i = 0; i < G::BUFS && i < n; ++i) ok = ok && scores(i) && dprobs(i);
-            for (int i = 0; ok && i < n; ++i) {
-                const int x = i % G::BUFS;
-                const uint32_t phase = (i / G::BUFS) & 1;
-                const bool more = i + G::BUFS < n;
-                if (!(ok = mbar_wait(p_full + 8 * x, phase, bound))) break;
-                fence_after();
-                mma_cols<DPAD>(tmem + DV_COL, tmem + x * BUF_COLS, 32, ring(now.at, 1), idesc_o, i > 0, leader);
-                mma_commit(dv_done + 8 * x, leader);
-                mma_commit(empty + 8 * (G::STAGES + now.at), leader);
-                // One buffer: the scores at once, while dS is formed. Two: behind dK, so that nothing waits for dV alone.
-                if (G::BUFS == 1 && more && !(ok = scores(i + G::BUFS))) break;
-                if (!(ok = mbar_wait(ds_full + 8 * x, phase, bound))) break;
-                fence_after();
-                mma_cols<DPAD>(tmem + DK_COL, tmem + x * BUF_COLS + DP_COL, 32, ring(now.at, 0), idesc_o, i > 0, leader);
-                mma_commit(dk_done + 8 * x, leader);
-                mma_commit(empty + 8 * now.at, leader);
-                if (G::BUFS > 1 && more && !(ok = scores(i + G::BUFS))) break;
-                if (more) ok = dprobs(i + G::BUFS);
-                now.next();
+            if (G::BUFS == 1) {
+                for (int i = 0; ok && i < n; ++i) {
+                    const bool more = i + 1 < n;  // the next scores while dS is formed, the next dP behind dk
+                    ok = sums_v(i) && (!more || scores(i + 1)) && sums_k(i) && (!more || dprobs(i + 1));
+                }
+            } else {
+                // Each overwritten operand is awaited while the product after the one that reads it runs.
+                for (int i = 0; ok && i < n; ++i) {
+                    const bool more = i + 2 < n;
+                    ok = sums_v(i) && sums_k(i) && (!more || (scores(i + 2) && dprobs(i + 2)));
+                }
             }
             mma_commit(acc_full, leader);
             mbar_drain(acc_full, 0, f.timeout_ns);  // before the tensor memory is given back
@@ -587,7 +632,7 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
         if (j < ny && nx > 0) column_cells(a, j, nx, ny, lo, hi);
         const int ilo = static_cast<int>(lo), width = static_cast<int>(hi - lo);
         bool ok = true;
-        Turn<G::STAGES> turn;
+        Turn<G::S0> turn;
         int tile = x;
         if (x == 1) turn.next();
         for (int it = x; it < n; it += G::BUFS) {
@@ -672,12 +717,6 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
     }
 }
 
-template <typename K>
-cudaError_t allow_smem(K kernel, int bytes)
-{
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-}
-
 template <typename T, int DPAD>
 cudaError_t backward_d(BwdArgs& f, cudaStream_t s)
 {
@@ -703,8 +742,9 @@ cudaError_t backward_d(BwdArgs& f, cudaStream_t s)
         e = cudaMemsetAsync(f.peak, 0, sizeof(uint32_t) * static_cast<size_t>(a.B) * a.Hkv, s);
         if (e != cudaSuccess) return e;
     }
-    if ((e = allow_smem(attend_dq_tc_kernel<T, DPAD>, G::BYTES)) != cudaSuccess) return e;
-    if ((e = allow_smem(attend_dkdv_tc_kernel<T, DPAD>, G::BYTES)) != cudaSuccess) return e;
+    static std::atomic<bool> allowed[2][128];
+    if ((e = allow_smem(attend_dq_tc_kernel<T, DPAD>, G::BYTES, allowed[0])) != cudaSuccess) return e;
+    if ((e = allow_smem(attend_dkdv_tc_kernel<T, DPAD>, G::BYTES, allowed[1])) != cudaSuccess) return e;
     f.tiles = static_cast<int>((a.N + kTile - 1) / kTile);
     attend_dq_tc_kernel<T, DPAD><<<static_cast<unsigned>(static_cast<int64_t>(a.B) * a.Hq * f.tiles), G::THREADS, G::BYTES, s>>>(
         q_rows, g_rows, k_cols, v_cols, f);

@@ -393,14 +393,6 @@ sdtw_status clip_run(const sdtw_tensor_ref* refs, int64_t count, int kind, bool 
     return e == cudaSuccess ? SDTW_OK : static_cast<sdtw_status>(e);
 }
 
-int sm_count(int& sms)
-{
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    return e;
-}
-
 sdtw_status clip_any(const sdtw_tensor_ref* refs, int64_t count, int kind, bool scale, double max_norm, void* norm,
                      int norm_f64, void* workspace, size_t workspace_bytes, void* stream)
 {
@@ -415,8 +407,9 @@ sdtw_status clip_any(const sdtw_tensor_ref* refs, int64_t count, int kind, bool 
         wide = wide || r.dtype == SDTW_F64;
     }
     if (workspace == nullptr || workspace_bytes < sdtw_clip_workspace_bytes(count)) return SDTW_EWORKSPACE;
-    int sms = 0;
-    if (const int e = sm_count(sms)) return static_cast<sdtw_status>(e);
+    int dev = 0, sms = 0;
+    const cudaError_t e = current_sms(dev, sms);
+    if (e != cudaSuccess) return static_cast<sdtw_status>(e);
     if (sms * kCtasPerSm > kMaxCtas) sms = kMaxCtas / kCtasPerSm;
     Squares* partials = static_cast<Squares*>(workspace);
     cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -418,8 +418,7 @@ template <typename T, bool GRAD>
 sdtw_status run(RotArgs& a, void* dweight, cudaStream_t s)
 {
     int dev = 0, sms = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    cudaError_t e = current_sms(dev, sms);
     if (e != cudaSuccess) return static_cast<sdtw_status>(e);
     const auto fits = [&](int V) {
         const int64_t bytes = V * static_cast<int64_t>(sizeof(T));

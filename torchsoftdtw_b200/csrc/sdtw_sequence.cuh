@@ -2,6 +2,8 @@
 // rotation, gradient clipping): element types, per-sample lengths, vector loads.
 #pragma once
 
+#include <atomic>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -9,6 +11,34 @@
 #include "sdtw_common.cuh"
 
 namespace sdtw {
+
+// SMs of the current device, asked of the driver once (a decoded token's call is bound by the host).
+inline cudaError_t current_sms(int& dev, int& sms)
+{
+    static std::atomic<int> known[128];
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 128) return cudaErrorInvalidDevice;
+    sms = known[dev].load(std::memory_order_relaxed);
+    if (sms > 0) return cudaSuccess;
+    e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e == cudaSuccess) known[dev].store(sms, std::memory_order_relaxed);
+    return e;
+}
+
+// Allows a kernel its dynamic shared memory, once a device (`done`: one flag a device, of this kernel alone).
+template <typename K>
+inline cudaError_t allow_smem(K kernel, int bytes, std::atomic<bool> (&done)[128])
+{
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 128) return cudaErrorInvalidDevice;
+    if (done[dev].load(std::memory_order_relaxed)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done[dev].store(true, std::memory_order_relaxed);
+    return e;
+}
 
 inline size_t dtype_size(int dt) { return dt == SDTW_F64 ? 8 : (dt == SDTW_F32 ? 4 : 2); }
 
