@@ -147,7 +147,9 @@ def test_one_tensor_in_all_places(cuda):
     (dx,) = torch.autograd.grad(T.cross_attention(x, x, x, bandwidth=9), x, dout)
     leaves = [x.detach().clone().requires_grad_(True) for _ in range(3)]
     parts = torch.autograd.grad(T.cross_attention(*leaves, bandwidth=9), leaves, dout)
-    bound = 2**-8 * sum(p.double().abs() for p in parts)  # two bf16 sums, half a step of each partial one
+    # Autograd adds three bf16 numbers in two sums, each off by at most u = 2^-8 of itself (half a step): together
+    # u |a + b| + u (|a + b| (1 + u) + |c|) <= 2 u (1 + u) (|a| + |b| + |c|).
+    bound = 2 * 2.0**-8 * (1 + 2.0**-8) * sum(p.double().abs() for p in parts)
     assert ((dx.double() - sum(p.double() for p in parts)).abs() <= bound).all()
 
 
