@@ -157,41 +157,87 @@ __device__ __forceinline__ void store_raw(const Raw<T, V, K>& r, T* row, const i
     }
 }
 
-// A lane's pairs, two by two: the firsts in p, the seconds in q (NP = pairs a lane, even).
+// Two neighbouring 16-bit features as floats, and back in one conversion.
+__device__ __forceinline__ F2 two_f(const __half* e)
+{
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(e));
+    return {f.x, f.y};
+}
+__device__ __forceinline__ F2 two_f(const __nv_bfloat16* e)
+{
+    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(e));
+    return {f.x, f.y};
+}
+__device__ __forceinline__ void put_two(__half* e, F2 f) { *reinterpret_cast<__half2*>(e) = __floats2half2_rn(f.x, f.y); }
+__device__ __forceinline__ void put_two(__nv_bfloat16* e, F2 f)
+{
+    *reinterpret_cast<__nv_bfloat162*>(e) = __floats2bfloat162_rn(f.x, f.y);
+}
+
+// A lane's pairs, two by two: the firsts in p, the seconds in q (V K pairs, an even number).
 template <typename T, int V, int K, bool SPLIT>
 __device__ __forceinline__ void unpack(const Raw<T, V, K>& r, F2 (&p)[V * K / 2], F2 (&q)[V * K / 2])
 {
-    const auto at = [&](int pair, bool second) {
-        const int k = pair / V, o = place<V, SPLIT>(pair % V, second);
-        return to_f(o < V ? r.v[k][0].e[o] : r.v[k][1].e[o - V]);
-    };
+    if constexpr (sizeof(T) == 2 && V > 1) {
 #pragma unroll
-    for (int i = 0; i < V * K / 2; ++i) {
-        p[i] = {at(2 * i, false), at(2 * i + 1, false)};
-        q[i] = {at(2 * i, true), at(2 * i + 1, true)};
+        for (int i = 0; i < V / 2; ++i) {
+            if constexpr (SPLIT) {
+                p[i] = two_f(r.v[0][0].e + 2 * i);
+                q[i] = two_f(r.v[0][1].e + 2 * i);
+            } else {  // features 4i .. 4i + 3: first, second, first, second
+                const F2 a = two_f(r.v[0][4 * i / V].e + 4 * i % V), b = two_f(r.v[0][(4 * i + 2) / V].e + (4 * i + 2) % V);
+                p[i] = {a.x, b.x};
+                q[i] = {a.y, b.y};
+            }
+        }
+    } else {
+        const auto at = [&](int pair, bool second) {
+            const int k = pair / V, o = place<V, SPLIT>(pair % V, second);
+            return to_f(o < V ? r.v[k][0].e[o] : r.v[k][1].e[o - V]);
+        };
+#pragma unroll
+        for (int i = 0; i < V * K / 2; ++i) {
+            p[i] = {at(2 * i, false), at(2 * i + 1, false)};
+            q[i] = {at(2 * i, true), at(2 * i + 1, true)};
+        }
     }
 }
 template <typename T, int V, int K, bool SPLIT>
 __device__ __forceinline__ void repack(Raw<T, V, K>& r, const F2 (&p)[V * K / 2], const F2 (&q)[V * K / 2])
 {
-    const auto put = [&](int pair, bool second, float x) {
-        const int k = pair / V, o = place<V, SPLIT>(pair % V, second);
-        (o < V ? r.v[k][0].e[o] : r.v[k][1].e[o - V]) = from_f<T>(x);
-    };
+    if constexpr (sizeof(T) == 2 && V > 1) {
 #pragma unroll
-    for (int i = 0; i < V * K / 2; ++i) {
-        put(2 * i, false, p[i].x);
-        put(2 * i + 1, false, p[i].y);
-        put(2 * i, true, q[i].x);
-        put(2 * i + 1, true, q[i].y);
+        for (int i = 0; i < V / 2; ++i) {
+            if constexpr (SPLIT) {
+                put_two(r.v[0][0].e + 2 * i, p[i]);
+                put_two(r.v[0][1].e + 2 * i, q[i]);
+            } else {
+                put_two(r.v[0][4 * i / V].e + 4 * i % V, {p[i].x, q[i].x});
+                put_two(r.v[0][(4 * i + 2) / V].e + (4 * i + 2) % V, {p[i].y, q[i].y});
+            }
+        }
+    } else {
+        const auto put = [&](int pair, bool second, float x) {
+            const int k = pair / V, o = place<V, SPLIT>(pair % V, second);
+            (o < V ? r.v[k][0].e[o] : r.v[k][1].e[o - V]) = from_f<T>(x);
+        };
+#pragma unroll
+        for (int i = 0; i < V * K / 2; ++i) {
+            put(2 * i, false, p[i].x);
+            put(2 * i + 1, false, p[i].y);
+            put(2 * i, true, q[i].x);
+            put(2 * i + 1, true, q[i].y);
+        }
     }
 }
 
-// How many heads a lane has in flight, and how many CTAs of an SM the registers that this takes leave room for.
+// How many heads a lane has in flight, and how many CTAs of an SM the registers that this takes leave room for. Measured,
+// 16 x 4096 x 16 x 128 bf16 (V = 8): forward 97 us with four heads and two CTAs, 126 with two and three; gradient 179 with
+// one, 204 with two. 32 x 512 x 8 x 64 float32 (V = 4): forward 17.4 with two and three, 19.5 with four and two.
 template <int V, bool GRAD>
-constexpr int kAhead = V == 1 ? 1 : (GRAD ? 1 : 2);
+constexpr int kAhead = V == 1 ? 1 : (V == 8 ? (GRAD ? 1 : 4) : 2);
 template <int V, bool GRAD>
-constexpr int kCtasPerSm = V == 8 && GRAD ? 2 : 3;
+constexpr int kCtasPerSm = V == 8 || GRAD ? 2 : 3;
 
 // cos and sin of `turns` whole turns, |turns| <= 1/2. 16-bit results: the hardware's functions, off by at most 2^-21 on
 // [-pi, pi], far below half a step.
@@ -437,7 +483,7 @@ sdtw_status run(RotArgs& a, void* dweight, cudaStream_t s)
     // A unit is a token, unless that leaves the groups with few and unequal shares of them: then parts of one.
     const int64_t groups = static_cast<int64_t>(sms) * kCtasPerSm<kWide, GRAD> * (kThreads / G);
     a.hpu = a.H;
-    while (a.hpu > 2 && a.tokens * ((a.H + a.hpu - 1) / a.hpu) < 8 * groups) a.hpu = (a.hpu + 3) / 4 * 2;
+    while (a.hpu > 4 && a.tokens * ((a.H + a.hpu - 1) / a.hpu) < 8 * groups) a.hpu = (a.hpu + 7) / 8 * 4;
     if (a.tokens * a.H < groups) a.hpu = 1;
     a.token_units = (a.H + a.hpu - 1) / a.hpu;
     const int64_t units = a.tokens * a.token_units;
