@@ -3,6 +3,9 @@ that follow from the roundings the kernels make (sequence_plain.py), at the size
 calling where they can go wrong."""
 
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -236,6 +239,15 @@ def test_bad_lengths_are_reported(cuda, shape, dtype):
             T.check_errors(cuda)
 
 
+@pytest.mark.parametrize("N", [3, 150])
+def test_a_band_wider_than_the_series_is_none(cuda, N):
+    t, lx, ly = make((2, N, 170, 2, 2, 64, -1), torch.bfloat16, 73, True)
+    want = run(t, lx, ly, -1)
+    for bw in (170, 2**40, 2**63 - 1):
+        got = run(t, lx, ly, bw)
+        assert all(torch.equal(got[n], want[n]) for n in want)
+
+
 def test_int32_and_mixed_lengths(cuda):
     t, lx, ly = make((3, 40, 50, 2, 2, 32, 6), torch.float32, 19, True)
     want = run(t, lx, ly, 6)
@@ -369,6 +381,18 @@ def test_differences(cuda):
         assert abs(D[1] - slope) <= 2 * abs(D[0] - D[1]) + noise + slack, name
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+def test_first_gradient_of_a_process(cuda, dtype):
+    """The first gradient of a process, whose thread has made no CUDA call before."""
+    code = ("import torch, torchsoftdtw_b200 as T; x = torch.randn(1, 200, 2, 64, device='cuda', dtype=torch." + dtype + ")"
+            ".requires_grad_(True); g, = torch.autograd.grad(T.cross_attention(x, x, x).float().sum(), x); "
+            "y = T.norm_rotate(x); h, = torch.autograd.grad(y.float().sum(), x); "
+            "assert bool(g.isfinite().all() and h.isfinite().all())")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
 def test_only_the_wanted_gradients(cuda):
     t, lx, ly = make((1, 5, 6, 2, 2, 16, -1), torch.float32, 53, False)
     k = t[1].detach().requires_grad_(True)
@@ -432,4 +456,34 @@ def test_a_training_step_together(cuda):
     factor = min(1.0, 0.5 / (exact.item() + 1e-6))
     for p, gr in zip(params, grads):
         torch.testing.assert_close(p.grad, (gr.double() * factor).float(), rtol=2**-20, atol=0)
+    T.check_errors(cuda)
+
+
+@pytest.mark.parametrize("which,name", [(1, "out"), (2, "dq"), (3, "dk")])
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_wait_that_runs_out_ends_the_kernel(cuda, d, which, name):
+    """One warp of the first CTA withholds an arrival: the waits behind it end at their limit, its rows are NaN, the others'
+    right, the error is reported, and the next call is right."""
+    lib = _ext.capi()
+    T.check_errors(cuda)
+    t, lx, ly = make((2, 700, 650, 2, 2, d, -1), torch.bfloat16, 71, False)
+    want = run(t, lx, ly, -1)
+    torch.cuda.synchronize()
+    lib.sdtw_set_wait_timeout(0.2)
+    try:
+        if which > 1:  # the forward as usual
+            leaves = [x.detach().requires_grad_(True) for x in t[:3]]
+            out = T.cross_attention(*leaves)
+        lib.sdtw_debug_attention_stall(which)
+        got = dict(zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, t[3]))) if which > 1 else run(t, lx, ly, -1, grads=False)
+        torch.cuda.synchronize()
+    finally:
+        lib.sdtw_debug_attention_stall(0)
+        lib.sdtw_set_wait_timeout(2.0)
+    assert got[name][0, 0, 0].isnan().all()  # the first CTA's: sample 0, head 0, first rows
+    assert torch.equal(got[name][1], want[name][1]) and torch.equal(got[name][0, :, 1], want[name][0, :, 1])
+    with pytest.raises(RuntimeError, match="timed out"):
+        T.check_errors(cuda)
+    again = run(t, lx, ly, -1)
+    assert all(torch.equal(again[n], want[n]) for n in want)
     T.check_errors(cuda)

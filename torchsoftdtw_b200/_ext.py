@@ -119,6 +119,7 @@ class TensorRef(ctypes.Structure):
 # Test and tuning hooks (declared in the .cu, not part of the public header).
 DEBUG_SIGNATURES: dict[str, tuple] = {
     "sdtw_debug_inject_stall": (None, [_i]),
+    "sdtw_debug_attention_stall": (None, [_i]),
     "sdtw_debug_force_path": (None, [_i]),
     "sdtw_debug_set_pair_warps": (None, [_i]),
     "sdtw_debug_kernel_launches": (ctypes.c_uint64, []),

@@ -13,12 +13,12 @@ namespace sdtw {
 namespace {
 
 constexpr int kDMax = 128;
+constexpr int64_t kMost = 1 << 24;  // rows of a sample, and samples
 
 sdtw_status checked(const sdtw_attention_problem* p)
 {
     if (p == nullptr) return SDTW_EINVAL;
     if (p->dtype != SDTW_F32 && p->dtype != SDTW_F16 && p->dtype != SDTW_BF16) return SDTW_EDTYPE;
-    constexpr int64_t kMost = 1 << 24;  // rows of a sample, heads and samples are counted in 32 bits
     if (p->B < 0 || p->N < 0 || p->M < 0 || p->Hq < 1 || p->Hkv < 1 || p->Hq % p->Hkv != 0) return SDTW_EINVAL;
     if (p->B > kMost || p->N > kMost || p->M > kMost || p->Hq > 65535 || p->d < 1 || p->d > kDMax) return SDTW_EINVAL;
     if (static_cast<double>(p->B) * static_cast<double>(p->Hq) * static_cast<double>(p->N + p->M + 256) > 2e9)
@@ -50,7 +50,8 @@ AttnArgs args_of(const sdtw_attention_problem* p)
     a.group = a.Hq / a.Hkv;
     a.lx = {p->lengths_x, p->lengths_int32};
     a.ly = {p->lengths_y, p->lengths_int32};
-    a.bw = p->bandwidth;
+    // A band as wide as the longer series holds every cell; wider ones would only overflow its products.
+    a.bw = p->bandwidth < kMost ? p->bandwidth : kMost;
     a.scale = static_cast<float>(p->scale);
     a.scale_log2 = static_cast<float>(p->scale * 1.4426950408889634);
     a.err = p->err_word;

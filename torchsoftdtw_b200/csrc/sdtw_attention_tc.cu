@@ -58,6 +58,7 @@ struct FwdArgs {
     int tiles;     // CTAs a head: ceil(N / (128 NT))
     int dn;        // d rounded up to 16: columns of O
     int negative;  // scale < 0: the scores change sign
+    int stall;     // attention_stall() == 1
 };
 
 template <typename T, int DPAD, int NT>
@@ -367,7 +368,7 @@ __global__ void __launch_bounds__(Geom<DPAD, NT>::THREADS, NT == 1 ? 2 : 1)
             wait_st();
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_full + 16 * w + 8 * (it & 1));
+            if (lane == 0 && !(f.stall && blockIdx.x == 0 && warp == 0 && it == 0)) mbar_arrive(p_full + 16 * w + 8 * (it & 1));
         }
         // (Not pv_full: PV products of this tile and the one before may both have completed by now, or neither, and a
         // parity tells a phase only from its neighbours.)
@@ -466,6 +467,8 @@ cudaError_t launch_forward(FwdArgs& f, const CUtensorMap& mq, const CUtensorMap&
 template <typename T>
 cudaError_t forward_t(const AttnArgs& a, cudaStream_t s)
 {
+    const cudaError_t bound = attention_bind_context();
+    if (bound != cudaSuccess) return bound;
     CUtensorMap mq, mk, mv;
     constexpr bool half = std::is_same<T, __half>::value;
     if (!attention_tile_map(&mq, half, a.q, a.qs, a.B, a.N, a.Hq, a.d, kTile) ||
@@ -477,12 +480,25 @@ cudaError_t forward_t(const AttnArgs& a, cudaStream_t s)
     f.timeout_ns = static_cast<uint64_t>(wait_timeout_s() * 1e9);
     f.dn = (a.d + 15) / 16 * 16;
     f.negative = a.scale_log2 < 0;
+    f.stall = attention_stall() == 1;
     f.a.scale_log2 = fmaxf(fabsf(a.scale_log2), 1e-30f);  // a scale of zero: all scores equal
     if (a.d <= 64) return launch_forward<T, 64, 1>(f, mq, mk, mv, s);
     return launch_forward<T, 128, 2>(f, mq, mk, mv, s);
 }
 
 }  // namespace
+
+namespace {
+std::atomic<int> g_stall{0};
+}
+int attention_stall() { return g_stall.load(std::memory_order_relaxed); }
+
+cudaError_t attention_bind_context()
+{
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    return e == cudaSuccess ? cudaSetDevice(dev) : e;
+}
 
 bool attention_tile_map(CUtensorMap* map, bool half, const void* ptr, const Strides& st, int64_t B, int64_t rows, int64_t H,
                         int64_t d, int box_rows)
@@ -513,3 +529,6 @@ cudaError_t attention_tc_forward(const AttnArgs& a, bool bf16, cudaStream_t s)
 }
 
 }  // namespace sdtw
+
+// Test hook (see attention_stall).
+extern "C" void sdtw_debug_attention_stall(int which) { sdtw::g_stall.store(which); }

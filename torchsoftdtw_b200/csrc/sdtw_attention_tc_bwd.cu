@@ -37,6 +37,7 @@ struct BwdArgs {
     uint64_t timeout_ns;
     int tiles;        // CTAs a head
     int dn;           // d rounded up to 16
+    int stall;        // attention_stall()
     uint32_t* peak;   // fp16: (B, Hkv) bits of the largest |do|^2 of the head's rows
 };
 
@@ -443,7 +444,7 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
             wait_st();
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(ds_full + 8 * x);
+            if (lane == 0 && !(f.stall == 2 && blockIdx.x == 0 && warp == 0 && it == 0)) mbar_arrive(ds_full + 8 * x);
         }
         if (ok && n > 0) ok = mbar_wait(acc_full, 0, bound);
         fence_after();
@@ -668,7 +669,7 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
             wait_st();
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_full + 8 * x);
+            if (lane == 0 && !(f.stall == 3 && blockIdx.x == 0 && warp == 0 && it == 0)) mbar_arrive(p_full + 8 * x);
             if (!(ok = mbar_wait(dp_full + 8 * x, phase, bound))) break;
             fence_after();
             tmem_ld32(tdp, p);
@@ -726,7 +727,8 @@ cudaError_t backward_d(BwdArgs& f, cudaStream_t s)
     // As rows of a product (128 a tile) and as columns (64 a tile).
     CUtensorMap q_rows, g_rows, k_cols, v_cols, k_rows, v_rows, q_cols, g_cols;
     const cudaError_t bad = cudaErrorInvalidValue;
-    cudaError_t e;
+    cudaError_t e = attention_bind_context();
+    if (e != cudaSuccess) return e;
     if (a.N > 0 && a.M > 0) {
         if (!attention_tile_map(&q_rows, half, a.q, a.qs, a.B, a.N, a.Hq, a.d, kTile) ||
             !attention_tile_map(&g_rows, half, a.dout, a.gs, a.B, a.N, a.Hq, a.d, kTile) ||
@@ -765,6 +767,7 @@ cudaError_t attention_tc_backward(const AttnArgs& a, bool bf16, uint32_t* peak, 
     f.timeout_ns = static_cast<uint64_t>(wait_timeout_s() * 1e9);
     f.dn = (a.d + 15) / 16 * 16;
     f.peak = peak;
+    f.stall = attention_stall();
     if (bf16) return a.d <= 64 ? backward_d<__nv_bfloat16, 64>(f, s) : backward_d<__nv_bfloat16, 128>(f, s);
     return a.d <= 64 ? backward_d<__half, 64>(f, s) : backward_d<__half, 128>(f, s);
 }
