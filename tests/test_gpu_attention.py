@@ -487,3 +487,24 @@ def test_a_wait_that_runs_out_ends_the_kernel(cuda, d, which, name):
     again = run(t, lx, ly, -1)
     assert all(torch.equal(again[n], want[n]) for n in want)
     T.check_errors(cuda)
+
+
+@pytest.mark.parametrize("B,N,M,Hq,Hkv,d", [(2, 300, 300, 4, 2, 128), (1, 4000, 1000, 2, 1, 16), (2, 300, 2000, 4, 4, 64),
+                                            (1, 20, 30000, 4, 4, 128), (2, 1, 4000, 8, 2, 128)])
+def test_float32_over_long_sums(cuda, B, N, M, Hq, Hkv, d):
+    """Relative error over an output's elements, where roundings of one sign would add up.
+
+    An operand in two parts is off by 2^-24, the dropped product of tails by 2^-24: a product by 2^-22.4, and by a third
+    of that as a root mean square over operands. A score adds the same to its weight's exponent (scores have a standard
+    deviation of 1.5). A sum of n parts in 32 bits adds half of 2^-24 n^(1/2) at most where roundings have either sign:
+    2^-20.6 for n = 940 tiles (30000 states). Five such terms in squares stay below 2^-19.
+    """
+    t, lx, ly = make((B, N, M, Hq, Hkv, d, -1), torch.float32, 81, False)
+    got = run(t, lx, ly, -1, given=False)
+    q, k, v, dout = [x.double().detach().requires_grad_() for x in t]
+    kk, vv = [x.repeat_interleave(Hq // Hkv, 2) for x in (k, v)]
+    p = (torch.einsum("bnhd,bmhd->bhnm", q, kk) * d**-0.5).softmax(-1)
+    out = torch.einsum("bhnm,bmhd->bnhd", p, vv)
+    want = dict(zip(("dq", "dk", "dv"), torch.autograd.grad(out, (q, k, v), dout)), out=out.detach())
+    for name, w in want.items():
+        assert ((got[name].double() - w).norm() / w.norm()).item() <= 2**-19, name

@@ -2,7 +2,10 @@
 // alignment.
 //
 // Fragments (one m16n8 accumulator c: rows lane / 4 and + 8, columns 2 (lane % 4) and + 1): 16-bit operands by m16n8k16,
-// float32 as three TF32 products m16n8k8 of an 11-bit head and tail (x = head + tail to 2^-22; tail.tail is dropped).
+// float32 as three TF32 products m16n8k8 of an 11-bit head and tail (x = head + tail to 2^-23; tail.tail is dropped). The
+// matrix pipe's adder cuts off where an add in 32 bits rounds, an error of one sign for each instruction that a sum goes
+// through. So at most four head products follow one another before their sum is added to the total by an ordinary add, and
+// the tails' products have a sum of their own, 2^-11 of the heads'.
 #pragma once
 
 #include <type_traits>
@@ -25,10 +28,18 @@ __device__ __forceinline__ void split2(float x, uint32_t& head, uint32_t& tail)
 }
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <int NB>
+__device__ __forceinline__ void add(float (&c)[NB][4], const float (&x)[NB][4])
+{
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[i][e] += x[i][e];
 }
 template <typename T>
 __device__ __forceinline__ void mma_16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
@@ -93,23 +104,30 @@ __device__ __forceinline__ void product_rows(float (&c)[NB][4], const T* A, cons
     } else {
         const float* ar = A + (lane >> 2) * LD + (lane & 3);
         const float* br = B + (lane >> 2) * LD + (lane & 3);
-#pragma unroll 4
-        for (int k = 0; k < DPAD; k += 8) {
-            uint32_t ah[4], al[4];
-            split2(ar[k], ah[0], al[0]);
-            split2(ar[8 * LD + k], ah[1], al[1]);
-            split2(ar[k + 4], ah[2], al[2]);
-            split2(ar[8 * LD + k + 4], ah[3], al[3]);
+        float tails[NB][4] = {};
+#pragma unroll 1
+        for (int k0 = 0; k0 < DPAD; k0 += 32) {
+            float heads[NB][4] = {};
 #pragma unroll
-            for (int x = 0; x < NB; ++x) {
-                uint32_t bh[2], bl[2];
-                split2(br[8 * x * LD + k], bh[0], bl[0]);
-                split2(br[8 * x * LD + k + 4], bh[1], bl[1]);
-                mma_tf32(c[x], al, bh[0], bh[1]);
-                mma_tf32(c[x], ah, bl[0], bl[1]);
-                mma_tf32(c[x], ah, bh[0], bh[1]);
+            for (int k = k0; k < k0 + 32; k += 8) {
+                uint32_t ah[4], al[4];
+                split2(ar[k], ah[0], al[0]);
+                split2(ar[8 * LD + k], ah[1], al[1]);
+                split2(ar[k + 4], ah[2], al[2]);
+                split2(ar[8 * LD + k + 4], ah[3], al[3]);
+#pragma unroll
+                for (int x = 0; x < NB; ++x) {
+                    uint32_t bh[2], bl[2];
+                    split2(br[8 * x * LD + k], bh[0], bl[0]);
+                    split2(br[8 * x * LD + k + 4], bh[1], bl[1]);
+                    mma_tf32(tails[x], al, bh[0], bh[1]);
+                    mma_tf32(heads[x], ah, bh[0], bh[1]);
+                    mma_tf32(tails[x], ah, bl[0], bl[1]);
+                }
             }
+            add(c, heads);
         }
+        add(c, tails);
     }
 }
 
@@ -134,22 +152,29 @@ __device__ __forceinline__ void product_columns(float (&o)[DPAD / 8][4], const f
     } else {
         // The accumulator's columns 2t, 2t + 1 serve as the operand's K = t, t + 4; B's rows are taken in that order.
         const float* br = B + 2 * (lane & 3) * LD + (lane >> 2);
+        static_assert(NB <= 4, "four head products a sum");
+        uint32_t ah[NB][4], al[NB][4];
 #pragma unroll
         for (int x = 0; x < NB; ++x) {
-            uint32_t ah[4], al[4];
-            split2(s[x][0], ah[0], al[0]);
-            split2(s[x][2], ah[1], al[1]);
-            split2(s[x][1], ah[2], al[2]);
-            split2(s[x][3], ah[3], al[3]);
+            split2(s[x][0], ah[x][0], al[x][0]);
+            split2(s[x][2], ah[x][1], al[x][1]);
+            split2(s[x][1], ah[x][2], al[x][2]);
+            split2(s[x][3], ah[x][3], al[x][3]);
+        }
 #pragma unroll
-            for (int y = 0; y < DPAD / 8; ++y) {
+        for (int y = 0; y < DPAD / 8; ++y) {
+            float heads[4] = {}, tails[4] = {};
+#pragma unroll
+            for (int x = 0; x < NB; ++x) {
                 uint32_t bh[2], bl[2];
                 split2(br[8 * x * LD + 8 * y], bh[0], bl[0]);
                 split2(br[(8 * x + 1) * LD + 8 * y], bh[1], bl[1]);
-                mma_tf32(o[y], al, bh[0], bh[1]);
-                mma_tf32(o[y], ah, bl[0], bl[1]);
-                mma_tf32(o[y], ah, bh[0], bh[1]);
+                mma_tf32(tails, al[x], bh[0], bh[1]);
+                mma_tf32(heads, ah[x], bh[0], bh[1]);
+                mma_tf32(tails, ah[x], bl[0], bl[1]);
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[y][e] += heads[e] + tails[e];
         }
     }
 }
