@@ -82,8 +82,8 @@ def clip_grad_norm_(
     norm_type: float = 2.0,
     error_if_nonfinite: bool = False,
 ) -> torch.Tensor:
-    """Clip the gradients of the parameters in place by their global norm; the counterpart of
-    ``torch.nn.utils.clip_grad_norm_`` on this library's kernels.
+    """Clip the gradients of the parameters in place by their global norm, for a training loop
+    between the backward pass and the optimizer's step.
 
     Args:
         parameters: a tensor or an iterable of tensors; those without a gradient are passed over.

@@ -3,6 +3,8 @@
 // like them without atomics on results. One kernel serves both: the tile's rows (Q, dO; or K, V) stay in shared memory, 16 a
 // warp, and the other side streams past in tiles of TC rows:
 //   S = X1 Y1^T, dP = X2 Y2^T;   dq: sum dS Y1;   dk: sum dS Y1, dv: sum P Y2.
+// float32 is bound by the instructions that split operands into heads and tails, once for each use: 64 x 256 x 192 x 4 x 32,
+// band 32, 138 us; 2 x 2048 x 2048 x 8 x 128 3.55 ms, 34 TFLOP/s of the seven products.
 #include "sdtw_attention_mma.cuh"
 #include "sdtw_attention_split.h"
 

@@ -10,6 +10,10 @@
 // tiles are in flight on an SM: of two CTAs (d <= 64), or of one that has two groups of elementwise warps and two sets of S and
 // dP in tensor memory, for the even and the odd tiles (BUFS = 2).
 //
+// Bound, like the forward, by the elementwise step between products: 2 x 4096 x 4096 x 16 x 128 bf16 960 us (1000 TFLOP/s
+// of the seven products), 4 x 4096 x 4096 x 16 x 64 1023 us, 32 x 512 x 512 x 8 x 64 120 us, where the CTAs' first loads,
+// of all SMs at once, take a third of the time. Sums of the tile before placed between S and dP: 10% slower.
+//
 // fp16: P is kept 2^10 larger and dS scaled by a power of two that brings the rows' |do| to [8, 16) (a row's own in
 // dq, where a row is a lane; the largest of the head in dk), so that neither under- nor overflows where the gradients do not.
 #include <mutex>
@@ -213,7 +217,11 @@ __device__ __forceinline__ void mma_cols(uint32_t d, uint32_t a, uint32_t half, 
         mma_ts(d, a + (k / 2) * half + (k % 2) * 8, desc_at(cd, 2048 * k), idesc, more || k > 0, leader);
 }
 
-template <typename T, int DPAD>
+// TAIL (d <= 32): what the rounding of dS dropped goes through a second product. With few features the scores' tails are heavier
+// and a few large dS carry dq, whose rounding nothing averages: without it dq is off by 1.6 times its own rounding at
+// d = 16 (1.4 from d = 64 on), with it by 1.1 times; 4 x 4096 x 4096 x 16 x 16 1.04 -> 1.16 ms. At d <= 32 tensor memory has room
+// for it beside the narrow sum.
+template <typename T, int DPAD, bool TAIL>
 __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
     attend_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mg,
                         const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
@@ -222,8 +230,9 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
     using G = Geom<DPAD>;
     // Each buffer: S, dP, dS.
     constexpr uint32_t DP_COL = kCols, DS_COL = 2 * kCols, BUF_COLS = 2 * kCols + kCols / 2, ACC_COL = G::BUFS * BUF_COLS;
-    constexpr uint32_t TMEM_COLS = ACC_COL + DPAD <= 256 ? 256 : 512;
-    static_assert(ACC_COL + DPAD <= 512, "tensor memory");
+    constexpr uint32_t TAIL_COL = ACC_COL + DPAD, ALL_COLS = TAIL_COL + (TAIL ? kCols / 2 : 0);
+    constexpr uint32_t TMEM_COLS = ALL_COLS <= 256 ? 256 : 512;
+    static_assert(ALL_COLS <= 512 && (!TAIL || G::BUFS == 1), "tensor memory");
     const AttnArgs& a = f.a;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* sm = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
@@ -322,6 +331,7 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
                 if (!mbar_wait(ds_full + 8 * x, (i / G::BUFS) & 1, bound)) return false;
                 fence_after();
                 mma_cols<DPAD>(tmem + ACC_COL, tmem + x * BUF_COLS + DS_COL, 16, ring(now.at, 0), idesc_q, i > 0, leader);
+                if constexpr (TAIL) mma_cols<DPAD>(tmem + ACC_COL, tmem + TAIL_COL, 16, ring(now.at, 0), idesc_q, true, leader);
                 mma_commit(ds_free + 8 * x, leader);
                 mma_commit(empty + 8 * now.at, leader);
                 now.next();
@@ -430,17 +440,23 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(dp_free + 8 * x);
-            uint32_t w[16];
+            uint32_t w[16], wt[TAIL ? 16 : 1];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const float p0 = __uint_as_float(p[2 * e]), p1 = __uint_as_float(p[2 * e + 1]);
                 const float d0 = is_half<T> ? fmaf(p0, cf, -delta) : p0 - delta;
                 const float d1 = is_half<T> ? fmaf(p1, cf, -delta) : p1 - delta;
-                w[e] = pack2(__uint_as_float(s[2 * e]) * d0, __uint_as_float(s[2 * e + 1]) * d1, T());
+                const float v0 = __uint_as_float(s[2 * e]) * d0, v1 = __uint_as_float(s[2 * e + 1]) * d1;
+                w[e] = pack2(v0, v1, T());
+                if constexpr (TAIL) {
+                    const Vec<T, 2> head = *reinterpret_cast<const Vec<T, 2>*>(&w[e]);
+                    wt[e] = pack2(v0 - to_f(head.e[0]), v1 - to_f(head.e[1]), T());
+                }
             }
             if (it >= G::BUFS && !(ok = mbar_wait(ds_free + 8 * x, phase ^ 1, bound))) break;
             fence_after();
             tmem_st16(tds, w);
+            if constexpr (TAIL) tmem_st16(tds + (TAIL_COL - DS_COL), wt);
             wait_st();
             fence_before();
             __syncwarp();
@@ -744,11 +760,13 @@ cudaError_t backward_d(BwdArgs& f, cudaStream_t s)
         e = cudaMemsetAsync(f.peak, 0, sizeof(uint32_t) * static_cast<size_t>(a.B) * a.Hkv, s);
         if (e != cudaSuccess) return e;
     }
-    static std::atomic<bool> allowed[2][128];
-    if ((e = allow_smem(attend_dq_tc_kernel<T, DPAD>, G::BYTES, allowed[0])) != cudaSuccess) return e;
+    static std::atomic<bool> allowed[3][128];
+    const bool tail = DPAD == 64 && a.d <= 32;
+    const auto dq = tail ? attend_dq_tc_kernel<T, DPAD, DPAD == 64> : attend_dq_tc_kernel<T, DPAD, false>;
+    if ((e = allow_smem(dq, G::BYTES, allowed[tail ? 2 : 0])) != cudaSuccess) return e;
     if ((e = allow_smem(attend_dkdv_tc_kernel<T, DPAD>, G::BYTES, allowed[1])) != cudaSuccess) return e;
     f.tiles = static_cast<int>((a.N + kTile - 1) / kTile);
-    attend_dq_tc_kernel<T, DPAD><<<static_cast<unsigned>(static_cast<int64_t>(a.B) * a.Hq * f.tiles), G::THREADS, G::BYTES, s>>>(
+    dq<<<static_cast<unsigned>(static_cast<int64_t>(a.B) * a.Hq * f.tiles), G::THREADS, G::BYTES, s>>>(
         q_rows, g_rows, k_cols, v_cols, f);
     count_launch();
     f.tiles = static_cast<int>((a.M + kTile - 1) / kTile);
