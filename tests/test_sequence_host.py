@@ -163,3 +163,18 @@ def test_fake_kernels():
         assert T.norm_rotate(q, w).shape == q.shape
         norm = torch.ops.torchsoftdtw_b200.global_norm([q, w.double()], 2.0)
         assert norm.dtype == torch.float64 and norm.dim() == 0
+
+
+def test_forward_mode_is_refused():
+    """A tangent would otherwise be dropped without a word."""
+    import torch.autograd.forward_ad as fwad
+
+    x = torch.randn(1, 2, 1, 8)
+    with fwad.dual_level():
+        d = fwad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            T.cross_attention(d, x, x)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            T.norm_rotate(d)
+        with pytest.raises(RuntimeError, match="forward-mode"), torch.no_grad():
+            T.norm_rotate(x, fwad.make_dual(torch.ones(8), torch.ones(8)))

@@ -73,8 +73,9 @@ def cross_attention(
     Returns:
         out: (B, N, Hq, d), contiguous, in q's dtype. Rows at or past ``lengths_x`` (and all rows of a sample whose
         ``lengths_y`` is 0) are zero and have no gradient. Rows of q, k and v past the lengths are not used: they
-        may hold anything, NaN included. A length outside [0, N] / [0, M] makes the sample's rows NaN (its
-        gradients zero) and is reported by :func:`check_errors`.
+        may hold anything, NaN included; a NaN or infinity inside the lengths may reach every row of its sample. A
+        length outside [0, N] / [0, M] makes the sample's rows NaN (its gradients zero) and is reported by
+        :func:`check_errors`.
     """
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1]) if q.dim() > 0 and q.shape[-1] > 0 else 1.0

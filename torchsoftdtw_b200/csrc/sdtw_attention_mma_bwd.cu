@@ -21,7 +21,8 @@ constexpr bool is_half = std::is_same<T, __half>::value;
 template <typename T, int DPAD>
 struct Geom {
     static constexpr int TC = sizeof(T) == 4 && DPAD == 128 ? 16 : 32;
-    static constexpr int CTAS = sizeof(T) == 4 && DPAD == 32 ? 4 : 2;  // an SM: fp32, d = 32: 144 -> 136 us; d = 128: 3.69 -> 3.54 ms
+    // CTAs an SM, registers given up for them: fp32, d = 32: 144 -> 136 us; d = 128: 3.69 -> 3.54 ms
+    static constexpr int CTAS = sizeof(T) == 4 && DPAD == 32 ? 4 : 2;
     static constexpr int UNIT = 16 / sizeof(T);
     static constexpr int LD = DPAD + UNIT;
     static constexpr int STAGES = 2;

@@ -2,8 +2,9 @@
 //
 // The N group query rows that read one key head are packed (row r is query r / group of head r % group): a CTA takes
 // ROWS of them and one split of the states that their cells touch. K and V stream through a ring of cp.async tiles;
-// products are warp-level mma (16-bit operands m16n8k16; float32 as three TF32 products of heads and tails). With ROWS = 16 the four warps take different states of each tile and join at the end; with
-// ROWS = 64 each takes its own 16 rows and all states.
+// products are warp-level mma (16-bit operands m16n8k16; float32 as three TF32 products of heads and tails). With
+// ROWS = 16 the four warps take different states of each tile and join at the end; with ROWS = 64 each takes its own 16 rows
+// and all states.
 //
 // Few rows are bound by reading K and V once, so the rows of a padded mma cost nothing; the splits exist to have every SM
 // read. Up to eight splits form a cluster and join their sums through distributed shared memory, in one launch; more

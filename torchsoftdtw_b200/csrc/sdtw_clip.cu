@@ -6,8 +6,8 @@
 // CTA, the second combines the partials in every CTA (in one fixed order, so each run and each CTA gets the
 // same bits) and scales. Tensors are cut into chunks of 64 KB, or less where there would be fewer than four chunks a
 // CTA; CTA c takes chunks c, c + grid, and the second launch walks them backwards, so that what the first one read last is
-// still in L2: 252 million bf16 (504 MB) 252 us in place, 6.0 TB/s of its 1.51 GB; 231 us is a copy's rate for them. Few small tensors are
-// bound by the two launches: 25 tensors, 0.4 MB, 19 us a call with the host's part.
+// still in L2: 252 million bf16 (504 MB) 252 us in place, 6.0 TB/s of its 1.51 GB; 231 us is a copy's rate for them.
+// Few small tensors are bound by the two launches: 25 tensors, 0.4 MB, 19 us a call with the host's part.
 #include <cmath>
 #include <cstring>
 

@@ -519,12 +519,16 @@ const auto& norm_rotate_backward_op()
 
 OptTensor optional_of(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 Tensor tensor_of(const OptTensor& t) { return t ? *t : Tensor(); }
-bool wants_grad(std::initializer_list<Tensor> ts)
+// Whether a call belongs to a graph. Forward-mode tangents are refused rather than dropped.
+bool wants_grad(const char* name, std::initializer_list<Tensor> ts)
 {
-    if (!at::GradMode::is_enabled()) return false;
-    for (const Tensor& t : ts)
-        if (t.defined() && t.requires_grad()) return true;
-    return false;
+    bool wants = false;
+    for (const Tensor& t : ts) {
+        if (!t.defined()) continue;
+        TORCH_CHECK(!t._fw_grad(0).defined(), name, " has no forward-mode derivative");
+        wants = wants || t.requires_grad();
+    }
+    return wants && at::GradMode::is_enabled();
 }
 
 // The gradients themselves are not differentiable: differentiating them raises.
@@ -551,7 +555,7 @@ std::tuple<Tensor, Tensor, Tensor> attention_backward_autograd(const Tensor& dou
                                                                const Tensor& lse, const OptTensor& lx, const OptTensor& ly,
                                                                int64_t bandwidth, double scale)
 {
-    if (wants_grad({dout, q, k, v, out})) {
+    if (wants_grad("cross_attention", {dout, q, k, v, out})) {
         const variable_list g = AttentionBackward::apply(dout, q, k, v, out, out_lo, lse, lx, ly, bandwidth, scale);
         return {g[0], g[1], g[2]};
     }
@@ -583,7 +587,7 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
 Tensor cross_attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& lx, const OptTensor& ly,
                                 int64_t bandwidth, double scale)
 {
-    if (wants_grad({q, k, v})) return CrossAttention::apply(q, k, v, lx, ly, bandwidth, scale);
+    if (wants_grad("cross_attention", {q, k, v})) return CrossAttention::apply(q, k, v, lx, ly, bandwidth, scale);
     at::AutoDispatchBelowADInplaceOrView guard;
     return cross_attention_op().call(q, k, v, lx, ly, bandwidth, scale);
 }
@@ -606,7 +610,7 @@ std::tuple<Tensor, Tensor> norm_rotate_backward_autograd(const Tensor& dy, const
                                                          int64_t rotary, double base, bool interleaved, double eps,
                                                          bool need_weight)
 {
-    if (wants_grad({dy, x, tensor_of(weight)})) {
+    if (wants_grad("norm_rotate", {dy, x, tensor_of(weight)})) {
         const variable_list g = NormRotateBackward::apply(dy, x, weight, lengths, positions, rotary, base, interleaved, eps,
                                                           need_weight);
         return {g[0], g[1]};
@@ -644,7 +648,7 @@ struct NormRotate : torch::autograd::Function<NormRotate> {
 Tensor norm_rotate_autograd(const Tensor& x, const OptTensor& weight, const OptTensor& lengths, const OptTensor& positions,
                             int64_t rotary, double base, bool interleaved, double eps)
 {
-    if (wants_grad({x, tensor_of(weight)}))
+    if (wants_grad("norm_rotate", {x, tensor_of(weight)}))
         return NormRotate::apply(x, weight, lengths, positions, rotary, base, interleaved, eps);
     at::AutoDispatchBelowADInplaceOrView guard;
     return norm_rotate_op().call(x, weight, lengths, positions, rotary, base, interleaved, eps);
