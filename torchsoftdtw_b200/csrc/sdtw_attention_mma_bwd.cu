@@ -4,7 +4,7 @@
 // warp, and the other side streams past in tiles of TC rows:
 //   S = X1 Y1^T, dP = X2 Y2^T;   dq: sum dS Y1;   dk: sum dS Y1, dv: sum P Y2.
 // float32 is bound by the instructions that split operands into heads and tails, once for each use: 64 x 256 x 192 x 4 x 32,
-// band 32, 138 us; 2 x 2048 x 2048 x 8 x 128 3.55 ms, 34 TFLOP/s of the seven products.
+// band 32, 135 us; 2 x 2048 x 2048 x 8 x 128 3.55 ms, 34 TFLOP/s of the seven products.
 #include "sdtw_attention_mma.cuh"
 #include "sdtw_attention_split.h"
 
@@ -189,6 +189,9 @@ __global__ void __launch_bounds__(kThreads, Geom<T, DPAD>::CTAS) attend_backward
         const T* y2 = y1 + G::TILE;
         const float* st = col_stat + t % G::STAGES * 2 * G::TC;
         const int64_t c = c0 + static_cast<int64_t>(KV ? t % per_head : t) * G::TC;
+        // A warp passes over tiles without a cell of its rows (those of a band are not those of its CTA).
+        const bool some = (c < hi[0] && c + G::TC > lo[0]) || (c < hi[1] && c + G::TC > lo[1]);
+        if (!__any_sync(kFull, some)) continue;
         float s[G::TC / 8][4], dp[G::TC / 8][4];
 #pragma unroll
         for (int x = 0; x < G::TC / 8; ++x)

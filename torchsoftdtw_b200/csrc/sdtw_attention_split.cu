@@ -196,6 +196,9 @@ __global__ void __launch_bounds__(kThreads, Geom<T, DPAD, ROWWARPS>::CTAS) atten
         const T* kt = ring + (t - t0) % G::STAGES * 2 * G::TILE + kw * G::NK * G::LD;
         const T* vt = kt + G::TILE;
         const int64_t jw = j0 + static_cast<int64_t>(t) * G::TK + kw * G::NK;  // this warp's first state
+        // A warp passes over tiles without a cell of its rows (those of a band are not those of its CTA).
+        const bool cells = (jw < hi[0] && jw + G::NK > lo[0]) || (jw < hi[1] && jw + G::NK > lo[1]);
+        if (!__any_sync(kFull, cells)) continue;
         float s[G::NK / 8][4];
 #pragma unroll
         for (int x = 0; x < G::NK / 8; ++x)
