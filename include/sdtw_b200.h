@@ -283,7 +283,7 @@ sdtw_status sdtw_grad_dist(sdtw_dtype dtype, int kind, const void* X, const void
  * q, k and v past the lengths are not used and may hold anything, NaN included; a NaN or infinity inside the
  * lengths may reach every row of its sample.
  *   out (B, N, Hq, d), contiguous. lse (B, Hq, N) fp32 (optional, the backward needs it): log2 of the softmax denominator of s / ln 2 (-inf in
- *   empty rows). out_lo (optional, 16-bit types): what rounding out to its type dropped, out's type; the
+ *   empty rows). out_lo (optional, 16-bit types): what rounding out to its type dropped, out's type (SDTW_F16: 2^11 times that); the
  *   backward takes p . dp from out + out_lo, which keeps gradients exact where one state holds all the weight.
  *   A length outside [0, N] / [0, M] raises SDTW_ERR_BAD_LENGTH; that sample's rows are NaN, its gradients 0.
  *   backward: dout (B, N, Hq, d) with any strides; dq, dk, dv contiguous, each written in full, in one fixed

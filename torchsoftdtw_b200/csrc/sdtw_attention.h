@@ -1,6 +1,8 @@
 // The problem of one cross-attention call as the kernels see it.
 #pragma once
 
+#include <type_traits>
+
 #include "sdtw_sequence.cuh"
 
 namespace sdtw {
@@ -28,6 +30,11 @@ struct AttnArgs {
     void *dq, *dk, *dv;
     float* delta;  // (B, Hq, N): sum_j p_ij dp_ij
 };
+
+// What out_lo holds of an output's remainder (what rounding it to its type dropped): fp16's is kept 2^11 larger, about as large
+// as the output itself, for the remainders of outputs below 2^-3 end among fp16's subnormal numbers.
+template <typename T>
+constexpr float kLoScale = std::is_same<T, __half>::value ? 0x1p11f : 1.f;
 
 // The lengths of sample b, and whether one of them is out of range (reported; the sample is then empty).
 __device__ __forceinline__ bool pair_lengths(const AttnArgs& a, int64_t b, int64_t& nx, int64_t& ny)

@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, Geom<T, DPAD>::CTAS) attend_backward
                 for (int c = lane; c < a.d; c += 32) {
                     const float g = to_f(r2p[i * r2s.n + c]);
                     float o = to_f(static_cast<const T*>(a.o)[at + c]);
-                    if (a.o_lo) o += to_f(static_cast<const T*>(a.o_lo)[at + c]);
+                    if (a.o_lo) o = fmaf(to_f(static_cast<const T*>(a.o_lo)[at + c]), 1.f / kLoScale<T>, o);
                     dot = fmaf(g, o, dot);
                     nrm = fmaf(g, g, nrm);
                 }

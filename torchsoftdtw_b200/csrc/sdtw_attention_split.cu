@@ -78,7 +78,7 @@ __device__ __forceinline__ void store_out(const AttnArgs& a, int b, int hk, int6
     const int64_t at = ((static_cast<int64_t>(b) * a.N + n) * a.Hq + h) * a.d + f;
     const T y = from_f<T>(v);
     static_cast<T*>(a.out)[at] = y;
-    if (a.out_lo) static_cast<T*>(a.out_lo)[at] = from_f<T>(v - to_f(y));
+    if (a.out_lo) static_cast<T*>(a.out_lo)[at] = from_f<T>((v - to_f(y)) * kLoScale<T>);
 }
 __device__ __forceinline__ void store_lse(const AttnArgs& a, int b, int hk, int64_t r, float v)
 {

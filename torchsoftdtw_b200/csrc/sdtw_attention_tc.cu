@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(Geom<DPAD, NT>::THREADS, NT == 1 ? 2 : 1)
                         v[x] = pack2(v0, v1, T());
                         if (part == 1) {
                             const T* r = reinterpret_cast<const T*>(&v[x]);
-                            v[x] = pack2(v0 - to_f(r[0]), v1 - to_f(r[1]), T());
+                            v[x] = pack2((v0 - to_f(r[0])) * kLoScale<T>, (v1 - to_f(r[1])) * kLoScale<T>, T());
                         }
                     }
                     rows[lane * UPR + (((c + e) / 8) ^ (lane & 7))] = make_uint4(v[0], v[1], v[2], v[3]);

@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float gf = on ? to_f(g[t].e[e]) : 0.f;
-                    dot = on ? fmaf(gf, to_f(o[t].e[e]) + to_f(lo[t].e[e]), dot) : 0.f;
+                    dot = on ? fmaf(gf, fmaf(to_f(lo[t].e[e]), 1.f / kLoScale<T>, to_f(o[t].e[e])), dot) : 0.f;
                     nrm = fmaf(gf, gf, nrm);
                 }
 #pragma unroll
