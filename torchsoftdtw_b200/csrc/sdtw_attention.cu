@@ -6,6 +6,7 @@
 // C entry points' arguments and chooses the kernels.
 #include <cmath>
 
+#include "sdtw_attention_range.cuh"
 #include "sdtw_attention_split.h"
 #include "sdtw_attention_tc.h"
 
@@ -29,6 +30,8 @@ sdtw_status checked(const sdtw_attention_problem* p)
     if ((rows || states) && p->err_word == nullptr) return SDTW_EINVAL;
     return SDTW_OK;
 }
+
+int64_t peak_blocks(int64_t rows) { return (rows + kPeakRows - 1) / kPeakRows; }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
@@ -115,9 +118,11 @@ sdtw_status sdtw_cross_attention(const sdtw_attention_problem* p, void* out, voi
 
 size_t sdtw_cross_attention_backward_workspace_bytes(const sdtw_attention_problem* p)
 {
-    if (sdtw::checked(p) != SDTW_OK) return 0;
-    // delta, and a word a key head
-    return (static_cast<size_t>(p->B) * p->Hq * p->N + static_cast<size_t>(p->B) * p->Hkv) * sizeof(float);
+    using namespace sdtw;
+    if (checked(p) != SDTW_OK) return 0;
+    size_t words = static_cast<size_t>(p->B) * p->Hq * p->N;  // delta
+    if (p->dtype == SDTW_F16) words += static_cast<size_t>(p->B) * p->Hkv * (peak_blocks(p->M) + 2 * peak_blocks(p->N));
+    return words * sizeof(float);
 }
 
 sdtw_status sdtw_cross_attention_backward(const sdtw_attention_problem* p, const void* out, const void* out_lo,
@@ -144,10 +149,19 @@ sdtw_status sdtw_cross_attention_backward(const sdtw_attention_problem* p, const
     a.dv = dv;
     a.delta = static_cast<float*>(workspace);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    uint32_t* peak = reinterpret_cast<uint32_t*>(a.delta + static_cast<size_t>(a.B) * a.Hq * a.N);
+    if (p->dtype == SDTW_F16) {
+        const size_t heads = static_cast<size_t>(a.B) * a.Hkv;
+        a.v_blocks = peak_blocks(a.M);
+        a.q_blocks = peak_blocks(a.N);
+        a.v_peak = a.delta + static_cast<size_t>(a.B) * a.Hq * a.N;
+        a.do_peak = a.v_peak + heads * a.v_blocks;
+        a.delta_peak = a.do_peak + heads * a.q_blocks;
+        const cudaError_t e = attention_peaks(a, s);
+        if (e != cudaSuccess) return static_cast<sdtw_status>(e);
+    }
     if (p->N > 0 && takes_tc(p, a) && attention_tc_takes(a.dout, a.gs, a.B, a.N, a.Hq, a.d))
-        return static_cast<sdtw_status>(attention_tc_backward(a, p->dtype == SDTW_BF16, peak, s));
-    return static_cast<sdtw_status>(attention_mma_backward(a, p->dtype, peak, s));
+        return static_cast<sdtw_status>(attention_tc_backward(a, p->dtype == SDTW_BF16, s));
+    return static_cast<sdtw_status>(attention_mma_backward(a, p->dtype, s));
 }
 
 }  // extern "C"

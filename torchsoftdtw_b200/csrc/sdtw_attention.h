@@ -7,6 +7,8 @@
 
 namespace sdtw {
 
+constexpr int kPeakRows = 64;  // rows (states, or queries) that share one word of the maxima below
+
 struct Strides {
     int64_t b, n, h;
 };
@@ -29,6 +31,10 @@ struct AttnArgs {
     Strides gs;
     void *dq, *dk, *dv;
     float* delta;  // (B, Hq, N): sum_j p_ij dp_ij
+    // fp16 (sdtw_attention_range.cuh): per key head, the largest |v| of each kPeakRows states; the largest |do|^2 and |delta| of
+    // each kPeakRows queries of its query heads
+    float *v_peak, *do_peak, *delta_peak;
+    int64_t v_blocks, q_blocks;
 };
 
 // What out_lo holds of an output's remainder (what rounding it to its type dropped): fp16's is kept 2^11 larger, about as large

@@ -6,6 +6,7 @@
 // float32 is bound by the instructions that split operands into heads and tails, once for each use: 64 x 256 x 192 x 4 x 32,
 // band 32, 135 us; 2 x 2048 x 2048 x 8 x 128 3.55 ms, 34 TFLOP/s of the seven products.
 #include "sdtw_attention_mma.cuh"
+#include "sdtw_attention_range.cuh"
 #include "sdtw_attention_split.h"
 
 namespace sdtw {
@@ -35,23 +36,15 @@ struct Geom {
 
 struct Args {
     AttnArgs a;
-    int tiles;       // CTAs a head
-    uint32_t* peak;  // fp16: (B, Hkv) bits of the largest |do|^2 of the head's rows
+    int tiles;  // CTAs a head
 };
-
-// A power of two that brings `norm2` = |do|^2 to [64, 256), or one (fp16; as in the tensor-core kernels).
-__device__ __forceinline__ float gradient_scale(float norm2)
-{
-    if (!(norm2 > 1e-30f) || !(norm2 < 1e30f)) return 1.f;
-    return exp2f(3.f - floorf(0.5f * log2f(norm2)));
-}
 
 template <typename T, int DPAD, int VB, bool KV>
 __global__ void __launch_bounds__(kThreads, Geom<T, DPAD>::CTAS) attend_backward_mma_kernel(const __grid_constant__ Args f)
 {
     using G = Geom<T, DPAD>;
     constexpr int UPR = DPAD / G::UNIT;
-    constexpr float kShift = is_half<T> ? 10.f : 0.f;  // P is kept 2^10 larger
+    constexpr float kShift = is_half<T> ? kHalfShift : 0.f, kUnshift = is_half<T> ? kHalfUnshift : 1.f;
     const AttnArgs& a = f.a;
     extern __shared__ __align__(128) unsigned char sm[];
     T* x1 = reinterpret_cast<T*>(sm);
@@ -93,8 +86,10 @@ __global__ void __launch_bounds__(kThreads, Geom<T, DPAD>::CTAS) attend_backward
     const Strides &r1s = KV ? a.ks : a.qs, &r2s = KV ? a.vs : a.gs, &y1s = KV ? a.qs : a.ks, &y2s = KV ? a.gs : a.vs;
     const T* r1p = static_cast<const T*>(KV ? a.k : a.q) + b * r1s.b + hr * r1s.h;
     const T* r2p = static_cast<const T*>(KV ? a.v : a.dout) + b * r2s.b + hr * r2s.h;
-    const float gscale = is_half<T> && KV ? gradient_scale(__uint_as_float(f.peak[b * a.Hkv + hk])) : 1.f;
-    const float cf = is_half<T> ? gscale * 0x1p-10f : 1.f;
+    float gscale = 1.f;  // of dS: here for all states of the CTA, in dq a row's own
+    if (is_half<T> && KV && c1 > c0)
+        gscale = half_scale(bound_of(bound_part(a, b, hk, c0, c1, row0, row0 + kRows < nr ? row0 + kRows : nr)));
+    const float cf = gscale * kUnshift;
 
     const auto load_tile = [&](int t) {
         const int h = KV ? hk * a.group + t / per_head : hk;
@@ -136,8 +131,11 @@ __global__ void __launch_bounds__(kThreads, Geom<T, DPAD>::CTAS) attend_backward
     }
     if (steps > 0) load_tile(0);
     cp_async_commit();
+    float v_top = 0.f;  // the largest |v| of the CTA's states
+    if (is_half<T> && !KV && c1 > c0) v_top = value_part(a, b, hk, c0, c1);
     if constexpr (!KV) {
         // delta and |do|^2 of this warp's rows.
+        float top_delta = 0.f, top_norm = 0.f;
         for (int r = warp * 16; r < warp * 16 + 16; ++r) {
             const int64_t i = row0 + r;
             float dot = 0.f, nrm = 0.f;
@@ -157,17 +155,20 @@ __global__ void __launch_bounds__(kThreads, Geom<T, DPAD>::CTAS) attend_backward
                 row_stat[r] = dot;
                 row_stat[kRows + r] = nrm;
                 if (i < a.N) a.delta[(static_cast<int64_t>(b) * a.Hq + hr) * a.N + i] = dot;
-                if (is_half<T> && i < nx) atomicMax(f.peak + b * a.Hkv + hk, __float_as_uint(nrm));
             }
+            top_delta = fmaxf(top_delta, fabsf(dot));
+            top_norm = fmaxf(top_norm, nrm);
         }
+        if (is_half<T> && lane == 0 && row0 + warp * 16 < nx) raise_gradient_peak(a, b, hk, row0 + warp * 16, top_norm, top_delta);
         __syncwarp();
     }
     float r_bias[2], r_delta[2], r_scale[2], r_cf[2];  // dq: of this thread's rows
+    v_top = warp_maxf(v_top);
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
         const int r = warp * 16 + (lane >> 2) + 8 * x;
-        r_scale[x] = is_half<T> && !KV ? gradient_scale(row_stat[kRows + r]) : gscale;
-        r_cf[x] = is_half<T> && !KV ? r_scale[x] * 0x1p-10f : cf;
+        r_scale[x] = is_half<T> && !KV ? half_scale(fmaf(sqrtf(row_stat[kRows + r]), v_top, fabsf(row_stat[r]))) : gscale;
+        r_cf[x] = is_half<T> && !KV ? r_scale[x] * kUnshift : cf;
         r_delta[x] = KV ? 0.f : row_stat[r] * r_cf[x];
         r_bias[x] = !KV && hi[x] > lo[x] ? kShift - a.lse[(static_cast<int64_t>(b) * a.Hq + hr) * a.N + row0 + r] : -INFINITY;
     }
@@ -231,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, Geom<T, DPAD>::CTAS) attend_backward
                 const int col = 8 * y + 2 * (lane & 3) + e;
                 if (col >= a.d) continue;
                 out1[col] = from_f<T>(any ? acc1[y][2 * x + e] * back : 0.f);
-                if constexpr (KV) out2[col] = from_f<T>(any ? acc2[y][2 * x + e] * (is_half<T> ? 0x1p-10f : 1.f) : 0.f);
+                if constexpr (KV) out2[col] = from_f<T>(any ? acc2[y][2 * x + e] * kUnshift : 0.f);
             }
     }
 }
@@ -282,15 +283,11 @@ cudaError_t backward_t(Args& f, cudaStream_t s)
 
 }  // namespace
 
-cudaError_t attention_mma_backward(const AttnArgs& a, int dtype, uint32_t* peak, cudaStream_t s)
+cudaError_t attention_mma_backward(const AttnArgs& a, int dtype, cudaStream_t s)
 {
     Args f{};
     f.a = a;
-    f.peak = peak;
-    if (dtype == SDTW_F16) {
-        const cudaError_t e = cudaMemsetAsync(peak, 0, sizeof(uint32_t) * static_cast<size_t>(a.B) * a.Hkv, s);
-        return e != cudaSuccess ? e : backward_t<__half>(f, s);
-    }
+    if (dtype == SDTW_F16) return backward_t<__half>(f, s);
     return dtype == SDTW_F32 ? backward_t<float>(f, s) : backward_t<__nv_bfloat16>(f, s);
 }
 

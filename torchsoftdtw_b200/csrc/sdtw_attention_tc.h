@@ -26,7 +26,8 @@ bool attention_tile_map(CUtensorMap* map, bool half, const void* ptr, const Stri
 // out, out_lo and lse of a (M > 0), from q, k and v that attention_tc_takes.
 cudaError_t attention_tc_forward(const AttnArgs& a, bool bf16, cudaStream_t s);
 
-// dq, dk, dv and delta of a (N, M > 0), from q, k, v and dout that attention_tc_takes. peak: (B, Hkv) words, fp16 only.
-cudaError_t attention_tc_backward(const AttnArgs& a, bool bf16, uint32_t* peak, cudaStream_t s);
+// dq, dk, dv and delta of a (N, M > 0), from q, k, v and dout that attention_tc_takes; fp16 behind
+// attention_peaks.
+cudaError_t attention_tc_backward(const AttnArgs& a, bool bf16, cudaStream_t s);
 
 }  // namespace sdtw

@@ -14,12 +14,12 @@
 // of the seven products), 4 x 4096 x 4096 x 16 x 64 1023 us, 32 x 512 x 512 x 8 x 64 120 us, where the CTAs' first loads,
 // of all SMs at once, take a third of the time. Sums of the tile before placed between S and dP: 10% slower.
 //
-// fp16: P is kept 2^10 larger and dS scaled by a power of two that brings the rows' |do| to [8, 16) (a row's own in
-// dq, where a row is a lane; the largest of the head in dk), so that neither under- nor overflows where the gradients do not.
+// fp16: P is kept 2^14 larger and dS scaled by a power of two (a row's own in dq, where a row is a lane; one for the CTA's states in
+// dk): sdtw_attention_range.cuh.
 #include <mutex>
 #include <type_traits>
 
-#include "sdtw_attention.h"
+#include "sdtw_attention_range.cuh"
 #include "sdtw_attention_tc.h"
 #include "sdtw_tc.cuh"
 
@@ -34,23 +34,17 @@ constexpr int kTile = 128;  // rows of a product: queries in dq, states in dk/dv
 template <typename T>
 constexpr bool is_half = std::is_same<T, __half>::value;
 template <typename T>
-constexpr float kPShift = is_half<T> ? 10.f : 0.f;
+constexpr float kPShift = is_half<T> ? kHalfShift : 0.f;
+template <typename T>
+constexpr float kPUnshift = is_half<T> ? kHalfUnshift : 1.f;
 
 struct BwdArgs {
     AttnArgs a;
     uint64_t timeout_ns;
-    int tiles;        // CTAs a head
-    int dn;           // d rounded up to 16
-    int stall;        // attention_stall()
-    uint32_t* peak;   // fp16: (B, Hkv) bits of the largest |do|^2 of the head's rows
+    int tiles;  // CTAs a head
+    int dn;     // d rounded up to 16
+    int stall;  // attention_stall()
 };
-
-// A power of two that brings `norm2` = |do|^2 to [64, 256), or one.
-__device__ __forceinline__ float gradient_scale(float norm2)
-{
-    if (!(norm2 > 1e-30f) || !(norm2 < 1e30f)) return 1.f;
-    return exp2f(3.f - floorf(0.5f * log2f(norm2)));
-}
 
 constexpr int kCols = 64;  // columns of a product: states in dq, queries in dk/dv
 
@@ -360,7 +354,12 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
         // delta and |do|^2 of the tile's rows: LPR lanes a row, all loads ahead of the sums (rows and features outside read a
         // place inside, and count as zero).
         constexpr int LPR = DPAD / 8, RPW = 32 / LPR, ROUNDS = kTile / (G::ELEM_WARPS * RPW);
+        float v_top = 0.f;  // fp16: the largest |v| of the tile's states
         if (n > 0) {
+            if constexpr (is_half<T>) {
+                const int64_t end = static_cast<int64_t>(ja + n) * kCols;
+                v_top = value_part(a, b, hk, static_cast<int64_t>(ja) * kCols, end < ny ? end : ny);
+            }
             Vec<T, 8> g[ROUNDS], o[ROUNDS], lo[ROUNDS];
             const int c = lane % LPR * 8 < a.d ? lane % LPR * 8 : 0;
 #pragma unroll
@@ -390,10 +389,7 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
                 if (lane % LPR == 0) {
                     s_delta[r] = dot;
                     s_norm[r] = nrm;
-                    if (row0 + r < nx) {
-                        a.delta[(static_cast<int64_t>(b) * a.Hq + h) * a.N + row0 + r] = dot;
-                        if (is_half<T>) atomicMax(f.peak + b * a.Hkv + hk, __float_as_uint(nrm));
-                    }
+                    if (row0 + r < nx) a.delta[(static_cast<int64_t>(b) * a.Hq + h) * a.N + row0 + r] = dot;
                 }
             }
         }
@@ -407,8 +403,17 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
         const uint32_t ts = tmem + lanes + x * BUF_COLS + 32 * half, tdp = ts + DP_COL;
         const uint32_t tds = tmem + lanes + x * BUF_COLS + DS_COL + 16 * half;
-        const float gscale = is_half<T> ? gradient_scale(s_norm[r]) : 1.f;
-        const float cf = is_half<T> ? gscale * exp2f(-kPShift<T>) : 1.f;
+        float gscale = 1.f;
+        if (is_half<T> && n > 0) {
+            if (warp < kTile / kPeakRows) {
+                const int r1 = warp * kPeakRows + lane;
+                const float norm2 = warp_maxf(fmaxf(s_norm[r1], s_norm[r1 + 32]));
+                const float top = warp_maxf(fmaxf(fabsf(s_delta[r1]), fabsf(s_delta[r1 + 32])));
+                if (lane == 0 && row0 + warp * kPeakRows < nx) raise_gradient_peak(a, b, hk, row0 + warp * kPeakRows, norm2, top);
+            }
+            gscale = half_scale(fmaf(sqrtf(s_norm[r]), warp_maxf(v_top), fabsf(s_delta[r])));
+        }
+        const float cf = gscale * kPUnshift<T>;
         const float delta = s_delta[r] * cf, bias = kPShift<T> - lse;
         bool ok = true;
         for (int it = x; it < n; it += G::BUFS) {
@@ -544,12 +549,16 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
     const int ia = static_cast<int>(*reinterpret_cast<volatile uint32_t*>(misc + 2));
     const int nq = static_cast<int>(*reinterpret_cast<volatile uint32_t*>(misc + 3)) - ia;  // tiles a query head
     const int n = nq > 0 ? nq * a.group : 0;
-    // One power of two for all rows that share the sums.
-    const float gscale = is_half<T> ? gradient_scale(__uint_as_float(f.peak[b * a.Hkv + hk])) : 1.f;
-    const float cf = is_half<T> ? gscale * exp2f(-kPShift<T>) : 1.f;
+    // fp16: one power of two for all rows that share the sums.
+    BoundPart part{};
+    if (is_half<T> && n > 0) {
+        const int64_t end = static_cast<int64_t>(ia + nq) * kCols;
+        part = bound_part(a, b, hk, static_cast<int64_t>(ia) * kCols, end < nx ? end : nx, row0, row0 + kTile < ny ? row0 + kTile : ny);
+    }
 
     if (warp == G::TMA_WARP) {
         int head = hk * a.group, tile = -1;  // of the step that coords() was last asked for
+        float cf = is_half<T> ? 0.f : 1.f;   // formed behind the row tiles' loads
         load_tiles<DPAD>(
             sm, base, &mk, &mv, &mq, &mg, row0, hk, b, n, nx, a.N, row_full, fix, full, empty, bound, lane,
             [&](int, int& c0, int& hd) {
@@ -564,6 +573,7 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
                 const int i0 = (ia + tile) * kCols;
                 const int64_t at = (static_cast<int64_t>(b) * a.Hq + head) * a.N + i0;
                 float* st = stats + stage * 2 * kCols;
+                if (is_half<T> && cf == 0.f) cf = half_scale(bound_of(part)) * kPUnshift<T>;
 #pragma unroll
                 for (int c = lane; c < kCols; c += 32) {
                     const bool on = i0 + c < nx;  // a query past the length has P = 2^-inf = 0
@@ -645,6 +655,7 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
         const int64_t j = row0 + 32 * (warp & 3) + lane;
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
         const uint32_t ts = tmem + lanes + x * BUF_COLS + 32 * half, tdp = ts + DP_COL;
+        const float gscale = is_half<T> ? half_scale(bound_of(part)) : 1.f, cf = gscale * kPUnshift<T>;
         int64_t lo = 0, hi = 0;
         if (j < ny && nx > 0) column_cells(a, j, nx, ny, lo, hi);
         const int ilo = static_cast<int>(lo), width = static_cast<int>(hi - lo);
@@ -724,7 +735,7 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
                                 a.d, static_cast<T*>(a.dk) + at, pitch, a.M - j0);
         if (x == G::BUFS - 1)
             store_rows<T, DPAD>(tmem + lanes + DV_COL, rows + G::ROW_BYTES / 16, lane, half, 6 + (warp & 3), any, width > 0, !ok,
-                                is_half<T> ? exp2f(-kPShift<T>) : 1.f, f.dn, a.d, static_cast<T*>(a.dv) + at, pitch, a.M - j0);
+                                kPUnshift<T>, f.dn, a.d, static_cast<T*>(a.dv) + at, pitch, a.M - j0);
         fence_before();
     }
     __syncthreads();
@@ -756,10 +767,6 @@ cudaError_t backward_d(BwdArgs& f, cudaStream_t s)
             !attention_tile_map(&g_cols, half, a.dout, a.gs, a.B, a.N, a.Hq, a.d, kCols))
             return bad;
     }
-    if (half) {
-        e = cudaMemsetAsync(f.peak, 0, sizeof(uint32_t) * static_cast<size_t>(a.B) * a.Hkv, s);
-        if (e != cudaSuccess) return e;
-    }
     static std::atomic<bool> allowed[3][128];
     const bool tail = DPAD == 64 && a.d <= 32;
     const auto dq = tail ? attend_dq_tc_kernel<T, DPAD, DPAD == 64> : attend_dq_tc_kernel<T, DPAD, false>;
@@ -778,13 +785,12 @@ cudaError_t backward_d(BwdArgs& f, cudaStream_t s)
 
 }  // namespace
 
-cudaError_t attention_tc_backward(const AttnArgs& a, bool bf16, uint32_t* peak, cudaStream_t s)
+cudaError_t attention_tc_backward(const AttnArgs& a, bool bf16, cudaStream_t s)
 {
     BwdArgs f{};
     f.a = a;
     f.timeout_ns = static_cast<uint64_t>(wait_timeout_s() * 1e9);
     f.dn = (a.d + 15) / 16 * 16;
-    f.peak = peak;
     f.stall = attention_stall();
     if (bf16) return a.d <= 64 ? backward_d<__nv_bfloat16, 64>(f, s) : backward_d<__nv_bfloat16, 128>(f, s);
     return a.d <= 64 ? backward_d<__half, 64>(f, s) : backward_d<__half, 128>(f, s);
