@@ -63,8 +63,8 @@ struct Geom {
     static constexpr int OFF_STAT = OFF_RING + (S0 + S1) * COL_BYTES;
     static constexpr int STAT_BYTES = 4 * (S0 * 2 * kCols > 2 * kTile ? S0 * 2 * kCols : 2 * kTile);
     static constexpr int OFF_BAR = OFF_STAT + STAT_BYTES;
-    // row_full, fix, full[S0 + S1], empty[S0 + S1], acc_full, and six a buffer
-    static constexpr int NBAR = 3 + 2 * (S0 + S1) + 6 * BUFS;
+    // row_full, fix, full[S0 + S1], empty[S0 + S1], acc_full, idle, and six a buffer
+    static constexpr int NBAR = 4 + 2 * (S0 + S1) + 6 * BUFS;
     static_assert(S0 % BUFS == 0, "a group of elementwise warps sees every turn of its stages");
     static constexpr int OFF_MISC = OFF_BAR + 8 * NBAR;
     static constexpr int BYTES = OFF_MISC + 32 + 1024;
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
     const uint32_t base = smem_addr(sm);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t row_full = base + G::OFF_BAR, fix = row_full + 8, full = fix + 8, empty = full + 8 * (G::S0 + G::S1);
-    const uint32_t acc_full = empty + 8 * (G::S0 + G::S1), s_full = acc_full + 8, s_free = s_full + 8 * G::BUFS;
+    const uint32_t acc_full = empty + 8 * (G::S0 + G::S1), idle = acc_full + 8, s_full = idle + 8, s_free = s_full + 8 * G::BUFS;
     const uint32_t dp_full = s_free + 8 * G::BUFS, dp_free = dp_full + 8 * G::BUFS, ds_full = dp_free + 8 * G::BUFS;
     const uint32_t ds_free = ds_full + 8 * G::BUFS;
     uint32_t* misc = reinterpret_cast<uint32_t*>(sm + G::OFF_MISC);
@@ -252,6 +252,7 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
         mbar_init(fix, 1);
         for (int s = 0; s < 2 * (G::S0 + G::S1); ++s) mbar_init(full + 8 * s, 1);
         mbar_init(acc_full, 1);
+        mbar_init(idle, 1);
         for (int x = 0; x < G::BUFS; ++x) {
             mbar_init(s_full + 8 * x, 1);
             mbar_init(s_free + 8 * x, 8);
@@ -345,8 +346,9 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
                     ok = ok && sums(i);
                 }
             }
-            mma_commit(acc_full, leader);
-            mbar_drain(acc_full, 0, f.timeout_ns);  // before the tensor memory is given back
+            if (ok) mma_commit(acc_full, leader);  // else the elementwise warps' wait for it ends by the abort
+            mma_commit(idle, leader);
+            mbar_drain(idle, 0, f.timeout_ns);  // before the tensor memory is given back
         }
         __syncwarp();
     } else {
@@ -502,7 +504,7 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
     const uint32_t base = smem_addr(sm);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t row_full = base + G::OFF_BAR, fix = row_full + 8, full = fix + 8, empty = full + 8 * (G::S0 + G::S1);
-    const uint32_t acc_full = empty + 8 * (G::S0 + G::S1), s_full = acc_full + 8, p_full = s_full + 8 * G::BUFS;
+    const uint32_t acc_full = empty + 8 * (G::S0 + G::S1), idle = acc_full + 8, s_full = idle + 8, p_full = s_full + 8 * G::BUFS;
     const uint32_t dp_full = p_full + 8 * G::BUFS, ds_full = dp_full + 8 * G::BUFS, dv_done = ds_full + 8 * G::BUFS;
     const uint32_t dk_done = dv_done + 8 * G::BUFS;
     uint32_t* misc = reinterpret_cast<uint32_t*>(sm + G::OFF_MISC);
@@ -519,6 +521,7 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
         mbar_init(fix, 1);
         for (int s = 0; s < 2 * (G::S0 + G::S1); ++s) mbar_init(full + 8 * s, 1);
         mbar_init(acc_full, 1);
+        mbar_init(idle, 1);
         for (int x = 0; x < G::BUFS; ++x) {
             mbar_init(s_full + 8 * x, 1);
             mbar_init(p_full + 8 * x, 8);
@@ -645,8 +648,9 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
                     ok = sums_v(i) && sums_k(i) && (!more || (scores(i + 2) && dprobs(i + 2)));
                 }
             }
-            mma_commit(acc_full, leader);
-            mbar_drain(acc_full, 0, f.timeout_ns);  // before the tensor memory is given back
+            if (ok) mma_commit(acc_full, leader);  // else the elementwise warps' wait for it ends by the abort
+            mma_commit(idle, leader);
+            mbar_drain(idle, 0, f.timeout_ns);  // before the tensor memory is given back
         }
         __syncwarp();
     } else {
