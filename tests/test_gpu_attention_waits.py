@@ -1,4 +1,5 @@
-"""GPU: waits of the tensor-core kernels that run out, where the tile that they are about is the last one of its rows."""
+"""GPU: waits of the tensor-core kernels that run out, where the tile that they are about is the last one of its rows, or is being
+cleared behind a length."""
 
 import pytest
 import torch
@@ -53,3 +54,12 @@ def stalled(which, name, N, M, d, lens=(None, None)):
 def test_in_the_last_tiles(cuda, d, which, name, N, M):
     """Few tiles: the warps that are not stalled have theirs when the wait runs out."""
     stalled(which, name, N, M, d)
+
+
+@pytest.mark.parametrize("length", [60, 100, 600])
+@pytest.mark.parametrize("which,name", STALLS)
+@pytest.mark.parametrize("d", [64, 128])
+def test_beside_a_padded_tile(cuda, d, which, name, length):
+    """The stalled sample's last tile is loaded and cleared while the others wait (the short ones), or after."""
+    lens = torch.tensor([length, 650], device=cuda), torch.tensor([length, 640], device=cuda)
+    stalled(which, name, 700, 650, d, lens)

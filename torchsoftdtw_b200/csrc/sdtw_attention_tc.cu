@@ -173,6 +173,7 @@ __global__ void __launch_bounds__(Geom<DPAD, NT>::THREADS, NT == 1 ? 2 : 1)
                 bool ok = true;
                 if (clear) {
                     ok = mbar_wait(fix, 0, bound);
+                    if (!ok) mbar_drain(fix, 0, f.timeout_ns);  // `full`, drained below, will not tell of this load
                     for (int x = 0; x < G::NBLOCK; ++x)
                         for (int u = static_cast<int>(left) * 8 + lane; u < kStates * 8; u += 32)
                             *reinterpret_cast<uint4*>(sm + at + x * G::KV_BLOCK + 16 * u) = make_uint4(0, 0, 0, 0);

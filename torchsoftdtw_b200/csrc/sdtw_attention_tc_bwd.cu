@@ -167,6 +167,7 @@ __device__ __forceinline__ void load_tiles(unsigned char* sm, uint32_t base, con
             __syncwarp();
             if (clear) {
                 ok = mbar_wait(fix, fixes & 1, bound);
+                if (!ok) mbar_drain(fix, fixes & 1, bound.timeout_ns);  // `full`, drained below, will not tell of this load
                 ++fixes;
                 for (int x = 0; x < G::NBLOCK; ++x)
                     for (int u = static_cast<int>(left) * 8 + lane; u < kCols * 8; u += 32)
