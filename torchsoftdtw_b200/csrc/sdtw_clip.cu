@@ -97,11 +97,12 @@ __device__ __forceinline__ void for_entries(const T* p, int n, F f)
 }
 
 // A sum of squares whose float64 entries may square out of their range: entries above 2^400 enter `big` scaled
-// by 2^-500, entries below 2^-400 `small` scaled by 2^500, all others `mid`.
+// by 2^-600, entries below 2^-400 `small` scaled by 2^600, all others `mid`. Scaled, the largest entry squares to 2^848, the
+// smallest subnormal one to 2^-948, and those next to the borders to 2^-400 and 2^400.
 struct Squares {
     double mid, big, small;
 };
-constexpr double kUp = 0x1p500, kDown = 0x1p-500;
+constexpr double kUp = 0x1p600, kDown = 0x1p-600;
 
 __device__ __forceinline__ double norm_of(const Squares& q)
 {
