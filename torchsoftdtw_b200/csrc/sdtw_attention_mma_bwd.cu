@@ -213,6 +213,14 @@ __global__ void __launch_bounds__(kThreads, Geom<T, DPAD>::CTAS) attend_backward
                 dp[x][e] = p * fmaf(dp[x][e], is_half<T> ? r_cf[row] : 1.f, -delta);
             }
         product_columns<T, DPAD, G::LD, G::TC / 8>(acc1, dp, y1, lane);
+        // dq of few features: what the rounding of dS dropped goes through a second product (as in the tensor-core kernel).
+        if constexpr (!KV && sizeof(T) == 2 && DPAD == 32) {
+#pragma unroll
+            for (int x = 0; x < G::TC / 8; ++x)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dp[x][e] -= to_f(from_f<T>(dp[x][e]));
+            product_columns<T, DPAD, G::LD, G::TC / 8>(acc1, dp, y1, lane);
+        }
         if constexpr (KV) product_columns<T, DPAD, G::LD, G::TC / 8>(acc2, s, y2, lane);
     }
     cp_async_wait<0>();
