@@ -58,7 +58,7 @@ def clip_grads(
         norm_type: 2 or ``inf``.
         out: tensors of the gradients' shapes and dtypes that the result is written to; the gradients themselves
             clip in place (and where nothing exceeds the bound, nothing is written). No two of them, nor one of
-            them and another gradient, may share memory. Defaults to new tensors.
+            them and another gradient, may share an entry (slices of one buffer may lie between one another). Defaults to new tensors.
 
     Returns:
         (clipped, norm): the list of results and the norm before clipping, a 0-dim tensor. Nothing waits for the

@@ -4,6 +4,7 @@
 // Autograd is in C++: at these kernels' times, a training step through Python functions would be bound by the host
 // (about 100 us a step against 45 us of kernels at 32 x 512 x 8 x 64).
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -381,6 +382,63 @@ sdtw_tensor_ref ref_of(const Tensor& src, void* dst)
     return {src.data_ptr(), dst, src.numel(), static_cast<int32_t>(code_of(src.scalar_type())), 0};
 }
 
+// Where a tensor's entries lie: `width` bytes at every sum of a multiple of each stride (in bytes, largest first) below its size.
+struct Places {
+    struct Dim {
+        int64_t size, stride;
+    };
+    std::vector<Dim> dims;
+    int64_t width;
+    int64_t extent(size_t from) const  // of the dimensions from `from` on
+    {
+        int64_t e = width;
+        for (size_t i = from; i < dims.size(); ++i) e += (dims[i].size - 1) * dims[i].stride;
+        return e;
+    }
+};
+
+Places places_of(const Tensor& t)
+{
+    Places p;
+    p.width = t.element_size();
+    for (int64_t i = 0; i < t.dim(); ++i)
+        if (t.size(i) > 1 && t.stride(i) > 0) p.dims.push_back({t.size(i), t.stride(i) * p.width});
+    std::sort(p.dims.begin(), p.dims.end(), [](const Places::Dim& a, const Places::Dim& b) { return a.stride > b.stride; });
+    while (!p.dims.empty() && p.dims.back().stride <= p.width) {  // neighbours without a gap are one piece
+        p.width += (p.dims.back().size - 1) * p.dims.back().stride;
+        p.dims.pop_back();
+    }
+    return p;
+}
+
+// Whether dimensions i.. of a and j.. of b, which begins `at` bytes behind a, share a byte. Extents that do not meet share none; rows of
+// one pitch meet by their difference alone; otherwise the tensor with the longer pitch is taken row by row. After `steps` the
+// answer is yes.
+bool share(const Places& a, size_t i, const Places& b, size_t j, int64_t at, int& steps)
+{
+    if (at >= a.extent(i) || -at >= b.extent(j)) return false;
+    const bool more_a = i < a.dims.size(), more_b = j < b.dims.size();
+    if ((!more_a && !more_b) || --steps < 0) return true;
+    const auto ceil = [](int64_t x, int64_t y) { return x / y + (x % y > 0); };
+    const auto floor = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
+    const int64_t pa = more_a ? a.dims[i].stride : 0, pb = more_b ? b.dims[j].stride : 0;
+    const size_t ni = pa >= pb ? i + 1 : i, nj = pb >= pa ? j + 1 : j;
+    const int64_t pitch = std::max(pa, pb), wa = a.extent(ni), wb = b.extent(nj);
+    // x: a row of b less a row of a (one of them 0, where only one tensor has rows of this pitch).
+    const int64_t first = std::max(pa >= pb ? 1 - a.dims[i].size : 0, ceil(1 - wb - at, pitch));
+    const int64_t last = std::min(pb >= pa ? b.dims[j].size - 1 : 0, floor(wa - 1 - at, pitch));
+    for (int64_t x = first; x <= last; ++x)
+        if (share(a, ni, b, nj, at + x * pitch, steps)) return true;
+    return false;
+}
+
+bool share_memory(const Tensor& a, const Tensor& b)
+{
+    int steps = 1 << 20;
+    const int64_t at = static_cast<int64_t>(reinterpret_cast<intptr_t>(b.data_ptr()) - reinterpret_cast<intptr_t>(a.data_ptr()));
+    return share(places_of(a), 0, places_of(b), 0, at, steps);
+}
+
 Tensor norm_result(const Tensor& like, bool wide)
 {
     return at::empty({}, like.options().dtype(wide ? at::kDouble : at::kFloat));
@@ -422,6 +480,7 @@ Tensor clip_grads_cuda(at::TensorList grads, at::TensorList out, double max_norm
         uintptr_t begin, end;
         size_t index;
         bool written;
+        const Tensor* tensor;
     };
     std::vector<Range> ranges;
     std::vector<Tensor> keep;                          // copies of gradients that are not dense
@@ -434,13 +493,15 @@ Tensor clip_grads_cuda(at::TensorList grads, at::TensorList out, double max_norm
         if (!t.is_contiguous())
             for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
         const uintptr_t p = reinterpret_cast<uintptr_t>(t.data_ptr());
-        return Range{p, p + static_cast<uintptr_t>(last + 1) * t.element_size(), i, written};
+        return Range{p, p + static_cast<uintptr_t>(last + 1) * t.element_size(), i, written, &t};
     };
     for (size_t i = 0; i < grads.size(); ++i) {
         const Tensor &g = grads[i], &o = out[i];
         TORCH_CHECK(o.sizes() == g.sizes() && o.scalar_type() == g.scalar_type() && o.device() == g.device() &&
                         o.layout() == at::kStrided,
                     "out[", num(i), "] must have the gradient's shape, dtype and device");
+        TORCH_CHECK(g.numel() == 0 || is_dense(o) || at::has_internal_overlap(o) != at::MemOverlap::Yes, "out[", num(i),
+                    "] holds several entries in one place");
         const bool alike = o.strides() == g.strides();
         if (g.numel() > 0) {
             ranges.push_back(range_of(o, true, i));
@@ -461,11 +522,17 @@ Tensor clip_grads_cuda(at::TensorList grads, at::TensorList out, double max_norm
         }
     }
     std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
-    uintptr_t read_end = 0, write_end = 0;
+    std::vector<const Range*> open;  // those that end behind the present one's begin
     for (const Range& r : ranges) {
-        TORCH_CHECK(r.begin >= write_end && !(r.written && r.begin < read_end),
-                    "clip_grads: tensor ", num(r.index), " shares memory with another one that is written");
-        (r.written ? write_end : read_end) = std::max(r.written ? write_end : read_end, r.end);
+        size_t kept = 0;
+        for (const Range* o : open) {
+            if (o->end <= r.begin) continue;
+            open[kept++] = o;
+            TORCH_CHECK(!(o->written || r.written) || !share_memory(*o->tensor, *r.tensor), "clip_grads: tensor ", num(r.index),
+                        " shares memory with another one that is written");
+        }
+        open.resize(kept);
+        open.push_back(&r);
     }
     const Tensor norm = norm_result(grads[0], wide);
     const size_t wsb = sdtw_clip_workspace_bytes(static_cast<int64_t>(refs.size()));
