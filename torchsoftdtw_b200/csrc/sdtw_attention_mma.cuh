@@ -69,16 +69,6 @@ __device__ __forceinline__ void ldmatrix4t(uint32_t addr, uint32_t (&r)[4])
                  : "r"(addr)
                  : "memory");
 }
-__device__ __forceinline__ uint32_t pack(float lo, float hi, __half)
-{
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ uint32_t pack(float lo, float hi, __nv_bfloat16)
-{
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
 
 // c[x] += A B^T for the NB 8-row groups of B: A 16 rows, B 8 NB rows, both row-major of pitch LD in shared memory, K over their
 // DPAD features.
@@ -139,8 +129,8 @@ __device__ __forceinline__ void product_columns(float (&o)[DPAD / 8][4], const f
         const uint32_t b_at = smem_addr(B) + 2 * (((lane & 7) + ((lane >> 3) & 1) * 8) * LD + ((lane >> 4) & 1) * 8);
 #pragma unroll
         for (int x = 0; x < NB / 2; ++x) {
-            const uint32_t a[4] = {pack(s[2 * x][0], s[2 * x][1], T()), pack(s[2 * x][2], s[2 * x][3], T()),
-                                   pack(s[2 * x + 1][0], s[2 * x + 1][1], T()), pack(s[2 * x + 1][2], s[2 * x + 1][3], T())};
+            const uint32_t a[4] = {pack2(s[2 * x][0], s[2 * x][1], T()), pack2(s[2 * x][2], s[2 * x][3], T()),
+                                   pack2(s[2 * x + 1][0], s[2 * x + 1][1], T()), pack2(s[2 * x + 1][2], s[2 * x + 1][3], T())};
 #pragma unroll
             for (int y = 0; y < DPAD / 16; ++y) {
                 uint32_t b[4];
@@ -190,8 +180,6 @@ __device__ __forceinline__ void copy_unit(T* dst, const T* src, int f, int d, bo
         if (f + e >= d) break;
         if constexpr (VB == 16)
             cp_async_16(dst, src, on ? 16 : 0);
-        else if constexpr (VB == 8)
-            cp_async_8(dst + e, src + e, on ? 8 : 0);
         else if constexpr (VB == 4)
             cp_async_4(dst + e, src + e, on ? 4 : 0);
         else

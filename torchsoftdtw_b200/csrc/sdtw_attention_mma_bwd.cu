@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, Geom<T, DPAD>::CTAS) attend_backward
         __syncwarp();
     }
     float r_bias[2], r_delta[2], r_scale[2], r_cf[2];  // dq: of this thread's rows
-    v_top = warp_maxf(v_top);
+    if constexpr (is_half<T> && !KV) v_top = warp_maxf(v_top);
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
         const int r = warp * 16 + (lane >> 2) + 8 * x;

@@ -758,20 +758,17 @@ cudaError_t backward_d(BwdArgs& f, cudaStream_t s)
     constexpr bool half = is_half<T>;
     // As rows of a product (128 a tile) and as columns (64 a tile).
     CUtensorMap q_rows, g_rows, k_cols, v_cols, k_rows, v_rows, q_cols, g_cols;
-    const cudaError_t bad = cudaErrorInvalidValue;
     cudaError_t e = attention_bind_context();
     if (e != cudaSuccess) return e;
-    if (a.N > 0 && a.M > 0) {
-        if (!attention_tile_map(&q_rows, half, a.q, a.qs, a.B, a.N, a.Hq, a.d, kTile) ||
-            !attention_tile_map(&g_rows, half, a.dout, a.gs, a.B, a.N, a.Hq, a.d, kTile) ||
-            !attention_tile_map(&k_cols, half, a.k, a.ks, a.B, a.M, a.Hkv, a.d, kCols) ||
-            !attention_tile_map(&v_cols, half, a.v, a.vs, a.B, a.M, a.Hkv, a.d, kCols) ||
-            !attention_tile_map(&k_rows, half, a.k, a.ks, a.B, a.M, a.Hkv, a.d, kTile) ||
-            !attention_tile_map(&v_rows, half, a.v, a.vs, a.B, a.M, a.Hkv, a.d, kTile) ||
-            !attention_tile_map(&q_cols, half, a.q, a.qs, a.B, a.N, a.Hq, a.d, kCols) ||
-            !attention_tile_map(&g_cols, half, a.dout, a.gs, a.B, a.N, a.Hq, a.d, kCols))
-            return bad;
-    }
+    if (!attention_tile_map(&q_rows, half, a.q, a.qs, a.B, a.N, a.Hq, a.d, kTile) ||
+        !attention_tile_map(&g_rows, half, a.dout, a.gs, a.B, a.N, a.Hq, a.d, kTile) ||
+        !attention_tile_map(&k_cols, half, a.k, a.ks, a.B, a.M, a.Hkv, a.d, kCols) ||
+        !attention_tile_map(&v_cols, half, a.v, a.vs, a.B, a.M, a.Hkv, a.d, kCols) ||
+        !attention_tile_map(&k_rows, half, a.k, a.ks, a.B, a.M, a.Hkv, a.d, kTile) ||
+        !attention_tile_map(&v_rows, half, a.v, a.vs, a.B, a.M, a.Hkv, a.d, kTile) ||
+        !attention_tile_map(&q_cols, half, a.q, a.qs, a.B, a.N, a.Hq, a.d, kCols) ||
+        !attention_tile_map(&g_cols, half, a.dout, a.gs, a.B, a.N, a.Hq, a.d, kCols))
+        return cudaErrorInvalidValue;
     static std::atomic<bool> allowed[3][128];
     const bool tail = DPAD == 64 && a.d <= 32;
     const auto dq = tail ? attend_dq_tc_kernel<T, DPAD, DPAD == 64> : attend_dq_tc_kernel<T, DPAD, false>;

@@ -78,6 +78,18 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x)
     return __float2bfloat16_rn(x);
 }
 
+// Two 16-bit numbers in a word.
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half)
+{
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16)
+{
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 // V elements moved as one access of V * sizeof(T) bytes (16 at most, aligned to that size).
 template <typename T, int V>
 struct alignas(V * sizeof(T)) Vec {

@@ -225,22 +225,5 @@ __device__ __forceinline__ void settle(uint32_t (&r)[N])
     for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
 
-__device__ __forceinline__ void settle32(uint32_t* r)
-{
-#pragma unroll
-    for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
-}
-
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half)
-{
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16)
-{
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 }  // namespace tc
 }  // namespace sdtw
