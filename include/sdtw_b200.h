@@ -272,12 +272,15 @@ sdtw_status sdtw_grad_dist(sdtw_dtype dtype, int kind, const void* X, const void
 /* ---------------------------------------------------------------------------------------------------
  * Operators of a sequence model that trains under the loss. They take SDTW_F32, SDTW_F16 and SDTW_BF16 (the
  * gradient norm SDTW_F64 too); sums, softmax statistics and norms are kept in 32 bits or more, and an output
- * is rounded to its type once.
+ * is rounded to its type once. What else is held in fewer bits than 32: with 16-bit types the weights P as operand of P v and
+ * P^T dout, and dS = P (dP - delta) as operand of dS k and dS^T q (rounded to the type once, fp16 scaled against under- and overflow;
+ * for dq of d <= 32 what that rounding dropped is multiplied too); with SDTW_F32 a product is that of an 11-bit head and tail of each
+ * factor without tail times tail (2^-22 of it); cos and sin of the rotation of 16-bit x are off by up to 2^-21.
  *
  * Cross attention: N queries of a sample attend to the M states of another series.
  *   s_ij = scale q_i . k_j,  p_i = softmax of s_ij over the cells of row i,  out_i = sum_j p_ij v_j
  * The cells of row i < nx are the columns of sdtw_band_row_range(i, nx, ny, bandwidth) (all of [0, ny) with
- * bandwidth < 0), nx = lengths_x[b], ny = lengths_y[b]. Rows i >= nx, and every row when ny = 0, come out as
+ * bandwidth < 0), nx = lengths_x[b], ny = lengths_y[b] (so a single row has no band). Rows i >= nx, and every row when ny = 0, come out as
  * zeros and have no gradient. q (B, N, Hq, d), k and v (B, M, Hkv, d) have any strides (in elements; batch,
  * row, head) with neighbouring features; query head h reads key head h / (Hq / Hkv). 1 <= d <= 128. Rows of
  * q, k and v past the lengths are not used and may hold anything, NaN included; a NaN or infinity inside the

@@ -61,6 +61,14 @@ def cross_attention(
     ``(lengths_x[b] - 1, lengths_y[b] - 1)``. Differentiable in q, k and v (once). One query row a sample (N = 1, a
     decoded token) up to long series run through the same call; with few rows the states are split over the GPU.
 
+    The band lies between the two series *of the call*, as in the loss: a series of one row has no diagonal, and its row spans all
+    states whatever the band. A row that is decoded alone out of a longer, banded series is therefore called without a band
+    on the states of its interval, ``cross_attention(q[:, i:i + 1], k[:, lo:hi], v[:, lo:hi])``.
+
+    Scores, softmax statistics and sums are held in 32 bits. 16-bit operands: the weights, and in the gradients dS (see the
+    header of the C ABI), are rounded to the operands' type once for their product, so that results are off by up to 1.5 times
+    their own rounding. float32: products of an 11-bit head and tail each, without tail times tail (2^-22 a product).
+
     Args:
         q: (B, N, Hq, d) queries, float16, bfloat16 or float32; any strides.
         k: (B, M, Hkv, d) keys. Hq is a multiple of Hkv: query head h reads head ``h // (Hq // Hkv)``.
@@ -111,7 +119,8 @@ def norm_rotate(
         eps: floor of the mean square.
 
     Returns:
-        y: (B, N, H, d), contiguous, in x's dtype. Differentiable in x and weight (once).
+        y: (B, N, H, d), contiguous, in x's dtype. Differentiable in x and weight (once). Norms, products and sums are held in
+        32 bits, angles in 64; cos and sin of 16-bit x are the hardware's (off by 2^-21 at most).
     """
     if rotary_dim is None:
         rotary_dim = x.shape[-1] // 2 * 2 if x.dim() > 0 else 0

@@ -240,7 +240,8 @@ template <int V, bool GRAD>
 constexpr int kCtasPerSm = V == 8 || GRAD ? 2 : 3;
 
 // cos and sin of `turns` whole turns, |turns| <= 1/2. 16-bit results: the hardware's functions, off by at most 2^-21 on
-// [-pi, pi], far below half a step.
+// [-pi, pi], far below half a step of y and dx. A float32 dweight of 16-bit x takes them too: its sums over tokens are held in
+// 32 bits a lane and carry as much (the full functions in the gradient: 128 us instead of 121, 8 x 4097 x 13 x 96 fp16).
 template <typename T>
 __device__ __forceinline__ void cos_sin(float turns, float& c, float& s)
 {
