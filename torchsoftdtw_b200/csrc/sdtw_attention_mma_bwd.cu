@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kThreads, Geom<T, DPAD>::CTAS) attend_backward
     const T* r2p = static_cast<const T*>(KV ? a.v : a.dout) + b * r2s.b + hr * r2s.h;
     float gscale = 1.f;  // of dS: here for all states of the CTA, in dq a row's own
     if (is_half<T> && KV && c1 > c0)
-        gscale = half_scale(bound_of(bound_part(a, b, hk, c0, c1, row0, row0 + kRows < nr ? row0 + kRows : nr)));
+        gscale = half_scale(gradient_bound(a, b, hk, c0, c1, row0, row0 + kRows < nr ? row0 + kRows : nr));
     const float cf = gscale * kUnshift;
 
     const auto load_tile = [&](int t) {
@@ -131,8 +131,8 @@ __global__ void __launch_bounds__(kThreads, Geom<T, DPAD>::CTAS) attend_backward
     }
     if (steps > 0) load_tile(0);
     cp_async_commit();
-    float v_top = 0.f;  // the largest |v| of the CTA's states
-    if (is_half<T> && !KV && c1 > c0) v_top = value_part(a, b, hk, c0, c1);
+    PeakPart v_part{};  // of the largest |v| of the CTA's states
+    if (is_half<T> && !KV && c1 > c0) v_part = value_part(a, b, hk, c0, c1);
     if constexpr (!KV) {
         // delta and |do|^2 of this warp's rows.
         float top_delta = 0.f, top_norm = 0.f;
@@ -163,7 +163,8 @@ __global__ void __launch_bounds__(kThreads, Geom<T, DPAD>::CTAS) attend_backward
         __syncwarp();
     }
     float r_bias[2], r_delta[2], r_scale[2], r_cf[2];  // dq: of this thread's rows
-    if constexpr (is_half<T> && !KV) v_top = warp_maxf(v_top);
+    float v_top = 0.f;
+    if constexpr (is_half<T> && !KV) v_top = peak_of(v_part);
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
         const int r = warp * 16 + (lane >> 2) + 8 * x;

@@ -16,36 +16,39 @@ namespace sdtw {
 constexpr float kHalfShift = 14.f;             // log2 of what fp16 P is kept larger by in the gradients
 constexpr float kHalfUnshift = 0x1p-14f;
 
-// A lane's part of the largest of p[first .. last] (numbers that are not negative). Joined over the warp (warp_maxf) where it is
-// used, so that the load runs beside what comes between.
-__device__ __forceinline__ float peak_part(const float* p, int64_t first, int64_t last)
+// A lane's part of the largest of p[first .. last] (numbers that are not negative). Joined over the warp where it is used, so
+// that the loads run beside what comes between.
+struct PeakPart {
+    float m[2];
+};
+__device__ __forceinline__ PeakPart peak_part(const float* p, int64_t first, int64_t last)
 {
+    PeakPart r;
     int64_t i = first + (threadIdx.x & 31);
-    float m = i <= last ? p[i] : 0.f;
-    for (i += 32; i <= last; i += 32) m = fmaxf(m, p[i]);
-    return m;
+    r.m[0] = i <= last ? p[i] : 0.f;
+    r.m[1] = i + 32 <= last ? p[i + 32] : 0.f;
+    for (i += 64; i <= last; i += 32) r.m[0] = fmaxf(r.m[0], p[i]);
+    return r;
+}
+// (As integers, whose order is that of the numbers: one instruction.)
+__device__ __forceinline__ float peak_of(const PeakPart& p)
+{
+    return __uint_as_float(__reduce_max_sync(kFull, __float_as_uint(fmaxf(p.m[0], p.m[1]))));
 }
 // Of the |v| of states [lo, hi) of key head (b, hk), hi > lo.
-__device__ __forceinline__ float value_part(const AttnArgs& a, int64_t b, int64_t hk, int64_t lo, int64_t hi)
+__device__ __forceinline__ PeakPart value_part(const AttnArgs& a, int64_t b, int64_t hk, int64_t lo, int64_t hi)
 {
     return peak_part(a.v_peak + (b * a.Hkv + hk) * a.v_blocks, lo / kPeakRows, (hi - 1) / kPeakRows);
 }
-// Of the bound on |dP - delta| between queries [q0, q1) (of all query heads) and states [j0, j1) of key head (b, hk), neither empty.
-struct BoundPart {
-    float v, norm2, delta;
-};
-__device__ __forceinline__ BoundPart bound_part(const AttnArgs& a, int64_t b, int64_t hk, int64_t q0, int64_t q1, int64_t j0, int64_t j1)
+// The bound on |dP - delta| between queries [q0, q1) (of all query heads) and states [j0, j1) of key head (b, hk), neither empty.
+__device__ __forceinline__ float gradient_bound(const AttnArgs& a, int64_t b, int64_t hk, int64_t q0, int64_t q1, int64_t j0,
+                                                int64_t j1)
 {
     const int64_t at = (b * a.Hkv + hk) * a.q_blocks;
-    BoundPart p;
-    p.v = value_part(a, b, hk, j0, j1);
-    p.norm2 = peak_part(a.do_peak + at, q0 / kPeakRows, (q1 - 1) / kPeakRows);
-    p.delta = peak_part(a.delta_peak + at, q0 / kPeakRows, (q1 - 1) / kPeakRows);
-    return p;
-}
-__device__ __forceinline__ float bound_of(const BoundPart& p)
-{
-    return fmaf(sqrtf(warp_maxf(p.norm2)), warp_maxf(p.v), warp_maxf(p.delta));
+    const PeakPart v = value_part(a, b, hk, j0, j1);
+    const PeakPart norm2 = peak_part(a.do_peak + at, q0 / kPeakRows, (q1 - 1) / kPeakRows);
+    const PeakPart delta = peak_part(a.delta_peak + at, q0 / kPeakRows, (q1 - 1) / kPeakRows);
+    return fmaf(sqrtf(peak_of(norm2)), peak_of(v), peak_of(delta));
 }
 // Takes the largest |do|^2 and |delta| of some queries of one 64-row block into its maxima.
 __device__ __forceinline__ void raise_gradient_peak(const AttnArgs& a, int64_t b, int64_t hk, int64_t i, float norm2, float delta)

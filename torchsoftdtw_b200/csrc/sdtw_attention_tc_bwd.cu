@@ -357,11 +357,11 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
         // delta and |do|^2 of the tile's rows: LPR lanes a row, all loads ahead of the sums (rows and features outside read a
         // place inside, and count as zero).
         constexpr int LPR = DPAD / 8, RPW = 32 / LPR, ROUNDS = kTile / (G::ELEM_WARPS * RPW);
-        float v_top = 0.f;  // fp16: the largest |v| of the tile's states
+        PeakPart v_part{};  // fp16: of the largest |v| of the tile's states
         if (n > 0) {
             if constexpr (is_half<T>) {
                 const int64_t end = static_cast<int64_t>(ja + n) * kCols;
-                v_top = value_part(a, b, hk, static_cast<int64_t>(ja) * kCols, end < ny ? end : ny);
+                v_part = value_part(a, b, hk, static_cast<int64_t>(ja) * kCols, end < ny ? end : ny);
             }
             Vec<T, 8> g[ROUNDS], o[ROUNDS], lo[ROUNDS];
             const int c = lane % LPR * 8 < a.d ? lane % LPR * 8 : 0;
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
         const uint32_t ts = tmem + lanes + x * BUF_COLS + 32 * half, tdp = ts + DP_COL;
         const uint32_t tds = tmem + lanes + x * BUF_COLS + DS_COL + 16 * half;
-        float gscale = 1.f;
+        float cf = 1.f;  // of dP and delta: the scale of dS, less the shift of P
         if (is_half<T> && n > 0) {
             if (warp < kTile / kPeakRows) {
                 const int r1 = warp * kPeakRows + lane;
@@ -414,9 +414,8 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
                 const float top = warp_maxf(fmaxf(fabsf(s_delta[r1]), fabsf(s_delta[r1 + 32])));
                 if (lane == 0 && row0 + warp * kPeakRows < nx) raise_gradient_peak(a, b, hk, row0 + warp * kPeakRows, norm2, top);
             }
-            gscale = half_scale(fmaf(sqrtf(s_norm[r]), warp_maxf(v_top), fabsf(s_delta[r])));
+            cf = half_scale(fmaf(sqrtf(s_norm[r]), peak_of(v_part), fabsf(s_delta[r]))) * kHalfUnshift;
         }
-        const float cf = gscale * kPUnshift<T>;
         const float delta = s_delta[r] * cf, bias = kPShift<T> - lse;
         bool ok = true;
         for (int it = x; it < n; it += G::BUFS) {
@@ -476,7 +475,7 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
         const int64_t i0 = row0 + 32 * (warp & 3);
         if (x == 0)
             store_rows<T, DPAD>(tmem + lanes + ACC_COL, reinterpret_cast<uint4*>(sm) + (warp & 3) * 32 * (DPAD / 8), lane, half,
-                            2 + (warp & 3), n > 0 && ok, width > 0, !ok, a.scale / gscale, f.dn, a.d,
+                            2 + (warp & 3), n > 0 && ok, width > 0, !ok, a.scale * kPUnshift<T> / cf, f.dn, a.d,
                             static_cast<T*>(a.dq) + ((static_cast<int64_t>(b) * a.N + i0) * a.Hq + h) * a.d,
                             static_cast<int64_t>(a.Hq) * a.d, a.N - i0);
         fence_before();
@@ -553,16 +552,18 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
     const int ia = static_cast<int>(*reinterpret_cast<volatile uint32_t*>(misc + 2));
     const int nq = static_cast<int>(*reinterpret_cast<volatile uint32_t*>(misc + 3)) - ia;  // tiles a query head
     const int n = nq > 0 ? nq * a.group : 0;
-    // fp16: one power of two for all rows that share the sums.
-    BoundPart part{};
+    // fp16: one power of two for all rows that share the sums. (Formed by the warps apart, beside the first loads: 5% slower, for
+    // the elementwise loop's registers.)
+    float cf = 1.f;
     if (is_half<T> && n > 0) {
         const int64_t end = static_cast<int64_t>(ia + nq) * kCols;
-        part = bound_part(a, b, hk, static_cast<int64_t>(ia) * kCols, end < nx ? end : nx, row0, row0 + kTile < ny ? row0 + kTile : ny);
+        const float bound_s = gradient_bound(a, b, hk, static_cast<int64_t>(ia) * kCols, end < nx ? end : nx, row0,
+                                             row0 + kTile < ny ? row0 + kTile : ny);
+        cf = half_scale(bound_s) * kHalfUnshift;
     }
 
     if (warp == G::TMA_WARP) {
         int head = hk * a.group, tile = -1;  // of the step that coords() was last asked for
-        float cf = is_half<T> ? 0.f : 1.f;   // formed behind the row tiles' loads
         load_tiles<DPAD>(
             sm, base, &mk, &mv, &mq, &mg, row0, hk, b, n, nx, a.N, row_full, fix, full, empty, bound, lane,
             [&](int, int& c0, int& hd) {
@@ -577,7 +578,6 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
                 const int i0 = (ia + tile) * kCols;
                 const int64_t at = (static_cast<int64_t>(b) * a.Hq + head) * a.N + i0;
                 float* st = stats + stage * 2 * kCols;
-                if (is_half<T> && cf == 0.f) cf = half_scale(bound_of(part)) * kPUnshift<T>;
 #pragma unroll
                 for (int c = lane; c < kCols; c += 32) {
                     const bool on = i0 + c < nx;  // a query past the length has P = 2^-inf = 0
@@ -660,7 +660,6 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
         const int64_t j = row0 + 32 * (warp & 3) + lane;
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
         const uint32_t ts = tmem + lanes + x * BUF_COLS + 32 * half, tdp = ts + DP_COL;
-        const float gscale = is_half<T> ? half_scale(bound_of(part)) : 1.f, cf = gscale * kPUnshift<T>;
         int64_t lo = 0, hi = 0;
         if (j < ny && nx > 0) column_cells(a, j, nx, ny, lo, hi);
         const int ilo = static_cast<int>(lo), width = static_cast<int>(hi - lo);
@@ -736,7 +735,7 @@ __global__ void __launch_bounds__(Geom<DPAD>::THREADS, Geom<DPAD>::CTAS)
         uint4* rows = reinterpret_cast<uint4*>(sm) + (warp & 3) * 32 * (DPAD / 8);
         const bool any = n > 0 && ok;
         if (x == 0)
-            store_rows<T, DPAD>(tmem + lanes + DK_COL, rows, lane, half, 2 + (warp & 3), any, width > 0, !ok, a.scale / gscale, f.dn,
+            store_rows<T, DPAD>(tmem + lanes + DK_COL, rows, lane, half, 2 + (warp & 3), any, width > 0, !ok, a.scale * kPUnshift<T> / cf, f.dn,
                                 a.d, static_cast<T*>(a.dk) + at, pitch, a.M - j0);
         if (x == G::BUFS - 1)
             store_rows<T, DPAD>(tmem + lanes + DV_COL, rows + G::ROW_BYTES / 16, lane, half, 6 + (warp & 3), any, width > 0, !ok,
