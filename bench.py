@@ -149,12 +149,18 @@ class ClockSampler:
 # The reference's CPU path (timed baseline and reference arm). Only the oracle is loaded here: the
 # reference's compiled CPU operator (oracle/_ref) under its module glue, restated in oracle/oracle.py.
 # ---------------------------------------------------------------------------------------------------
+class ReferenceUnavailable(Exception):
+    """The reference's compiled CPU operator is not there and cannot be built (its sources are absent)."""
+
+
 def cpu_reference_measure(w, sample_pairs: int, steps: int, warmup: int, min_seconds: float = 0.0):
     """Cells/s of the reference CPU path on `sample_pairs` pairs of the workload, all host threads."""
     from oracle import oracle as O
 
     if not O.ref_available():
         O.build()
+    if not O.ref_available():
+        raise ReferenceUnavailable("the reference's CPU operator is not built (oracle/_ref) and its sources are absent")
     O.load_ref()
     threads = os.cpu_count() or 1
     torch.set_num_threads(threads)
@@ -182,7 +188,11 @@ def run_reference_arm(args, w, rank, world):
     if rank != 0:
         return
     sample = args.cpu_sample
-    r = cpu_reference_measure(w, sample, max(args.steps, 1), max(args.warmup, 1))
+    try:
+        r = cpu_reference_measure(w, sample, max(args.steps, 1), max(args.warmup, 1))
+    except ReferenceUnavailable as e:
+        print(json.dumps({"impl": "reference", "unavailable": str(e)}), flush=True)
+        return
     line = {
         "impl": "reference", "metric": metric_name(w), "value": r["value"], "unit": "cells/s",
         "n_gpus": world, "steps": args.steps, "warmup": args.warmup, "ms_per_step": r["s_per_step"] * 1e3,
@@ -509,8 +519,11 @@ def main():
                               "per_kernel_ms": kt}
         result["clocks"] = clocks
         if not args.no_cpu_baseline and world == 1:
-            r = cpu_reference_measure(w, args.cpu_sample, 2, 1, min_seconds=10.0)
-            result["cpu_baseline"] = {k: r[k] for k in ("value", "unit", "cores", "kind", "sample")}
+            try:
+                r = cpu_reference_measure(w, args.cpu_sample, 2, 1, min_seconds=10.0)
+                result["cpu_baseline"] = {k: r[k] for k in ("value", "unit", "cores", "kind", "sample")}
+            except ReferenceUnavailable as e:
+                result["cpu_baseline"] = {"unavailable": str(e)}
         print(json.dumps(result), flush=True)
     if world > 1:
         dist.destroy_process_group()
