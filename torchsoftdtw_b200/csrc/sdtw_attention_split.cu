@@ -11,7 +11,8 @@
 // (a single sequence of few heads) leave partial sums in the workspace for a second launch. Both join in split order.
 //
 // Memory bound with few rows: 16 x 1 x 32771 x 32/8 x 128 bf16 379 us, 5.65 TB/s of 6.55 measured for a copy (two splits a head;
-// three to eight 393 to 500 us). Short caches are bound by launch and latency: 8 x 1 x 512 x 8 x 64 10 us a call. float32 with
+// three to eight 393 to 500 us). Short caches are bound by launch and latency: 8 x 1 x 512 x 8 x 64 10 us a call. A token's float32
+// cache is read at 2.86 TB/s (1.51 ms for the same sizes): its operands are split for a product of 16 rows. float32 with
 // many rows is bound by the instructions that split operands: 64 x 256 x 192 x 4 x 32, band 32, 49 us; 2 x 2048 x 2048 x 8 x 128
 // 0.98 ms, 35 TFLOP/s (3 x 35 on the matrix pipe).
 #include "sdtw_attention_mma.cuh"

@@ -8,13 +8,14 @@
 //     as K). A row tile has two S buffers, so that the scores of the next state tile are there when a softmax ends;
 //   * one TMA warp: Q once, then K and V tiles through a ring.
 // The running maximum m is only raised, and O rescaled, when a row's scores outgrow it by 2^8: P stays below 2^8
-// until then, and the final division by the row's sum makes it exact. So a tile's weights are formed at once with the m of
+// until then, and the final division by the row's sum makes it exact. (P is rounded to the operands' type for its product, which leaves
+// out off by 1.1 to 1.5 times its own rounding; its sum is that of the 32-bit weights.) So a tile's weights are formed at once with the m of
 // the tile before, beside its maximum, and formed again in the rare case that the maximum has outgrown it; the two threads
 // of a row only have to agree on that, which one barrier with an OR does.
 //
 // Bound by the chain of a softmax step (wait, load of S, exponentials, meeting of a row's two threads, store of P), which two
-// row tiles an SM, each with scores in hand, overlap in part: 2 x 4096 x 4096 x 16 x 128 bf16 270 us, 1020 TFLOP/s of 1718
-// measured for a plain product; 4 x 4096 x 4096 x 16 x 64 418 us, 658 TFLOP/s. Tiles of 64 states: S and O of two row tiles with
+// row tiles an SM, each with scores in hand, overlap in part: 2 x 4096 x 4096 x 16 x 128 bf16 270 us alone, 1020 TFLOP/s of 1718
+// measured for a plain product, and 300 us (917) among others; 4 x 4096 x 4096 x 16 x 64 430 us, 640 TFLOP/s. Tiles of 64 states: S and O of two row tiles with
 // two S buffers each fill tensor memory (d = 128). Exponentials as polynomials on the FMA pipe, an eighth to a half of them:
 // no gain. Short series are bound by a CTA's start and end: 32 x 512 x 512 x 8 x 64 49 us, 350 TFLOP/s.
 #include <mutex>

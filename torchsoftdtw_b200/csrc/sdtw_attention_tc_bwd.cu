@@ -4,14 +4,14 @@
 //   dq = scale dS K;   dv = P^T dO,  dk = scale dS^T Q  (S^T = K Q^T and dP^T = V dO^T directly, states as rows)
 // Seven products where one launch with atomic sums of dq would take five: the price of sums in one fixed order.
 // P and dS go to tensor memory as the 16-bit A operand of the next product, so nothing of size queries x states leaves
-// the SM. A CTA keeps 128 rows (of Q and dO, or of K and V) and streams 64 columns (of the other two) at a time; eight
+// the SM. (Rounded once: gradients are off by 1.1 to 1.5 times their own rounding.) A CTA keeps 128 rows (of Q and dO, or of K and V) and streams 64 columns (of the other two) at a time; eight
 // elementwise warps take a tile, two threads a row, 32 columns each. Products complete in no promised order among themselves,
 // so whatever one of them reads is only overwritten when it has been awaited. To have work for the tensor core meanwhile, two
 // tiles are in flight on an SM: of two CTAs (d <= 64), or of one that has two groups of elementwise warps and two sets of S and
 // dP in tensor memory, for the even and the odd tiles (BUFS = 2).
 //
 // Bound, like the forward, by the elementwise step between products: 2 x 4096 x 4096 x 16 x 128 bf16 960 us (1000 TFLOP/s
-// of the seven products), 4 x 4096 x 4096 x 16 x 64 1023 us, 32 x 512 x 512 x 8 x 64 120 us, where the CTAs' first loads,
+// of the seven products; fp16 1007), 4 x 4096 x 4096 x 16 x 64 1060 us, 32 x 512 x 512 x 8 x 64 124 us (fp16 138), where the CTAs' first loads,
 // of all SMs at once, take a third of the time. Sums of the tile before placed between S and dP: 10% slower.
 //
 // fp16: P is kept 2^14 larger and dS scaled by a power of two (a row's own in dq, where a row is a lane; one for the CTA's states in
