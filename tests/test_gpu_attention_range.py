@@ -145,3 +145,25 @@ def test_the_remainder_of_the_output(cuda, d, N, size):
     off = (out.double() + lo.double() * 2.0**-11 - mean).abs() - ((2.0**-22 + 2.0**-23) * mean.abs() + 2.0**-35)
     worst = off.max().item()
     assert worst <= 0
+
+
+@pytest.mark.parametrize("d", [64, 33])
+def test_replayed_on_gradients_of_another_size(cuda, d):
+    """The scale is that of the replay's inputs, not of the capture's: equal bits to an eager call, in any order."""
+    sets = []
+    for size in (1.0, 2.0**-12, 2.0**10):
+        t = [x.half() for x in tensors(2, 150, 170, 4, 2, d, 11)]
+        t[3] = (t[3] * size).half()
+        leaves = [x.clone().requires_grad_(True) for x in t[:3]]
+        sets.append((t, torch.autograd.grad(T.cross_attention(*leaves, bandwidth=20), leaves, t[3])))
+    held = [x.clone() for x in sets[0][0]]
+    leaves = [x.requires_grad_(True) for x in held[:3]]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads = torch.autograd.grad(T.cross_attention(*leaves, bandwidth=20), leaves, held[3])
+    for which in (1, 0, 2, 1):
+        held[3].copy_(sets[which][0][3])
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, want in zip(grads, sets[which][1]):
+            assert torch.equal(got, want)
